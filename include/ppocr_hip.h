@@ -220,6 +220,124 @@ int ppocr_hip_layer_norm(const float *x, const float *w, float *y, size_t rows, 
  * first column holding the maximum (as f32), y[2r+1] = 1 / sum exp(v - max). */
 int ppocr_hip_row_argmax(const float *x, float *y, size_t rows, size_t cols, void *stream);
 
+/* --- Layers of a text decoder on device memory ------------------------------
+ * What a program calls that writes or corrects text token by token after the
+ * recogniser (no reference counterpart: the engine's networks read a line in
+ * one pass). Device pointers and a HIP stream (`stream` NULL = the default
+ * stream of the current device; another device's stream is launched on that
+ * device, to which the pointers then belong). The calls queue their kernels
+ * and return: they never allocate, wait or keep anything, so they may be
+ * captured in a HIP graph and made from several threads. Each returns 0, or
+ * nonzero with the reason in `err`, and then has queued nothing.
+ *
+ * Types are the codes below. Strides count values from one row to the next;
+ * 0 means rows without a gap. Pointers are aligned to their type's size.
+ * Sums, norms, softmax statistics and products are held in 32 bits or more
+ * and rounded once, at the end, to the nearest value of the output's type. */
+enum {
+  PPOCR_F32 = 0,
+  PPOCR_BF16 = 1,
+  PPOCR_F16 = 2,
+  PPOCR_E4M3 = 3, /* 8-bit float, 4 exponent bits, largest 448, no infinity */
+  PPOCR_I8 = 4    /* signed 8-bit integer */
+};
+
+/* Root-mean-square norm over rows of `c` values with the residual's addition:
+ *   h = x + residual, rounded to `type` (h = x where `residual` is NULL),
+ *   y = h / sqrt(mean(h^2) + eps) * weight.
+ * `type` (F32, BF16, F16) is that of x, residual, weight [c] and sum, where h
+ * goes unless it is NULL (it may be x or residual themselves, row for row; y
+ * overlaps nothing). `y_type` is `type`, or E4M3 or I8: then the values of a
+ * row (`group` 0) or of each `group` (32, 64 or 128; the last may be cut off)
+ * share the scale max |y| / 448 or max |y| / 127 in `scales`
+ * [rows][groups, or 1], y is the nearest code of y / scale, and a group of
+ * zeros has scale 0 and codes 0. A group with an infinity or NaN has the
+ * scale NaN (codes 0x7f in E4M3, 0 in I8). Squares are summed in f32: values
+ * past 1e19 overflow the sum and give zeros. */
+int ppocr_hip_rms_norm(const void *x, size_t x_stride, const void *residual, size_t residual_stride,
+                       const void *weight, void *sum, size_t sum_stride, void *y, size_t y_stride, float *scales,
+                       size_t rows, size_t c, int type, int y_type, size_t group, float eps, void *stream, char *err,
+                       size_t err_len);
+
+/* Product of a few rows with 4-bit weights:
+ *   y[i][j] = bias[j] + sum over k of x[i][k] * scales[j][g] * (q[j][k] - zeros[j][g]),  g = k / group,
+ * for `m` rows of x, `n` outputs, `k` inputs. q: n rows of (k + 1) / 2 bytes,
+ * input 2b in the low and 2b + 1 in the high four bits of byte b. `group` is
+ * 32, 64 or 128 (the last may be cut off); scales [n][ceil(k / group)] of
+ * `scale_type` (F32, BF16, F16); zeros of the same shape, one byte each
+ * (0 to 15), NULL = 8; bias [n] of y_type, or NULL. x_type F32, BF16, F16,
+ * E4M3 or I8; 8-bit x has x_scales: [m] (`x_group` 0) or
+ * [m][ceil(k / group)] (`x_group` == group), as ppocr_hip_rms_norm writes
+ * them. y_type F32, BF16 or F16. The weights' integers are multiplied exactly
+ * and scaled in f32. Made for up to 64 rows: more read the weights again for
+ * every 64. An infinity in x gives NaN in its row. */
+int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, size_t x_group, const uint8_t *q,
+                         const void *scales, const uint8_t *zeros, const void *bias, void *y, size_t y_stride,
+                         size_t m, size_t n, size_t k, size_t group, int x_type, int scale_type, int y_type,
+                         void *stream, char *err, size_t err_len);
+
+/* A paged cache of keys and values: `pages` pages of `page_size` tokens of
+ * `heads` heads of `dim` values (up to 256) of `type` (F32, BF16, F16).
+ * Strides count values from page to page, token to token and head to head;
+ * all 0 means [page][token][head][dim] without gaps. A text's tokens lie in
+ * the pages its row of a page table (int32, `table_width` a row) names: token
+ * i in page table[i / page_size], at i % page_size. */
+typedef struct ppocr_kv_cache {
+  void *k, *v;
+  size_t pages, page_size, heads, dim;
+  size_t page_stride, token_stride, head_stride;
+  int type;
+} ppocr_kv_cache;
+
+/* Append new keys and values: text b's are rows starts[b] .. starts[b + 1] - 1
+ * of k and v (`rows` rows of heads x dim; starts NULL: one row a text, rows ==
+ * batch), and go to the last positions below lengths[b], its token count with
+ * them. Tokens whose position is negative or past the table's row, or whose
+ * table entry names no page, and rows past `rows`, are written nowhere. Two
+ * texts that share a page must not append to it in one call. */
+int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_stride, const ppocr_kv_cache *cache,
+                        const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
+                        size_t batch, size_t rows, void *stream, char *err, size_t err_len);
+
+/* Attention of each text's newest token over its cache:
+ *   y[b][h] = sum over i of softmax_i(scale * q[b][h] . k[i][h']) v[i][h'],  h' = h / (heads / cache heads),
+ * for q and y of `batch` rows of heads x dim in the cache's type, over tokens
+ * i < lengths[b]; with `window` > 0 only the last `window` of them and the
+ * first `sinks`. A text of length 0 (or less) gives zeros; one whose length
+ * passes table_width * page_size, or with a seen token in a page that does
+ * not exist, gives NaN. What lies in unseen tokens does not matter.
+ *
+ * `longest` bounds the lengths (0: table_width * page_size); it only guides
+ * how far the cache is split, and longer texts are right too. The parts are
+ * joined in `workspace`, 16-byte aligned, `workspace_bytes` long: as
+ * ppocr_hip_paged_attention_workspace says, or less (NULL, 0 = no split;
+ * slower). It is written and read within the call: calls that may overlap, and
+ * graphs that may run at once, each need their own. Results depend on the
+ * number of parts in their last bits, and on nothing else from call to call. */
+size_t ppocr_hip_paged_attention_workspace(const ppocr_kv_cache *cache, size_t batch, size_t heads, size_t longest);
+int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cache *cache, const int32_t *table,
+                              size_t table_width, const int32_t *lengths, void *y, size_t y_stride, size_t batch,
+                              size_t heads, float scale, size_t window, size_t sinks, size_t longest,
+                              void *workspace, size_t workspace_bytes, void *stream, char *err, size_t err_len);
+
+/* Causal attention of prompts with a sliding window and sinks: text b's
+ * queries are rows starts_q[b] .. starts_q[b + 1] - 1 of q (and y), its keys
+ * and values rows starts_k[b] .. starts_k[b + 1] - 1 of k and v. With nq
+ * queries and nk keys, query i stands at p = nk - nq + i and sees the keys
+ * j <= p with j > p - window (`window` 0: all) or j < sinks; y is as above.
+ * A query that sees no key gives zeros. Rows outside every text are left as
+ * they were. `rows_q`, `rows_k`: the rows there are; starts are int32, not
+ * decreasing, within them (rows past them are not touched). q and y: heads x
+ * dim a row, k and v: kv_heads x dim, dim up to 256, type F32, BF16 or F16.
+ * What lies in keys that a query does not see does not matter to it. In BF16
+ * and F16 the softmax's weights are rounded to the type before the product
+ * with v, as v itself is; their sum is not. */
+int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
+                               size_t v_stride, void *y, size_t y_stride, const int32_t *starts_q,
+                               const int32_t *starts_k, size_t batch, size_t rows_q, size_t rows_k, size_t heads,
+                               size_t kv_heads, size_t dim, int type, float scale, size_t window, size_t sinks,
+                               void *stream, char *err, size_t err_len);
+
 /* --- Host stages either side of the model ---------------------------------
  * CPU code in the same library: the recogniser's text from its [T][2]
  * output, and the detector's text boxes from its probability map. Each

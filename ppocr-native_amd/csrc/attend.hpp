@@ -1,0 +1,270 @@
+// Softmax attention of 16 query rows over keys, a wave's worth, on the matrix
+// cores: shared by the decode attention (the 16 are query heads of one key
+// head) and the prompt attention of any type and dim (16 queries of a head).
+//
+// The rows are the columns of every product, so that a lane holds one row's
+// numbers throughout (column lane % 16) and its running maximum and sum need
+// only two exchanges between the wave's quarters:
+//   S^T[key][row] = K Q^T,   O^T[d][row] += V^T P^T.
+// A 16-key result leaves quarter p with keys 4 p .. 4 p + 3 of its row, which
+// are then what that quarter holds of P^T: the order of the products' inner
+// index is free, so V's rows are loaded to match and P stays where it is.
+// V comes row by row (each lane DP / 16 neighbouring values of a key's row);
+// 16-bit values of two keys are paired by byte permutes.
+#pragma once
+#include "decoder.hpp"
+
+namespace ppocr {
+
+// Loads of `N` of a head's `dim` values at d: whole, or cut off at dim where
+// dims are not EVEN (a multiple of 8). Zeros past dim.
+template <bool EVEN, typename V, int N>
+__device__ __forceinline__ void load_dims(const V *p, int d, int dim, V (&v)[N]) {
+  if constexpr (EVEN) {
+    constexpr int M = N < 8 ? N : 8;
+#pragma unroll
+    for (int i = 0; i < N; i += M) {
+      if (d + i < dim) {
+        __builtin_memcpy(v + i, p + d + i, M * sizeof(V));
+      } else {
+#pragma unroll
+        for (int e = 0; e < M; e++) v[i + e] = V(0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] = V(0);
+      if (d + i < dim) v[i] = p[d + i];
+    }
+  }
+}
+
+template <int T>
+struct Tile;  // T's matrix products
+
+// 16-bit types: 32 keys a tile, inner index 32.
+template <int T>
+struct Tile16 {
+  typedef num_t<T> V;
+  static constexpr int keys = 32;
+  static __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c) {
+    if constexpr (T == PPOCR_F16)
+      return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0,
+                                                    0);
+    else
+      return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0,
+                                                     0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    if constexpr (T == PPOCR_F16)
+      return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2h));
+    else
+      return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
+  }
+  static __device__ __forceinline__ v2f unpack(uint32_t p) {
+    if constexpr (T == PPOCR_F16)
+      return __builtin_convertvector(__builtin_bit_cast(v2h, p), v2f);
+    else
+      return v2f{__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u)};
+  }
+};
+
+// The state of 16 rows over DP (padded) dims.
+template <int T, int DP, bool EVEN>
+struct Attend {
+  typedef num_t<T> V;
+  static constexpr bool F32 = T == PPOCR_F32;
+  static constexpr int KEYS = F32 ? 16 : 32;        // keys a tile
+  static constexpr int H = KEYS / 16;               // 16-key halves
+  static constexpr int QC = F32 ? DP / 16 : DP / 32;  // 16-byte pieces of a row a lane has
+  static constexpr int QN = F32 ? 4 : 8;            // values in one
+  static constexpr int E = DP / 16;                 // values of a V row a lane has
+  V q[QC][QN];
+  v4f o[E];  // O^T: this lane's row, d = E (4 quarter + r) + e
+  float m, l;  // running maximum (of 2-logarithms) and this lane's share of the sum
+
+  __device__ __forceinline__ void start(const V *qrow, int dim, int quarter) {
+#pragma unroll
+    for (int c = 0; c < QC; c++) load_dims<EVEN>(qrow, QN * (4 * c + quarter), dim, q[c]);
+#pragma unroll
+    for (int e = 0; e < E; e++) o[e] = v4f{0, 0, 0, 0};
+    m = -INFINITY;
+    l = 0.0f;
+  }
+
+  // O^T += V^T P^T for one tile, the keys of one column's zero weights
+  // multiplied all the same.
+  __device__ __forceinline__ void add(const V (&v)[H][4][E], const float (&p)[H][4], v4f (&o)[E]) {
+    if constexpr (F32) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][r][e], p[0][r], o[e], 0, 0, 0);
+    } else {
+      // P as a high and a low part of T: the weights keep f32's precision at
+      // twice the products, which memory hides.
+      v4u hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float a = p[i / 2][2 * (i % 2)], b = p[i / 2][2 * (i % 2) + 1];
+        hi[i] = Tile16<T>::pack(a, b);
+        const v2f back = Tile16<T>::unpack(hi[i]);
+        lo[i] = Tile16<T>::pack(a - back[0], b - back[1]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        v4u f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          f[i] = (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2)][e]) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2) + 1][e]) << 16;
+        o[e] = Tile16<T>::mfma(f, lo, o[e]);
+        o[e] = Tile16<T>::mfma(f, hi, o[e]);
+      }
+    }
+  }
+
+  // The same where some row does not see some key and V holds an infinity or
+  // NaN, which a weight of 0 would carry into that row: key by key, kept only
+  // by the rows that see it.
+  template <class Seen>
+  __device__ __noinline__ void add_seen(const V (&v)[H][4][E], const float (&p)[H][4], Seen seen, int quarter) {
+#pragma unroll 1
+    for (int i = 0; i < KEYS; i++) {
+      V vi[H][4][E];
+      float pi[H][4];
+#pragma unroll
+      for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const bool it = 16 * h + 4 * quarter + r == i;
+          pi[h][r] = it ? p[h][r] : 0.0f;
+#pragma unroll
+          for (int e = 0; e < E; e++) vi[h][r][e] = it ? v[h][r][e] : V(0);
+        }
+      v4f more[E];
+#pragma unroll
+      for (int e = 0; e < E; e++) more[e] = v4f{0, 0, 0, 0};
+      add(vi, pi, more);
+      if (seen(i)) {
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] += more[e];
+      }
+    }
+  }
+
+  static __device__ __forceinline__ bool finite(V x) {
+    if constexpr (F32)
+      return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+    else if constexpr (T == PPOCR_BF16)
+      return (__builtin_bit_cast(uint16_t, x) & 0x7f80) != 0x7f80;
+    else
+      return (__builtin_bit_cast(uint16_t, x) & 0x7c00) != 0x7c00;
+  }
+
+  // One tile of keys. RAGGED: the 16 rows do not see the same keys. k_row(key) and v_row(key) give the rows of the tile's
+  // keys 0 .. KEYS - 1, or NULL where no row of the 16 sees the key (nothing
+  // is read there); seen(key) says whether this lane's row does. `masked`
+  // (uniform): not every key of the tile is seen by every row. `scale` is
+  // for 2-logarithms.
+  template <bool RAGGED, class KR, class VR, class Seen>
+  __device__ __forceinline__ void tile(KR k_row, VR v_row, Seen seen, bool masked, int dim, float scale, int lane) {
+    const int col = lane % 16, quarter = lane / 16;
+    V k[H][QC][QN];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+      const V *p = k_row(16 * h + col);
+#pragma unroll
+      for (int c = 0; c < QC; c++) {
+        if (p) {
+          load_dims<EVEN>(p, QN * (4 * c + quarter), dim, k[h][c]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < QN; i++) k[h][c][i] = V(0);
+        }
+      }
+    }
+    V v[H][4][E];
+#pragma unroll
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const V *p = v_row(16 * h + 4 * quarter + r);
+        if (p) {
+          load_dims<EVEN>(p, E * col, dim, v[h][r]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; i++) v[h][r][i] = V(0);
+        }
+      }
+    v4f s[H];
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+      s[h] = v4f{0, 0, 0, 0};
+#pragma unroll
+      for (int c = 0; c < QC; c++) {
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[h][c][j], q[c][j], s[h], 0, 0, 0);
+        } else {
+          v4u a, b;
+          __builtin_memcpy(&a, k[h][c], 16);
+          __builtin_memcpy(&b, q[c], 16);
+          s[h] = Tile16<T>::mfma(a, b, s[h]);
+        }
+      }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        s[h][r] *= scale;
+        if (masked && !seen(16 * h + 4 * quarter + r)) s[h][r] = -INFINITY;
+        top = fmaxf(top, s[h][r]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
+    if (__any(now != m)) {
+      const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+      l *= shrink;
+#pragma unroll
+      for (int e = 0; e < E; e++) o[e] *= shrink;
+      m = now;
+    }
+    float p[H][4];
+#pragma unroll
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        p[h][r] = __builtin_amdgcn_exp2f(s[h][r] - base);
+        l += p[h][r];
+      }
+    if constexpr (RAGGED) {
+      if (masked) {
+        bool all = true;
+#pragma unroll
+        for (int h = 0; h < H; h++)
+#pragma unroll
+          for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int e = 0; e < E; e++) all = all && finite(v[h][r][e]);
+        if (__any(!all)) {
+          add_seen(v, p, seen, quarter);
+          return;
+        }
+      }
+    }
+    add(v, p, o);
+  }
+
+  // The row's whole sum, in all four quarters.
+  __device__ __forceinline__ float total() const {
+    float t = l + __shfl_xor(l, 16);
+    return t + __shfl_xor(t, 32);
+  }
+};
+
+}  // namespace ppocr

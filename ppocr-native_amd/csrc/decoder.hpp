@@ -1,0 +1,145 @@
+// The decoder layers' number types, launch arguments and launchers.
+//
+// A tensor's rows are `*_stride` values apart; types are the codes of
+// include/ppocr_hip.h. Launchers return a hipError_t from the launch; they
+// never synchronise or allocate. Shapes are checked by the C entries
+// (decoder.cpp).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "ppocr_hip.h"
+
+namespace ppocr {
+
+typedef float v2f __attribute__((ext_vector_type(2)));
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+typedef _Float16 v8h __attribute__((ext_vector_type(8)));
+
+// One number type: its values as floats and back (nearest, ties to even).
+template <int T>
+struct Num;
+template <>
+struct Num<PPOCR_F32> {
+  typedef float type;
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <>
+struct Num<PPOCR_BF16> {
+  typedef __bf16 type;
+  static __device__ __forceinline__ float get(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
+};
+template <>
+struct Num<PPOCR_F16> {
+  typedef _Float16 type;
+  static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
+};
+template <int T>
+using num_t = typename Num<T>::type;
+
+// N values at p (any alignment of a value's own size), or the first `have`
+// of them and zeros. Whole vectors are one load: global loads take any
+// alignment here.
+template <typename V, int N>
+__device__ __forceinline__ void load_n(const V *p, long have, V (&v)[N]) {
+  if (have >= N) {
+    __builtin_memcpy(v, p, sizeof v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      v[i] = V(0);
+      if (i < have) v[i] = p[i];
+    }
+  }
+}
+
+template <typename V, int N>
+__device__ __forceinline__ void store_n(V *p, long have, const V (&v)[N]) {
+  if (have >= N) {
+    __builtin_memcpy(p, v, sizeof v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < have) p[i] = v[i];
+  }
+}
+
+struct NormArgs {
+  const void *x, *residual, *weight;
+  void *sum, *y;
+  float *scales;
+  long x_stride, residual_stride, sum_stride, y_stride;
+  long rows;
+  int c, groups, group;  // group: values a scale covers (c: the whole row)
+  float eps;
+};
+hipError_t launch_rms_norm(const NormArgs &a, int type, int y_type, hipStream_t s);
+
+struct Q4Args {
+  const void *x;
+  const float *x_scales;
+  const uint8_t *q;
+  const void *scales;
+  const uint8_t *zeros;
+  const void *bias;
+  void *y;
+  long x_stride, y_stride, x_groups;
+  int m, n, k, group, groups;
+  int x_group;  // 0: one scale a row of x (8-bit x)
+  int scale_type, y_type;
+};
+hipError_t launch_q4_product(const Q4Args &a, int x_type, hipStream_t s);
+
+struct CacheArgs {
+  void *k, *v;
+  long page_stride, token_stride, head_stride;
+  int pages, page_size, heads, dim;
+  const int *table;
+  long table_width;
+  const int *lengths;
+};
+
+struct AppendArgs {
+  CacheArgs c;
+  const void *k, *v;
+  long k_stride, v_stride;
+  const int *starts;  // NULL: one row a text
+  long rows;
+  int batch;
+};
+hipError_t launch_kv_append(const AppendArgs &a, int type, hipStream_t s);
+
+struct PagedArgs {
+  CacheArgs c;
+  const void *q;
+  void *y;
+  long q_stride, y_stride;
+  int batch, heads, splits;
+  int window, sinks;  // window 0: every key is seen
+  float scale;
+  float *part;  // splits > 1: batch x heads x splits rows of dim + 2 floats
+};
+// The parts a text's cache of up to `longest` tokens is split into.
+int paged_splits(int batch, int heads, int kv_heads, int type, long longest);
+hipError_t launch_paged_attention(const PagedArgs &a, int type, hipStream_t s);
+
+struct PromptArgs {
+  const void *q, *k, *v;
+  void *y;
+  const int *starts_q, *starts_k;
+  long q_stride, k_stride, v_stride, y_stride;
+  int batch, rows_q, rows_k, heads, kv_heads, dim;
+  int window, sinks;
+  float scale;
+};
+hipError_t launch_window_attention(const PromptArgs &a, int type, hipStream_t s);
+
+}  // namespace ppocr

@@ -1,0 +1,301 @@
+// Root-mean-square norm with the residual's addition, 16- or 32-bit or 8-bit
+// output (ppocr_hip_rms_norm).
+//
+//   h = round(x + residual),  r = 1 / sqrt(mean(h^2) + eps),  y = h r w
+//
+// One pass over the data: L lanes hold a row in registers (CH runs of V
+// consecutive values a lane, V * size = 16 bytes, run i at (i L + lane) V),
+// so x and residual are read once and sum and y written once: memory bound.
+// The 8-bit forms take the largest |y| of a group as integers of its bits, so
+// that an infinity or NaN wins; a group of 32, 64 or 128 lies in neighbouring
+// lanes of one run.
+#include "decoder.hpp"
+
+namespace ppocr {
+namespace {
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
+  for (int o = lanes >> 1; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  return v;
+}
+
+// The sum (or the largest) over the L lanes of a row; every lane gets it.
+// A row of one wave needs no LDS.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float *lds) {
+  v = wave_sum(v);
+  if constexpr (L > 64) {
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < L / 64; i++) v += lds[i];
+  }
+  return v;
+}
+
+template <int L>
+__device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *lds) {
+  v = lanes_max(v, 64);
+  if constexpr (L > 64) {
+    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int i = 0; i < L / 64; i++) v = max(v, lds[i]);
+  }
+  return v;
+}
+
+constexpr float kTop8[2] = {448.0f, 127.0f};  // E4M3, I8
+
+// A group's scale from the bits of its largest |y|, and what to multiply y
+// with: 0 for a group whose scale would not be a normal number. Not finite:
+// NaN.
+__device__ __forceinline__ float scale8(uint32_t top, int i8, float &inverse) {
+  if (top >= 0x7f800000u) {
+    inverse = 0.0f;
+    return __uint_as_float(0x7fc00000u);
+  }
+  const float s = __uint_as_float(top) / kTop8[i8];
+  inverse = s >= 1.17549435e-38f ? 1.0f / s : 0.0f;
+  return inverse != 0.0f ? s : 0.0f;
+}
+
+// N values to their codes. `scale` NaN: the NaN code (E4M3) or 0 (I8).
+template <int N>
+__device__ __forceinline__ void codes8(const float (&y)[N], float inverse, float scale, int i8, uint8_t (&out)[N]) {
+  const bool bad = scale != scale;
+  if (i8) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const float v = bad ? 0.0f : fminf(fmaxf(y[i] * inverse, -127.0f), 127.0f);
+      out[i] = (uint8_t)(int8_t)(int)rintf(v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      const float a = fminf(fmaxf(y[i] * inverse, -448.0f), 448.0f);
+      const float b = fminf(fmaxf(y[i + 1] * inverse, -448.0f), 448.0f);
+      const int p = bad ? 0x7f7f : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+      out[i] = (uint8_t)p;
+      out[i + 1] = (uint8_t)(p >> 8);
+    }
+  }
+}
+
+// L lanes a row: 64 (four rows a workgroup) or the whole workgroup.
+template <int T, bool Y8, int L, int CH>
+__global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_rows(NormArgs a, int i8) {
+  typedef num_t<T> V;
+  constexpr int N = 16 / sizeof(V);
+  __shared__ float lds[32];
+  __shared__ uint32_t lds_top[32];
+  const int lane = threadIdx.x % L;
+  const long row = (long)blockIdx.x * (L == 64 ? 4 : 1) + (L == 64 ? threadIdx.x / 64 : 0);
+  if (row >= a.rows) return;  // whole waves; only where a row is one wave
+  const V *x = (const V *)a.x + row * a.x_stride;
+  const V *w = (const V *)a.weight;
+  V hv[CH][N], wv[CH][N];
+  float h[CH][N];
+#pragma unroll
+  for (int i = 0; i < CH; i++) load_n(x + (i * L + lane) * N, (long)a.c - (i * L + lane) * N, hv[i]);
+  if (a.residual) {
+    const V *r = (const V *)a.residual + row * a.residual_stride;
+    V rv[CH][N];
+#pragma unroll
+    for (int i = 0; i < CH; i++) load_n(r + (i * L + lane) * N, (long)a.c - (i * L + lane) * N, rv[i]);
+#pragma unroll
+    for (int i = 0; i < CH; i++)
+#pragma unroll
+      for (int e = 0; e < N; e++) hv[i][e] = Num<T>::put(Num<T>::get(hv[i][e]) + Num<T>::get(rv[i][e]));
+  }
+#pragma unroll
+  for (int i = 0; i < CH; i++) load_n(w + (i * L + lane) * N, (long)a.c - (i * L + lane) * N, wv[i]);
+  if (a.sum) {
+    V *s = (V *)a.sum + row * a.sum_stride;
+#pragma unroll
+    for (int i = 0; i < CH; i++) store_n(s + (i * L + lane) * N, (long)a.c - (i * L + lane) * N, hv[i]);
+  }
+  float q = 0.0f;
+#pragma unroll
+  for (int i = 0; i < CH; i++)
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      h[i][e] = Num<T>::get(hv[i][e]);
+      q = fmaf(h[i][e], h[i][e], q);
+    }
+  q = row_sum<L>(q, lds);
+  const float r = 1.0f / sqrtf(q / (float)a.c + a.eps);
+#pragma unroll
+  for (int i = 0; i < CH; i++)
+#pragma unroll
+    for (int e = 0; e < N; e++) h[i][e] = h[i][e] * r * Num<T>::get(wv[i][e]);
+  if constexpr (!Y8) {
+    V *y = (V *)a.y + row * a.y_stride;
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      V o[N];
+#pragma unroll
+      for (int e = 0; e < N; e++) o[e] = Num<T>::put(h[i][e]);
+      store_n(y + (i * L + lane) * N, (long)a.c - (i * L + lane) * N, o);
+    }
+  } else {
+    uint8_t *y = (uint8_t *)a.y + row * a.y_stride;
+    float *scales = a.scales + row * a.groups;
+    uint32_t top[CH], all = 0;
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      top[i] = 0;
+#pragma unroll
+      for (int e = 0; e < N; e++)  // values past the row's end are 0 (or NaN if r or the zeros' product is)
+        if ((i * L + lane) * N + e < a.c) top[i] = max(top[i], __float_as_uint(h[i][e]) & 0x7fffffffu);
+      all = max(all, top[i]);
+    }
+    const bool whole = a.groups == 1;
+    if (whole) all = row_max<L>(all, lds_top);
+#pragma unroll
+    for (int i = 0; i < CH; i++) {
+      const int at = (i * L + lane) * N;
+      float inverse;
+      const float s = scale8(whole ? all : lanes_max(top[i], a.group / N), i8, inverse);
+      if (whole ? i == 0 && lane == 0 : at < a.c && at % a.group == 0) scales[whole ? 0 : at / a.group] = s;
+      uint8_t o[N];
+      codes8(h[i], inverse, s, i8, o);
+      store_n(y + at, (long)a.c - at, o);
+    }
+  }
+}
+
+// Rows too long for registers: 1024 lanes walk the row twice (8-bit rows with
+// one scale: three times), reading h again from sum, or from x and residual.
+template <int T, bool Y8>
+__global__ __launch_bounds__(1024) void rms_norm_long(NormArgs a, int i8) {
+  typedef num_t<T> V;
+  constexpr int N = 16 / sizeof(V), L = 1024;
+  __shared__ float lds[32];
+  __shared__ uint32_t lds_top[32];
+  const long row = blockIdx.x;
+  const V *x = (const V *)a.x + row * a.x_stride;
+  const V *res = a.residual ? (const V *)a.residual + row * a.residual_stride : nullptr;
+  const V *w = (const V *)a.weight;
+  V *sum = a.sum ? (V *)a.sum + row * a.sum_stride : nullptr;
+  const int lane = threadIdx.x, runs = (a.c + L * N - 1) / (L * N);
+  auto load_h = [&](int at, V(&v)[N], bool first) {
+    if (!first && sum) {  // this lane's own stores
+      load_n((const V *)sum + at, (long)a.c - at, v);
+      return;
+    }
+    load_n(x + at, (long)a.c - at, v);
+    if (res) {
+      V rv[N];
+      load_n(res + at, (long)a.c - at, rv);
+#pragma unroll
+      for (int e = 0; e < N; e++) v[e] = Num<T>::put(Num<T>::get(v[e]) + Num<T>::get(rv[e]));
+    }
+  };
+  float q = 0.0f;
+  for (int i = 0; i < runs; i++) {
+    const int at = (i * L + lane) * N;
+    V v[N];
+    load_h(at, v, true);
+    if (sum) store_n(sum + at, (long)a.c - at, v);
+#pragma unroll
+    for (int e = 0; e < N; e++) q = fmaf(Num<T>::get(v[e]), Num<T>::get(v[e]), q);
+  }
+  q = row_sum<L>(q, lds);
+  const float r = 1.0f / sqrtf(q / (float)a.c + a.eps);
+  auto load_y = [&](int at, float(&y)[N]) {
+    V v[N], wv[N];
+    load_h(at, v, false);
+    load_n(w + at, (long)a.c - at, wv);
+#pragma unroll
+    for (int e = 0; e < N; e++) y[e] = Num<T>::get(v[e]) * r * Num<T>::get(wv[e]);
+  };
+  auto top_of = [&](int at, const float(&y)[N]) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int e = 0; e < N; e++)
+      if (at + e < a.c) t = max(t, __float_as_uint(y[e]) & 0x7fffffffu);
+    return t;
+  };
+  uint32_t all = 0;
+  const bool whole = a.groups == 1;
+  if constexpr (Y8) {
+    if (whole) {
+      for (int i = 0; i < runs; i++) {
+        float y[N];
+        load_y((i * L + lane) * N, y);
+        all = max(all, top_of((i * L + lane) * N, y));
+      }
+      all = row_max<L>(all, lds_top);
+    }
+  }
+  for (int i = 0; i < runs; i++) {
+    const int at = (i * L + lane) * N;
+    float y[N];
+    load_y(at, y);
+    if constexpr (!Y8) {
+      V o[N];
+#pragma unroll
+      for (int e = 0; e < N; e++) o[e] = Num<T>::put(y[e]);
+      store_n((V *)a.y + row * a.y_stride + at, (long)a.c - at, o);
+    } else {
+      float inverse;
+      const float s = scale8(whole ? all : lanes_max(top_of(at, y), a.group / N), i8, inverse);
+      float *scales = a.scales + row * a.groups;
+      if (whole ? at == 0 : at < a.c && at % a.group == 0) scales[whole ? 0 : at / a.group] = s;
+      uint8_t o[N];
+      codes8(y, inverse, s, i8, o);
+      store_n((uint8_t *)a.y + row * a.y_stride + at, (long)a.c - at, o);
+    }
+  }
+}
+
+template <int T, bool Y8>
+hipError_t launch(const NormArgs &a, int i8, hipStream_t s) {
+  constexpr int N = 16 / sizeof(num_t<T>);
+  const int vecs = (a.c + N - 1) / N;  // 16-byte vectors a row
+#define NORM(L, CH)                                                                                          \
+  hipLaunchKernelGGL((rms_norm_rows<T, Y8, L, CH>), dim3(unsigned(L == 64 ? (a.rows + 3) / 4 : a.rows)), \
+                     dim3(L < 256 ? 256 : L), 0, s, a, i8)
+  if (vecs <= 64)
+    NORM(64, 1);
+  else if (vecs <= 128)
+    NORM(64, 2);
+  else if (vecs <= 256)
+    NORM(256, 1);
+  else if (vecs <= 512)
+    NORM(256, 2);
+  else if (vecs <= 1024)
+    NORM(256, 4);
+  else if (vecs <= 2048)
+    NORM(1024, 2);
+  else if (vecs <= 4096)
+    NORM(1024, 4);
+  else
+    hipLaunchKernelGGL((rms_norm_long<T, Y8>), dim3(unsigned(a.rows)), dim3(1024), 0, s, a, i8);
+#undef NORM
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rms_norm(const NormArgs &a, int type, int y_type, hipStream_t s) {
+  const bool y8 = y_type == PPOCR_E4M3 || y_type == PPOCR_I8;
+  const int i8 = y_type == PPOCR_I8;
+  switch (type) {
+    case PPOCR_F32: return y8 ? launch<PPOCR_F32, true>(a, i8, s) : launch<PPOCR_F32, false>(a, i8, s);
+    case PPOCR_BF16: return y8 ? launch<PPOCR_BF16, true>(a, i8, s) : launch<PPOCR_BF16, false>(a, i8, s);
+    case PPOCR_F16: return y8 ? launch<PPOCR_F16, true>(a, i8, s) : launch<PPOCR_F16, false>(a, i8, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace ppocr
