@@ -82,76 +82,22 @@ struct Attend {
   static constexpr int E = DP / 16;                 // values of a V row a lane has
   V q[QC][QN];
   v4f o[E];  // O^T: this lane's row, d = E (4 quarter + r) + e
-  float m, l;  // running maximum (of 2-logarithms) and this lane's share of the sum
+  float m, l;  // running maximum of the products and this lane's share of the sum
 
-  __device__ __forceinline__ void start(const V *qrow, int dim, int quarter) {
+  // `turn`: the scale is negative, and q turns its sign instead.
+  __device__ __forceinline__ void start(const V *qrow, int dim, int quarter, bool turn) {
 #pragma unroll
-    for (int c = 0; c < QC; c++) load_dims<EVEN>(qrow, QN * (4 * c + quarter), dim, q[c]);
+    for (int c = 0; c < QC; c++) {
+      load_dims<EVEN>(qrow, QN * (4 * c + quarter), dim, q[c]);
+      if (turn) {
+#pragma unroll
+        for (int i = 0; i < QN; i++) q[c][i] = -q[c][i];
+      }
+    }
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = v4f{0, 0, 0, 0};
     m = -INFINITY;
     l = 0.0f;
-  }
-
-  // O^T += V^T P^T for one tile, the keys of one column's zero weights
-  // multiplied all the same.
-  __device__ __forceinline__ void add(const V (&v)[H][4][E], const float (&p)[H][4], v4f (&o)[E]) {
-    if constexpr (F32) {
-#pragma unroll
-      for (int r = 0; r < 4; r++)
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][r][e], p[0][r], o[e], 0, 0, 0);
-    } else {
-      // P as a high and a low part of T: the weights keep f32's precision at
-      // twice the products, which memory hides.
-      v4u hi, lo;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float a = p[i / 2][2 * (i % 2)], b = p[i / 2][2 * (i % 2) + 1];
-        hi[i] = Tile16<T>::pack(a, b);
-        const v2f back = Tile16<T>::unpack(hi[i]);
-        lo[i] = Tile16<T>::pack(a - back[0], b - back[1]);
-      }
-#pragma unroll
-      for (int e = 0; e < E; e++) {
-        v4u f;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          f[i] = (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2)][e]) |
-                 (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2) + 1][e]) << 16;
-        o[e] = Tile16<T>::mfma(f, lo, o[e]);
-        o[e] = Tile16<T>::mfma(f, hi, o[e]);
-      }
-    }
-  }
-
-  // The same where some row does not see some key and V holds an infinity or
-  // NaN, which a weight of 0 would carry into that row: key by key, kept only
-  // by the rows that see it.
-  template <class Seen>
-  __device__ __noinline__ void add_seen(const V (&v)[H][4][E], const float (&p)[H][4], Seen seen, int quarter) {
-#pragma unroll 1
-    for (int i = 0; i < KEYS; i++) {
-      V vi[H][4][E];
-      float pi[H][4];
-#pragma unroll
-      for (int h = 0; h < H; h++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const bool it = 16 * h + 4 * quarter + r == i;
-          pi[h][r] = it ? p[h][r] : 0.0f;
-#pragma unroll
-          for (int e = 0; e < E; e++) vi[h][r][e] = it ? v[h][r][e] : V(0);
-        }
-      v4f more[E];
-#pragma unroll
-      for (int e = 0; e < E; e++) more[e] = v4f{0, 0, 0, 0};
-      add(vi, pi, more);
-      if (seen(i)) {
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] += more[e];
-      }
-    }
   }
 
   static __device__ __forceinline__ bool finite(V x) {
@@ -163,13 +109,15 @@ struct Attend {
       return (__builtin_bit_cast(uint16_t, x) & 0x7c00) != 0x7c00;
   }
 
-  // One tile of keys. RAGGED: the 16 rows do not see the same keys. k_row(key) and v_row(key) give the rows of the tile's
+  // One tile of keys. k_row(key) and v_row(key) give the rows of the tile's
   // keys 0 .. KEYS - 1, or NULL where no row of the 16 sees the key (nothing
   // is read there); seen(key) says whether this lane's row does. `masked`
-  // (uniform): not every key of the tile is seen by every row. `scale` is
-  // for 2-logarithms.
+  // (uniform): not every key of the tile is seen by every row. `scale`: of
+  // 2-logarithms, positive. RAGGED: the 16 rows do not see the same keys; the
+  // result says whether this lane met an infinity or NaN in V in such a tile,
+  // which a weight of 0 carries into the rows that do not see it.
   template <bool RAGGED, class KR, class VR, class Seen>
-  __device__ __forceinline__ void tile(KR k_row, VR v_row, Seen seen, bool masked, int dim, float scale, int lane) {
+  __device__ __forceinline__ bool tile(KR k_row, VR v_row, Seen seen, bool masked, int dim, float scale, int lane) {
     const int col = lane % 16, quarter = lane / 16;
     V k[H][QC][QN];
 #pragma unroll
@@ -220,15 +168,14 @@ struct Attend {
     for (int h = 0; h < H; h++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        s[h][r] *= scale;
         if (masked && !seen(16 * h + 4 * quarter + r)) s[h][r] = -INFINITY;
         top = fmaxf(top, s[h][r]);
       }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
+    const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now * scale;
     if (__any(now != m)) {
-      const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - base);
+      const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * scale);
       l *= shrink;
 #pragma unroll
       for (int e = 0; e < E; e++) o[e] *= shrink;
@@ -239,25 +186,48 @@ struct Attend {
     for (int h = 0; h < H; h++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        p[h][r] = __builtin_amdgcn_exp2f(s[h][r] - base);
+        p[h][r] = __builtin_amdgcn_exp2f(fmaf(s[h][r], scale, -base));
         l += p[h][r];
       }
+    bool bad = false;
     if constexpr (RAGGED) {
       if (masked) {
-        bool all = true;
 #pragma unroll
         for (int h = 0; h < H; h++)
 #pragma unroll
           for (int r = 0; r < 4; r++)
 #pragma unroll
-            for (int e = 0; e < E; e++) all = all && finite(v[h][r][e]);
-        if (__any(!all)) {
-          add_seen(v, p, seen, quarter);
-          return;
-        }
+            for (int e = 0; e < E; e++) bad |= !finite(v[h][r][e]);
       }
     }
-    add(v, p, o);
+    if constexpr (F32) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][r][e], p[0][r], o[e], 0, 0, 0);
+    } else {
+      // P as a high and a low part of T: the weights keep f32's precision at
+      // twice the products, which memory hides.
+      v4u hi, lo;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const float x = p[i / 2][2 * (i % 2)], y = p[i / 2][2 * (i % 2) + 1];
+        hi[i] = Tile16<T>::pack(x, y);
+        const v2f back = Tile16<T>::unpack(hi[i]);
+        lo[i] = Tile16<T>::pack(x - back[0], y - back[1]);
+      }
+#pragma unroll
+      for (int e = 0; e < E; e++) {
+        v4u f;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          f[i] = (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2)][e]) |
+                 (uint32_t)__builtin_bit_cast(uint16_t, v[i / 2][2 * (i % 2) + 1][e]) << 16;
+        o[e] = Tile16<T>::mfma(f, lo, o[e]);
+        o[e] = Tile16<T>::mfma(f, hi, o[e]);
+      }
+    }
+    return bad;
   }
 
   // The row's whole sum, in all four quarters.

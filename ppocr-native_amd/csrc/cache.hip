@@ -98,7 +98,8 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a
   __syncthreads();
 
   A at;
-  at.start((const V *)a.q + b * a.q_stride + (long)(h0 + min(col, rows - 1)) * a.c.dim, a.c.dim, quarter);
+  at.start((const V *)a.q + b * a.q_stride + (long)(h0 + min(col, rows - 1)) * a.c.dim, a.c.dim, quarter,
+           a.turn);
   const int *table = a.c.table + b * a.c.table_width;
   const V *ck = (const V *)a.c.k + kv * a.c.head_stride, *cv = (const V *)a.c.v + kv * a.c.head_stride;
   bool bad = false;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a
     for (int w = 0; w < kWaves; w++) m = fmaxf(m, lds_m[w][row]);
 #pragma unroll
     for (int w = 0; w < kWaves; w++) {
-      const float f = lds_m[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lds_m[w][row] - m);
+      const float f = lds_m[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((lds_m[w][row] - m) * a.scale);
       sum += f * lds_l[w][row];
       o += f * lds_o[w][row][d];
     }
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(64) void paged_attention_join(PagedArgs a) {
     const float *part = p + (long)i * (dim + 2);
     // A part's maximum is -inf only where nothing of it is seen (or a seen
     // page does not exist: then its sum is NaN, and so is the whole).
-    const float f = part[0] == -INFINITY ? (part[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(part[0] - m);
+    const float f = part[0] == -INFINITY ? (part[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f((part[0] - m) * a.scale);
     sum += f * part[1];
 #pragma unroll
     for (int j = 0; j < 4; j++)

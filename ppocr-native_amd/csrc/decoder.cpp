@@ -57,6 +57,10 @@ bool is_real(int t) { return t == PPOCR_F32 || t == PPOCR_BF16 || t == PPOCR_F16
 size_t size_of(int t) { return t == PPOCR_F32 ? 4 : t == PPOCR_BF16 || t == PPOCR_F16 ? 2 : 1; }
 bool aligned(const void *p, size_t n) { return uintptr_t(p) % n == 0; }
 
+// A softmax's scale for 2-logarithms: positive (a hidden product, -inf, times
+// 0 would be NaN; 1e-30 makes the weights equal just as well).
+float scale_of(float scale) { return std::fmax(std::fabs(scale) * 1.44269504088896340736f, 1e-30f); }
+
 // A stride's value: rows without a gap where it is 0.
 bool stride_of(size_t given, size_t width, long *out) {
   *out = long(given ? given : width);
@@ -219,7 +223,7 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
   a.q = q, a.y = y, a.batch = int(batch), a.heads = int(heads), a.splits = n;
   a.window = int(window < (size_t(1) << 31) - 1 ? window : 0);
   a.sinks = int(sinks < (size_t(1) << 30) ? sinks : size_t(1) << 30);
-  a.scale = scale * 1.44269504088896340736f;
+  a.scale = scale_of(scale), a.turn = scale < 0.0f;
   a.part = static_cast<float *>(workspace);
   const OnDevice on{hipStream_t(stream)};
   if (on.e != hipSuccess) return fail.hip("paged attention", on.e);
@@ -256,7 +260,7 @@ int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, si
   a.heads = int(heads), a.kv_heads = int(kv_heads), a.dim = int(dim);
   a.window = int(window < (size_t(1) << 31) - 1 ? window : 0);
   a.sinks = int(sinks < (size_t(1) << 30) ? sinks : size_t(1) << 30);
-  a.scale = scale * 1.44269504088896340736f;
+  a.scale = scale_of(scale), a.turn = scale < 0.0f;
   const OnDevice on{hipStream_t(stream)};
   if (on.e != hipSuccess) return fail.hip("window attention", on.e);
   return fail.hip("window attention", launch_window_attention(a, type, hipStream_t(stream)));

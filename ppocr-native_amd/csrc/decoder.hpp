@@ -15,6 +15,7 @@ namespace ppocr {
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
@@ -124,7 +125,8 @@ struct PagedArgs {
   long q_stride, y_stride;
   int batch, heads, splits;
   int window, sinks;  // window 0: every key is seen
-  float scale;
+  float scale;        // of 2-logarithms, positive
+  bool turn;          // the given scale was negative: q turns its sign
   float *part;  // splits > 1: batch x heads x splits rows of dim + 2 floats
 };
 // The parts a text's cache of up to `longest` tokens is split into.
@@ -139,6 +141,7 @@ struct PromptArgs {
   int batch, rows_q, rows_k, heads, kv_heads, dim;
   int window, sinks;
   float scale;
+  bool turn;
 };
 hipError_t launch_window_attention(const PromptArgs &a, int type, hipStream_t s);
 

@@ -103,7 +103,6 @@ __device__ __forceinline__ v4u weights16(uint32_t w) {
 // Dwords between the wave's quarters (lanes 16 p .. 16 p + 15): before, dword
 // j of quarter p is stretch byte 16 p + 4 j; after, 16 j + 4 p.
 __device__ __forceinline__ void turn_quarters(uint32_t (&w)[4]) {
-  typedef uint32_t v2u __attribute__((ext_vector_type(2)));
   v2u t = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
   w[0] = t[0], w[2] = t[1];
   t = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);

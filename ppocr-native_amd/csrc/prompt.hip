@@ -1,12 +1,13 @@
 // Causal attention of prompts with a sliding window and sinks
 // (ppocr_hip_window_attention).
 #include "attend.hpp"
+#include "kernels.hpp"
 
 namespace ppocr {
 namespace {
 
 // A block of queries: which text, and which of its rows. Blocks are counted
-// through the texts; there are at most rows_q / SIZE + batch.
+// through the texts; there are at most rows_q / size + batch.
 struct Block {
   int q0, nq;  // the text's first row of q and its queries
   int k0, nk;
@@ -16,8 +17,7 @@ struct Block {
 // Finds block `index`; false if there are fewer. Every wave of a workgroup
 // walks the starts, 64 texts at a time. Starts past the rows there are, and
 // such as decrease, leave texts of no rows.
-template <int SIZE>
-__device__ __forceinline__ bool find_block(const PromptArgs &a, int index, Block &out) {
+__device__ __forceinline__ bool find_block(const PromptArgs &a, int index, int size, Block &out) {
   const int lane = threadIdx.x % 64;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
     const int b = b0 + lane;
@@ -26,7 +26,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, int index, Block
       q0 = min(max(a.starts_q[b], 0), a.rows_q);
       nq = max(min(a.starts_q[b + 1], a.rows_q) - q0, 0);
     }
-    const int blocks = (nq + SIZE - 1) / SIZE;
+    const int blocks = (nq + size - 1) / size;
     int upto = blocks;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -38,7 +38,7 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, int index, Block
       const int at = __ffsll(past) - 1;
       out.q0 = __shfl(q0, at);
       out.nq = __shfl(nq, at);
-      out.first = (index - (__shfl(upto, at) - __shfl(blocks, at))) * SIZE;
+      out.first = (index - (__shfl(upto, at) - __shfl(blocks, at))) * size;
       const int text = b0 + at;
       out.k0 = min(max(a.starts_k[text], 0), a.rows_k);
       out.nk = max(min(a.starts_k[text + 1], a.rows_k) - out.k0, 0);
@@ -49,25 +49,72 @@ __device__ __forceinline__ bool find_block(const PromptArgs &a, int index, Block
   return false;
 }
 
-// Any type and dim: four waves of 16 queries of one head each, keys and
-// values straight from memory (the caches).
+// Queries first .. first + count - 1 of a block's text by one wave, one after
+// another and every key by itself, so that nothing of an unseen key (an
+// infinity or NaN in V) reaches a query: what the fast kernels fall back to
+// where they meet one next to a mask. A lane is a key, then a value of dim.
+template <int T>
+__device__ __forceinline__ void attend_alone(const PromptArgs &a, const Block &bl, int head, int first, int count) {
+  typedef num_t<T> V;
+  const int lane = threadIdx.x % 64, kv = head / (a.heads / a.kv_heads);
+  const V *k = (const V *)a.k + (long)bl.k0 * a.k_stride + (long)kv * a.dim;
+  const V *v = (const V *)a.v + (long)bl.k0 * a.v_stride + (long)kv * a.dim;
+  for (int i = first; i < min(first + count, bl.nq); i++) {
+    const V *q = (const V *)a.q + (long)(bl.q0 + i) * a.q_stride + (long)head * a.dim;
+    const int p = bl.nk - bl.nq + i, low = a.window ? max(p - a.window + 1, 0) : 0;
+    auto seen = [&](int j) { return j <= p && (j >= low || j < a.sinks); };
+    float m = -INFINITY, l = 0.0f, o[4] = {0, 0, 0, 0};
+    for (int j0 = 0; j0 <= p; j0 += 64) {
+      if (j0 + 63 < low && j0 >= a.sinks) continue;
+      const int j = j0 + lane;
+      float s = -INFINITY;
+      if (seen(j)) {
+        s = 0.0f;
+        for (int d = 0; d < a.dim; d++) s = fmaf(Num<T>::get(q[d]), Num<T>::get(k[j * a.k_stride + d]), s);
+        s *= a.turn ? -a.scale : a.scale;
+      }
+      float top = s;
+#pragma unroll
+      for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+      const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now;
+      const float shrink = __builtin_amdgcn_exp2f(m - base);
+      const float w = seen(j) ? __builtin_amdgcn_exp2f(s - base) : 0.0f;
+      m = now;
+      l = l * shrink + w;
+#pragma unroll
+      for (int c = 0; c < 4; c++) o[c] *= shrink;
+      for (int u = 0; u < 64; u++) {
+        if (!seen(j0 + u)) continue;
+        const float wu = __shfl(w, u);
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+          if (lane + 64 * c < a.dim) o[c] = fmaf(wu, Num<T>::get(v[(j0 + u) * a.v_stride + lane + 64 * c]), o[c]);
+      }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    V *y = (V *)a.y + (long)(bl.q0 + i) * a.y_stride + (long)head * a.dim;
+#pragma unroll
+    for (int c = 0; c < 4; c++)
+      if (lane + 64 * c < a.dim) y[lane + 64 * c] = Num<T>::put(l == 0.0f ? 0.0f : o[c] / l);
+  }
+}
+
+// 16 queries of one head, from the block's query `first` on, by one wave,
+// keys and values straight from memory (the caches): any type and dim.
 template <int T, int DP, bool EVEN>
-__global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
+__device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl, int head, int first) {
   typedef Attend<T, DP, EVEN> A;
   typedef typename A::V V;
   constexpr int K = A::KEYS;
-  Block bl;
-  if (!find_block<64>(a, blockIdx.y, bl)) return;
   const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
-  const int per = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads, head = kv * per + blockIdx.x / a.kv_heads;
-  const int first = bl.first + threadIdx.x / 64 * 16;
-  if (first >= bl.nq) return;
+  const int kv = head / (a.heads / a.kv_heads);
   const int rows = min(16, bl.nq - first);
   const int p0 = bl.nk - bl.nq + first;  // the first query's place; the last's is p0 + rows - 1
   const int p = p0 + min(col, rows - 1);
   A at;
   at.start((const V *)a.q + (long)(bl.q0 + first + min(col, rows - 1)) * a.q_stride + (long)head * a.dim, a.dim,
-           quarter);
+           quarter, a.turn);
   const V *k = (const V *)a.k + (long)bl.k0 * a.k_stride + (long)kv * a.dim;
   const V *v = (const V *)a.v + (long)bl.k0 * a.v_stride + (long)kv * a.dim;
   const int last = p0 + rows - 1;                            // of all rows' keys
@@ -75,6 +122,7 @@ __global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
   const int sinks = min(a.sinks, low);                       // sinks before every window
   const int start = low / K * K, sink_tiles = min((sinks + K - 1) / K, start / K);
   const int tiles = sink_tiles + (last >= start ? (last - start) / K + 1 : 0);
+  bool bad = false;
   for (int t = 0; t < tiles; t++) {
     const int k0 = t < sink_tiles ? t * K : start + (t - sink_tiles) * K;
     const bool masked = k0 + K - 1 > p0 || (a.window && k0 <= last - a.window);
@@ -86,10 +134,14 @@ __global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
       const int j = k0 + i;
       return j <= last && (j >= low || j < a.sinks);
     };
-    at.template tile<true>(
+    bad |= at.template tile<true>(
         [&](int i) -> const V * { return masked && !any(i) ? nullptr : k + (long)(k0 + i) * a.k_stride; },
         [&](int i) -> const V * { return masked && !any(i) ? nullptr : v + (long)(k0 + i) * a.v_stride; }, seen,
         masked, a.dim, a.scale, lane);
+  }
+  if (__any(bad)) {
+    attend_alone<T>(a, bl, head, first, rows);
+    return;
   }
   const float l = at.total();
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -105,24 +157,292 @@ __global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
   }
 }
 
+template <int T, int DP, bool EVEN>
+__global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
+  Block bl;
+  if (!find_block(a, blockIdx.y, 64, bl)) return;
+  const int per = a.heads / a.kv_heads;
+  const int first = bl.first + threadIdx.x / 64 * 16;
+  if (first < bl.nq)
+    attend_rows<T, DP, EVEN>(a, bl, blockIdx.x % a.kv_heads * per + blockIdx.x / a.kv_heads, first);
+}
+
+// ------------------------------------------------- 16-bit types, tiles in LDS
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+constexpr int kTileKeys = 64;
+constexpr int kTileWaves = 4;
+
+// Where a key's row of a tile keeps its 16-byte piece c: place c ^ turn(key),
+// so that both the 16 rows that a read of K touches at one piece and the four
+// rows of four pieces that a transposing read of V touches lie in different
+// banks. C: pieces a row has room for.
+template <int C>
+__device__ __forceinline__ int turn(int key) {
+  return C == 8 ? (key >> 1 & 1) << 2 | (key >> 2 & 3) : (key & 3) << 2 | (key >> 2 & 3);
+}
+
+// Whether a dword holds a 16-bit infinity or NaN.
+template <int T>
+__device__ __forceinline__ int not_finite2(uint32_t x) {
+  constexpr uint32_t lo = T == PPOCR_F16 ? 0x7c00u : 0x7f80u, hi = lo << 16;
+  return ((x & lo) == lo ? 1 : 0) + ((x & hi) == hi ? 1 : 0);
+}
+
+// Four waves, each 32 queries of one head; `hg` heads of one key head (1, 2 or
+// 4) share the workgroup's tiles of 64 keys and values, which go straight from
+// memory to LDS, the next tile's while this one's are used. The products are
+// 32x32x16, the 32 queries the columns of each:
+//   S^T[key][query] = K Q^T, O^T[d][query] += V^T P^T,
+// so that a lane holds one query's numbers: row maxima and sums need one
+// exchange between the wave's halves, and P goes from the first product's
+// result to the second's operand in its own lane, rounded to T, its keys in
+// the order 4 (lane / 32) + {0..3, 8..11}; V is read to match, transposed on
+// its way out of LDS.
+template <int T, int DP, bool WHOLE>
+__global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_attention_tiles(PromptArgs a, int hg) {
+  typedef num_t<T> V;
+  constexpr int C = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // pieces of a row
+  constexpr int TILE = kTileKeys * C * 16;               // bytes
+  constexpr int KS = DP / 16, DB = DP / 32, PIECES = kTileKeys * C / (64 * kTileWaves);
+  extern __shared__ __attribute__((aligned(1024))) char lds[];  // [2][K, V][TILE]
+  const int index = gridDim.y - 1 - blockIdx.y;  // the last block of a text, which sees most, first
+  const int size = 32 * kTileWaves / hg;
+  Block bl;
+  if (!find_block(a, index, size, bl)) return;
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int half = lane / 32, col = lane % 32;
+  const int per = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads;
+  const int head = kv * per + blockIdx.x / a.kv_heads * hg + wave % hg;
+  const int w0 = bl.first + wave / hg * 32;  // this wave's first query
+  const int p_first = bl.nk - bl.nq + bl.first, p_last = bl.nk - bl.nq + min(bl.first + size, bl.nq) - 1;
+  const int query = min(w0 + col, bl.nq - 1), p = bl.nk - bl.nq + query;
+  const int pw_first = bl.nk - bl.nq + w0, pw_last = bl.nk - bl.nq + min(w0 + 32, bl.nq) - 1;
+
+  const int p_low = a.window ? p - a.window + 1 : 0;  // this query's window
+
+  // The tiles that the block sees: of sinks, then of the windows.
+  const int low = a.window ? max(p_first - a.window + 1, 0) : 0;
+  const int sinks = min(a.sinks, low), start = low / kTileKeys * kTileKeys;
+  const int sink_tiles = min((sinks + kTileKeys - 1) / kTileKeys, start / kTileKeys);
+  const int tiles = sink_tiles + (p_last >= start ? (p_last - start) / kTileKeys + 1 : 0);
+  auto tile_key = [&](int t) { return t < sink_tiles ? t * kTileKeys : start + (t - sink_tiles) * kTileKeys; };
+
+  const int pieces = a.dim / 8;  // WHOLE: C
+  if (!WHOLE) {  // pieces past dim stay zero
+    for (int i = tid; i < 4 * TILE / 16; i += 64 * kTileWaves) ((v4u *)lds)[i] = v4u{0, 0, 0, 0};
+    __syncthreads();
+  }
+  const char *k_base = (const char *)((const V *)a.k + (long)bl.k0 * a.k_stride + (long)kv * a.dim);
+  const char *v_base = (const char *)((const V *)a.v + (long)bl.k0 * a.v_stride + (long)kv * a.dim);
+  auto load = [&](int t, int buffer) {
+    const int k0 = tile_key(t);
+#pragma unroll
+    for (int i = 0; i < PIECES; i++) {
+      const int e = (i * kTileWaves + wave) * 64 + lane, row = e / C, piece = (e % C) ^ turn<C>(row);
+      const long key = min(k0 + row, bl.nk - 1);
+      char *to = lds + buffer * 2 * TILE + (i * kTileWaves + wave) * 1024;
+      if (WHOLE || piece < pieces) {
+        __builtin_amdgcn_global_load_lds((const void *)(k_base + key * a.k_stride * 2 + piece * 16),
+                                         (lds_void *)to, 16, 0, 0);
+        __builtin_amdgcn_global_load_lds((const void *)(v_base + key * a.v_stride * 2 + piece * 16),
+                                         (lds_void *)(to + TILE), 16, 0, 0);
+      }
+    }
+  };
+
+  v4u q[KS];
+  {
+    const V *row = (const V *)a.q + (long)(bl.q0 + query) * a.q_stride + (long)head * a.dim;
+    const uint32_t sign = a.turn ? 0x80008000u : 0u;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const int d = 16 * s + 8 * half;
+      q[s] = v4u{0, 0, 0, 0};
+      if (d < a.dim) __builtin_memcpy(&q[s], row + d, 16);
+#pragma unroll
+      for (int i = 0; i < 4; i++) q[s][i] ^= sign;
+    }
+  }
+  v16f o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; b++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[b][i] = 0.0f;
+  float m = -INFINITY, l = 0.0f;
+  int bad = 0;
+
+  if (tiles > 0) load(0, 0);
+  for (int t = 0; t < tiles; t++) {
+    const int k0 = tile_key(t);
+    __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0), lgkmcnt(0): this tile is in LDS, the last one read
+    ring_barrier();
+    const char *kt = lds + (t & 1) * 2 * TILE, *vt = kt + TILE;
+    if (t + 1 < tiles) load(t + 1, (t + 1) & 1);
+    // Where some query does not see some key of the tile, an infinity or NaN
+    // in V would reach it through its weight of 0.
+    if (k0 + kTileKeys - 1 > p_first || (a.window && k0 <= p_last - a.window)) {
+#pragma unroll
+      for (int i = 0; i < PIECES; i++) {
+        const v4u x = *(const v4u *)(vt + (i * 64 * kTileWaves + tid) * 16);
+        bad |= not_finite2<T>(x[0]) + not_finite2<T>(x[1]) + not_finite2<T>(x[2]) + not_finite2<T>(x[3]);
+      }
+    }
+    const bool none = k0 > pw_last || (a.window && k0 + kTileKeys - 1 <= pw_first - a.window && k0 >= a.sinks);
+    if (none || w0 >= bl.nq) continue;
+    const bool masked = k0 + kTileKeys - 1 > pw_first || (a.window && k0 <= pw_last - a.window);
+
+    v16f s[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
+      const char *row = kt + (32 * b + col) * C * 16;
+#pragma unroll
+      for (int c = 0; c < KS; c++) {
+        const v4u f = *(const v4u *)(row + ((2 * c + half) ^ turn<C>(col)) * 16);
+        if constexpr (T == PPOCR_F16)
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f), __builtin_bit_cast(v8h, q[c]), s[b],
+                                                        0, 0, 0);
+        else
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, f), __builtin_bit_cast(v8bf, q[c]),
+                                                         s[b], 0, 0, 0);
+      }
+    }
+    if (masked) {
+      const int here = k0 + 4 * half, last = p - here, from = p_low - here, sunk = a.sinks - here;
+#pragma unroll
+      for (int b = 0; b < 2; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int j = 32 * b + 8 * (i / 4) + i % 4;
+          const int hidden = int(j > last) | (int(j < from) & int(j >= sunk));
+          s[b][i] = hidden ? -INFINITY : s[b][i];
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) top = fmaxf(top, s[b][i]);
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // The maximum follows only where it grew by a factor of 2^8 or more: until
+    // then the weights are up to 2^8, which costs them no precision.
+    if (__any((top - m) * a.scale > 8.0f)) {
+      const float now = fmaxf(m, top);
+      const float shrink = now == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((m - now) * a.scale);
+      m = now;
+      l *= shrink;
+#pragma unroll
+      for (int b = 0; b < DB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[b][i] *= shrink;
+    }
+    const float base = m == -INFINITY ? 0.0f : m * a.scale;
+    v4u pf[4];
+#pragma unroll
+    for (int b = 0; b < 2; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -base));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale, -base));
+        l += x + y;
+        pf[2 * b + i / 8][i / 2 % 4] = Tile16<T>::pack(x, y);
+      }
+#pragma unroll
+    for (int b = 0; b < DB; b++) {
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        // Lane s of 16 names keys s / 4 of four and values 4 (s % 4) .. + 3 of
+        // 16, and gets value s of the four keys.
+        v4u f;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          const int key = 16 * c + 8 * g + 4 * half + lane % 16 / 4;
+          const int piece = 4 * b + 2 * (lane / 16 % 2) + lane % 4 / 2;
+          const char *at = vt + (key * C + (piece ^ turn<C>(key))) * 16 + lane % 2 * 8;
+          const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
+          f[2 * g] = __builtin_bit_cast(v2u, r)[0];
+          f[2 * g + 1] = __builtin_bit_cast(v2u, r)[1];
+        }
+        if constexpr (T == PPOCR_F16)
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f), __builtin_bit_cast(v8h, pf[c]),
+                                                        o[b], 0, 0, 0);
+        else
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, f), __builtin_bit_cast(v8bf, pf[c]),
+                                                         o[b], 0, 0, 0);
+      }
+    }
+  }
+  if (__syncthreads_or(bad)) {  // rare: key by key where it matters
+    attend_alone<T>(a, bl, head, w0, 32);
+    return;
+  }
+  l += __shfl_xor(l, 32);
+  if (w0 + col >= bl.nq) return;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
+  V *y = (V *)a.y + (long)(bl.q0 + query) * a.y_stride + (long)head * a.dim;
+#pragma unroll
+  for (int b = 0; b < DB; b++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = 32 * b + 2 * i + 4 * half;
+      V out[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) out[e] = Num<T>::put(l == 0.0f ? 0.0f : o[b][i + e] * f);
+      store_n(y + d, (long)a.dim - d, out);
+    }
+}
+
+template <int T, int DP, bool WHOLE>
+hipError_t launch_tiles_of(const PromptArgs &a, hipStream_t s) {
+  const int per = a.heads / a.kv_heads, hg = per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1;
+  const int size = 32 * kTileWaves / hg;
+  constexpr int bytes = 4 * kTileKeys * (DP <= 64 ? 8 : DP <= 128 ? 16 : 32) * 16;
+  const void *kernel = (const void *)&window_attention_tiles<T, DP, WHOLE>;
+  const hipError_t e = allow_lds(kernel, bytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((window_attention_tiles<T, DP, WHOLE>), dim3(a.heads / hg, a.rows_q / size + a.batch),
+                     dim3(64 * kTileWaves), bytes, s, a, hg);
+  return hipGetLastError();
+}
+
 template <int T, int DP>
-void launch_rows(const PromptArgs &a, hipStream_t s) {
+hipError_t launch_tiles(const PromptArgs &a, hipStream_t s) {
+  if constexpr (DP == 64 || DP == 128 || DP == 256)
+    if (a.dim == DP) return launch_tiles_of<T, DP, true>(a, s);
+  return launch_tiles_of<T, DP, false>(a, s);
+}
+
+template <int T, int DP>
+hipError_t launch_rows(const PromptArgs &a, hipStream_t s) {
   const dim3 grid(a.heads, a.rows_q / 64 + a.batch);
   if (a.dim % 8 == 0)
     hipLaunchKernelGGL((window_attention_rows<T, DP, true>), grid, dim3(256), 0, s, a);
   else
     hipLaunchKernelGGL((window_attention_rows<T, DP, false>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 template <int T>
 hipError_t launch(const PromptArgs &a, hipStream_t s) {
-  if (a.dim <= 64)
-    launch_rows<T, 64>(a, s);
-  else if (a.dim <= 128)
-    launch_rows<T, 128>(a, s);
-  else
-    launch_rows<T, 256>(a, s);
-  return hipGetLastError();
+  if constexpr (T != PPOCR_F32) {
+    // Loads to LDS move 16 aligned bytes.
+    auto a16 = [](const void *p, long stride) { return uintptr_t(p) % 16 == 0 && stride % 8 == 0; };
+    if (a.dim % 8 == 0 && a16(a.k, a.k_stride) && a16(a.v, a.v_stride)) {
+      if (a.dim <= 64) return launch_tiles<T, 64>(a, s);
+      if (a.dim <= 96) return launch_tiles<T, 96>(a, s);
+      if (a.dim <= 128) return launch_tiles<T, 128>(a, s);
+      if (a.dim <= 192) return launch_tiles<T, 192>(a, s);
+      return launch_tiles<T, 256>(a, s);
+    }
+  }
+  if (a.dim <= 64) return launch_rows<T, 64>(a, s);
+  if (a.dim <= 128) return launch_rows<T, 128>(a, s);
+  return launch_rows<T, 256>(a, s);
 }
 
 }  // namespace
