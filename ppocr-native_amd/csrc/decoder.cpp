@@ -145,7 +145,7 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
   if (group != 32 && group != 64 && group != 128)
     return fail("4-bit product: groups of %zu inputs: 32, 64 or 128 are taken", group);
   if (m == 0 || n == 0) return 0;
-  if (!k || k > kMost || n > kMost || m > size_t(16) * 65535)
+  if (!k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20 || (n + 15) / 16 * ((m + 15) / 16) > size_t(1) << 26)
     return fail("4-bit product: %zu rows of %zu inputs to %zu outputs", m, k, n);
   if (!x || !q || !scales || !y || (x8 && !x_scales))
     return fail("4-bit product: x, q, scales, y and (for 8-bit x) x_scales are needed");
@@ -155,15 +155,19 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
       !aligned(bias, size_of(y_type)) || !aligned(y, size_of(y_type)))
     return fail("4-bit product: a pointer is not aligned to its type");
   Q4Args a{};
-  if (!stride_of(x_stride, k, &a.x_stride) || !stride_of(y_stride, n, &a.y_stride))
+  if (!stride_of(x_stride, k, &a.x_stride) || a.x_stride > 1 << 24 || !stride_of(y_stride, n, &a.y_stride))
     return fail("4-bit product: strides %zu for %zu inputs, %zu for %zu outputs", x_stride, k, y_stride, n);
   a.x = x, a.x_scales = x_scales, a.q = q, a.scales = scales, a.zeros = zeros, a.bias = bias, a.y = y;
   a.m = int(m), a.n = int(n), a.k = int(k), a.group = int(group), a.groups = int((k + group - 1) / group);
-  a.x_group = int(x_group), a.x_groups = a.groups;
+  a.x_group = int(x_group);
   a.scale_type = scale_type, a.y_type = y_type;
   const OnDevice on{hipStream_t(stream)};
   if (on.e != hipSuccess) return fail.hip("4-bit product", on.e);
-  return fail.hip("4-bit product", launch_q4_product(a, x_type, hipStream_t(stream)));
+  const hipStream_t st = hipStream_t(stream);
+  return fail.hip("4-bit product", x_type == PPOCR_F32    ? launch_q4_f32(a, 0, st)
+                                   : x_type == PPOCR_BF16 ? launch_q4_bf16(a, 0, st)
+                                   : x_type == PPOCR_F16  ? launch_q4_f16(a, 0, st)
+                                                          : launch_q4_i8(a, x_type == PPOCR_E4M3, st));
 }
 
 int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_stride, const ppocr_kv_cache *cache,

@@ -92,12 +92,15 @@ struct Q4Args {
   const uint8_t *zeros;
   const void *bias;
   void *y;
-  long x_stride, y_stride, x_groups;
+  long x_stride, y_stride;
   int m, n, k, group, groups;
   int x_group;  // 0: one scale a row of x (8-bit x)
   int scale_type, y_type;
 };
-hipError_t launch_q4_product(const Q4Args &a, int x_type, hipStream_t s);
+hipError_t launch_q4_f32(const Q4Args &a, int, hipStream_t s);
+hipError_t launch_q4_bf16(const Q4Args &a, int, hipStream_t s);
+hipError_t launch_q4_f16(const Q4Args &a, int, hipStream_t s);
+hipError_t launch_q4_i8(const Q4Args &a, int e4m3, hipStream_t s);
 
 struct CacheArgs {
   void *k, *v;
