@@ -16,32 +16,37 @@
 
 namespace ppocr {
 
-// Loads of `N` of a head's `dim` values at d: whole, or cut off at dim where
-// dims are not EVEN (a multiple of 8). Zeros past dim.
-template <bool EVEN, typename V, int N>
+// How a head's dims fill the DP that the products have.
+enum Dims {
+  DIMS_WHOLE,  // dim == DP
+  DIMS_EVEN,   // a multiple of 8, at most DP
+  DIMS_ANY     // at most DP, value by value
+};
+
+// N values of a head at d. What lies past dim is some other value of the
+// head's: nothing is read behind a branch, which would be waited for.
+template <int DIMS, typename V, int N>
 __device__ __forceinline__ void load_dims(const V *p, int d, int dim, V (&v)[N]) {
-  if constexpr (EVEN) {
+  if constexpr (DIMS == DIMS_WHOLE) {
+    __builtin_memcpy(v, p + d, sizeof v);
+  } else if constexpr (DIMS == DIMS_EVEN) {
     constexpr int M = N < 8 ? N : 8;
 #pragma unroll
-    for (int i = 0; i < N; i += M) {
-      if (d + i < dim) {
-        __builtin_memcpy(v + i, p + d + i, M * sizeof(V));
-      } else {
-#pragma unroll
-        for (int e = 0; e < M; e++) v[i + e] = V(0);
-      }
-    }
+    for (int i = 0; i < N; i += M) __builtin_memcpy(v + i, p + (d + i < dim ? d + i : 0), M * sizeof(V));
   } else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      v[i] = V(0);
-      if (d + i < dim) v[i] = p[d + i];
-    }
+    for (int i = 0; i < N; i++) v[i] = p[min(d + i, dim - 1)];
   }
 }
 
-template <int T>
-struct Tile;  // T's matrix products
+// Zeros for those past dim.
+template <int DIMS, typename V, int N>
+__device__ __forceinline__ void cut_dims(int d, int dim, V (&v)[N]) {
+  if constexpr (DIMS != DIMS_WHOLE) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = d + i < dim ? v[i] : V(0);
+  }
+}
 
 // 16-bit types: 32 keys a tile, inner index 32.
 template <int T>
@@ -71,7 +76,7 @@ struct Tile16 {
 };
 
 // The state of 16 rows over DP (padded) dims.
-template <int T, int DP, bool EVEN>
+template <int T, int DP, int DIMS>
 struct Attend {
   typedef num_t<T> V;
   static constexpr bool F32 = T == PPOCR_F32;
@@ -88,7 +93,8 @@ struct Attend {
   __device__ __forceinline__ void start(const V *qrow, int dim, int quarter, bool turn) {
 #pragma unroll
     for (int c = 0; c < QC; c++) {
-      load_dims<EVEN>(qrow, QN * (4 * c + quarter), dim, q[c]);
+      load_dims<DIMS>(qrow, QN * (4 * c + quarter), dim, q[c]);
+      cut_dims<DIMS>(QN * (4 * c + quarter), dim, q[c]);
       if (turn) {
 #pragma unroll
         for (int i = 0; i < QN; i++) q[c][i] = -q[c][i];
@@ -109,43 +115,53 @@ struct Attend {
       return (__builtin_bit_cast(uint16_t, x) & 0x7c00) != 0x7c00;
   }
 
-  // One tile of keys. k_row(key) and v_row(key) give the rows of the tile's
-  // keys 0 .. KEYS - 1, or NULL where no row of the 16 sees the key (nothing
-  // is read there); seen(key) says whether this lane's row does. `masked`
-  // (uniform): not every key of the tile is seen by every row. `scale`: of
-  // 2-logarithms, positive. RAGGED: the 16 rows do not see the same keys; the
-  // result says whether this lane met an infinity or NaN in V in such a tile,
-  // which a weight of 0 carries into the rows that do not see it.
-  template <bool RAGGED, class KR, class VR, class Seen>
-  __device__ __forceinline__ bool tile(KR k_row, VR v_row, Seen seen, bool masked, int dim, float scale, int lane) {
+  // A tile's keys and values in registers.
+  struct Tile {
+    V k[H][QC][QN], v[H][4][E];
+  };
+
+  // k_row(key) and v_row(key) give the rows of the tile's keys 0 .. KEYS - 1,
+  // any row that may be read where no row of the 16 sees the key.
+  template <class KR, class VR>
+  static __device__ __forceinline__ void load(Tile &t, KR k_row, VR v_row, int dim, int lane) {
     const int col = lane % 16, quarter = lane / 16;
-    V k[H][QC][QN];
 #pragma unroll
     for (int h = 0; h < H; h++) {
       const V *p = k_row(16 * h + col);
 #pragma unroll
-      for (int c = 0; c < QC; c++) {
-        if (p) {
-          load_dims<EVEN>(p, QN * (4 * c + quarter), dim, k[h][c]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < QN; i++) k[h][c][i] = V(0);
-        }
-      }
+      for (int c = 0; c < QC; c++) load_dims<DIMS>(p, QN * (4 * c + quarter), dim, t.k[h][c]);
     }
-    V v[H][4][E];
 #pragma unroll
     for (int h = 0; h < H; h++)
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const V *p = v_row(16 * h + 4 * quarter + r);
-        if (p) {
-          load_dims<EVEN>(p, E * col, dim, v[h][r]);
-        } else {
+      for (int r = 0; r < 4; r++) load_dims<DIMS>(v_row(16 * h + 4 * quarter + r), E * col, dim, t.v[h][r]);
+  }
+
+  // Takes a tile in. seen(key) says whether this lane's row sees it, any(key)
+  // whether some row does; `masked` (uniform): not every key of the tile is
+  // seen by every row. `scale`: of 2-logarithms, positive. RAGGED: the 16 rows
+  // do not see the same keys; the result says whether this lane met an
+  // infinity or NaN in V in such a tile, which a weight of 0 carries into the
+  // rows that do not see it.
+  template <bool RAGGED, class Seen, class Any>
+  __device__ __forceinline__ bool use(Tile &t, Seen seen, Any any, bool masked, int dim, float scale, int lane) {
+    const int quarter = lane / 16;
+    auto &k = t.k;
+    auto &v = t.v;
 #pragma unroll
-          for (int i = 0; i < E; i++) v[h][r][i] = V(0);
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int c = 0; c < QC; c++) cut_dims<DIMS>(QN * (4 * c + quarter), dim, k[h][c]);
+    if (masked) {
+#pragma unroll
+      for (int h = 0; h < H; h++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const bool on = any(16 * h + 4 * quarter + r);
+#pragma unroll
+          for (int e = 0; e < E; e++) v[h][r][e] = on ? v[h][r][e] : V(0);
         }
-      }
+    }
     v4f s[H];
 #pragma unroll
     for (int h = 0; h < H; h++) {

@@ -1,5 +1,7 @@
 // The paged cache of keys and values: appending to it (ppocr_hip_kv_append)
 // and attention of one new token a text over it (ppocr_hip_paged_attention).
+#include <algorithm>
+
 #include "attend.hpp"
 
 namespace ppocr {
@@ -8,10 +10,24 @@ namespace {
 // ------------------------------------------------------------------- append
 
 // Text blockIdx.y; its new tokens are shared by the waves of gridDim.x
-// workgroups, a token a wave at a time. A token's rows of k and v are read
-// and written in 16-byte pieces of a head: memory bound, and at a token a
-// text bound by the launch.
+// workgroups, a token a wave at a time: its place is the same in all lanes,
+// its rows of k and v are copied in 16-byte pieces of a head, two of each on
+// their way. Memory bound; at a token a text bound by the launch. (Eight
+// tokens a workgroup, their places by one lane each and shared in LDS, took
+// 25 us for the 5 400 tokens that this copies in 12.)
+// WHOLE: heads are whole pieces.
 template <typename V>
+__device__ __forceinline__ v4u load16(const V *p) {
+  v4u v;
+  __builtin_memcpy(&v, p, 16);
+  return v;
+}
+template <typename V>
+__device__ __forceinline__ void store16(V *p, v4u v) {
+  __builtin_memcpy(p, &v, 16);
+}
+
+template <typename V, bool WHOLE>
 __global__ __launch_bounds__(256) void kv_append_rows(AppendArgs a) {
   constexpr int N = 16 / sizeof(V);
   const int b = blockIdx.y, lane = threadIdx.x % 64;
@@ -19,25 +35,41 @@ __global__ __launch_bounds__(256) void kv_append_rows(AppendArgs a) {
   long first = b, last = b + 1L;
   if (a.starts) first = a.starts[b], last = a.starts[b + 1];
   const long count = last - first;
-  const long end = a.c.lengths[b];
+  const int end = a.c.lengths[b];
   const int pieces = (a.c.dim + N - 1) / N, all = a.c.heads * pieces;
   for (long i = wave; i < count; i += waves) {
     const long row = first + i, at = end - count + i;
     if (row < 0 || row >= a.rows || at < 0) continue;
-    const long slot = at / a.c.page_size;
+    const int slot = a.c.by_page((int)at);  // (at < end, an int)
     if (slot >= a.c.table_width) continue;
     const int page = a.c.table[b * a.c.table_width + slot];
     if (page < 0 || page >= a.c.pages) continue;
-    const long to = page * a.c.page_stride + (at - slot * a.c.page_size) * a.c.token_stride;
-    const V *k = (const V *)a.k + row * a.k_stride, *v = (const V *)a.v + row * a.v_stride;
-    for (int p = lane; p < all; p += 64) {
-      const int head = p / pieces, d = (p - head * pieces) * N;
-      const long from = (long)head * a.c.dim + d, into = to + head * a.c.head_stride + d;
-      V kv[N], vv[N];
-      load_n(k + from, a.c.dim - d, kv);
-      load_n(v + from, a.c.dim - d, vv);
-      store_n((V *)a.c.k + into, a.c.dim - d, kv);
-      store_n((V *)a.c.v + into, a.c.dim - d, vv);
+    const long to = page * a.c.page_stride + (at - (long)slot * a.c.page_size) * a.c.token_stride;
+    const V *kr = (const V *)a.k + row * a.k_stride, *vr = (const V *)a.v + row * a.v_stride;
+    if constexpr (WHOLE) {
+      for (int p = lane; p < all; p += 128) {
+        const int p2 = min(p + 64, all - 1);  // (past the last: the last again)
+        const int h1 = p / pieces, d1 = (p - h1 * pieces) * N, h2 = p2 / pieces, d2 = (p2 - h2 * pieces) * N;
+        const long f1 = (long)h1 * a.c.dim + d1, f2 = (long)h2 * a.c.dim + d2;
+        const v4u k1 = load16(kr + f1), v1 = load16(vr + f1), k2 = load16(kr + f2), v2 = load16(vr + f2);
+        const long t1 = to + h1 * a.c.head_stride + d1, t2 = to + h2 * a.c.head_stride + d2;
+        store16((V *)a.c.k + t1, k1);
+        store16((V *)a.c.v + t1, v1);
+        if (p + 64 < all) {
+          store16((V *)a.c.k + t2, k2);
+          store16((V *)a.c.v + t2, v2);
+        }
+      }
+    } else {
+      for (int p = lane; p < all; p += 64) {
+        const int head = p / pieces, d = (p - head * pieces) * N, left = a.c.dim - d;
+        const long from = (long)head * a.c.dim + d, into = to + head * a.c.head_stride + d;
+        V k[N], v[N];
+        load_n(kr + from, left, k);
+        load_n(vr + from, left, v);
+        store_n((V *)a.c.k + into, left, k);
+        store_n((V *)a.c.v + into, left, v);
+      }
     }
   }
 }
@@ -67,23 +99,24 @@ __device__ __forceinline__ Seen seen_of(int length, int window, int sinks, int k
   return s;
 }
 
-// Tiles of a part: all parts but the last that is not empty have as many.
-constexpr int kLeastTiles = 4;
-__device__ __forceinline__ int tiles_a_part(int tiles, int splits) {
-  return max((tiles + splits - 1) / splits, kLeastTiles);
+// Tiles of a part: as many in every text, so that workgroups have equal work
+// where texts do not, unless a text is longer than was said.
+__device__ __forceinline__ int tiles_a_part(int tiles, int each, int splits) {
+  return max((tiles + splits - 1) / splits, each);
 }
 
 // Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.y, part
 // blockIdx.x of its tiles. PAGED16: pages are multiples of 16 tokens.
-template <int T, int DP, bool EVEN, bool PAGED16>
-__global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a) {
-  typedef Attend<T, DP, EVEN> A;
+template <int T, int DP, int DIMS, bool PAGED16>
+__global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attention_parts(PagedArgs a) {
+  typedef Attend<T, DP, DIMS> A;
   typedef typename A::V V;
   constexpr int K = A::KEYS;
   __shared__ float lds_o[kWaves][16][DP + 4];
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
   __shared__ int lds_bad;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, col = lane % 16, quarter = lane / 16;
+  const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int b = blockIdx.z, per = a.heads / a.c.heads, blocks = (per + 15) / 16;
   const int kv = blockIdx.y / blocks, h0 = kv * per + blockIdx.y % blocks * 16;
   const int rows = min(16, kv * per + per - h0);
@@ -91,7 +124,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a
   const int length = a.c.lengths[b];
   const bool too_long = length > capacity;
   const Seen s = seen_of(too_long ? 0 : length, a.window, a.sinks, K);
-  const int each = tiles_a_part(s.tiles, a.splits);
+  const int each = tiles_a_part(s.tiles, a.each, a.splits);
   const int begin = blockIdx.x * each, end = min(begin + each, s.tiles);
   if (begin >= end && blockIdx.x) return;  // part 0 of an empty text writes its zeros
   if (threadIdx.x == 0) lds_bad = too_long;
@@ -103,45 +136,84 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a
   const int *table = a.c.table + b * a.c.table_width;
   const V *ck = (const V *)a.c.k + kv * a.c.head_stride, *cv = (const V *)a.c.v + kv * a.c.head_stride;
   bool bad = false;
-  for (int t = begin + wave; t < end; t += kWaves) {
-    const int k0 = t < s.sink_tiles ? t * K : s.first + (t - s.sink_tiles) * K;
-    const bool masked = k0 + K > s.length || k0 < s.low;
-    auto seen = [&](int i) { return k0 + i < s.length && (k0 + i >= s.low || k0 + i < s.sinks); };
+  auto tile_key = [&](int t) { return t < s.sink_tiles ? t * K : s.first + (t - s.sink_tiles) * K; };
+  // Token k's row in its page, or -1 where that does not exist.
+  auto row_of = [&](int k) -> long {
+    const int slot = a.c.by_page(k), page = table[slot];
+    return page < 0 || page >= a.c.pages
+               ? -1
+               : page * a.c.page_stride + (long)(k - slot * a.c.page_size) * a.c.token_stride;
+  };
+
+  // Tiles that are seen whole: their loads run one tile ahead.
+  const int whole0 = max(begin, s.sink_tiles + (s.first < s.low ? 1 : 0));
+  const int whole1 = min(end, s.sink_tiles + (s.length - s.first) / K);
+  typename A::Tile ta, tb;
+  // The rows of tile t: with pages of multiples of 16 tokens where its halves
+  // start, the same in all lanes; else lane i's is token i's. (A page that
+  // does not exist is read as page 0, and the text's result is NaN.)
+  struct Rows {
+    long at[PAGED16 ? A::H : 1];
+  };
+  auto find = [&](int t) {
+    Rows r;
+    const int k0 = tile_key(min(t, whole1 - 1));
     if constexpr (PAGED16) {
-      long base[A::H];
 #pragma unroll
-      for (int h = 0; h < A::H; h++) {
-        const int k = k0 + 16 * h;  // the half's first token; a half past the text is not looked up
-        const int slot = k / a.c.page_size;
-        const int page = k < s.length ? table[slot] : 0;
-        base[h] = page * a.c.page_stride + (long)(k - slot * a.c.page_size) * a.c.token_stride;
-        if (page < 0 || page >= a.c.pages) base[h] = -1;
-        // (A half of which only unseen tokens lie in the text is not read.)
-        bool any = false;
-        if (base[h] < 0) {
-          for (int i = 0; i < 16; i++) any = any || seen(16 * h + i);
-          bad = bad || any;
-        }
-      }
-      auto row = [&](const V *c, int i) -> const V * {
-        const long o = base[i / 16];
-        return o < 0 || (masked && !seen(i)) ? nullptr : c + o + (i % 16) * a.c.token_stride;
-      };
-      at.template tile<false>([&](int i) { return row(ck, i); }, [&](int i) { return row(cv, i); }, seen, masked, a.c.dim, a.scale,
-              lane);
+      for (int h = 0; h < A::H; h++) r.at[h] = row_of(k0 + 16 * h);
     } else {
-      auto row = [&](const V *c, int i) -> const V * {
-        if (masked && !seen(i)) return nullptr;
-        const int k = k0 + i, slot = k / a.c.page_size, page = table[slot];
-        if (page < 0 || page >= a.c.pages) {
-          bad = true;
-          return nullptr;
-        }
-        return c + page * a.c.page_stride + (long)(k - slot * a.c.page_size) * a.c.token_stride;
-      };
-      at.template tile<false>([&](int i) { return row(ck, i); }, [&](int i) { return row(cv, i); }, seen, masked, a.c.dim, a.scale,
-              lane);
+      r.at[0] = row_of(k0 + lane % K);
     }
+    return r;
+  };
+  auto load = [&](typename A::Tile &tile, Rows &r) {
+#pragma unroll
+    for (int h = 0; h < (PAGED16 ? A::H : 1); h++) {
+      bad |= r.at[h] < 0;
+      r.at[h] = max(r.at[h], 0L);
+    }
+    auto row = [&](const V *c, int i) -> const V * {
+      if constexpr (PAGED16) return c + r.at[i / 16] + (i % 16) * a.c.token_stride;
+      return c + (long)(((uint64_t)(uint32_t)__shfl((int)(r.at[0] >> 32), i) << 32) | (uint32_t)__shfl((int)r.at[0], i));
+    };
+    A::load(tile, [&](int i) { return row(ck, i); }, [&](int i) { return row(cv, i); }, a.c.dim, lane);
+  };
+  auto all = [](int) { return true; };
+  int t = whole0 + wave;
+  if (t < whole1) {
+    Rows r = find(t);
+    load(ta, r);
+    r = find(t + kWaves);
+    while (true) {
+      if (t + kWaves < whole1) load(tb, r);
+      r = find(t + 2 * kWaves);
+      at.template use<false>(ta, all, all, false, a.c.dim, a.scale, lane);
+      t += kWaves;
+      if (t >= whole1) break;
+      if (t + kWaves < whole1) load(ta, r);
+      r = find(t + 2 * kWaves);
+      at.template use<false>(tb, all, all, false, a.c.dim, a.scale, lane);
+      t += kWaves;
+      if (t >= whole1) break;
+    }
+  }
+  // The others: sinks, and the two ends of the window.
+  for (int u = begin + wave; u < end; u += kWaves) {
+    if (u >= whole0 && u < whole1) continue;
+    const int k0 = tile_key(u);
+    auto seen = [&](int i) { return k0 + i < s.length && (k0 + i >= s.low || k0 + i < s.sinks); };
+    long mine = 0;  // token lane % K's row; the cache's first where it is not seen
+    if (seen(lane % K)) {
+      mine = row_of(k0 + lane % K);
+      bad |= mine < 0;
+      mine = max(mine, 0L);
+    }
+    auto row = [&](const V *c, int i) -> const V * {
+      const long o = (long)(((uint64_t)(uint32_t)__shfl((int)(mine >> 32), i) << 32) | (uint32_t)__shfl((int)mine, i));
+      return c + o;
+    };
+    A::load(ta, [&](int i) { return row(ck, i); }, [&](int i) { return row(cv, i); }, a.c.dim, lane);
+    at.template use<false>(ta, seen, seen, true, a.c.dim, a.scale, lane);
   }
   // The waves' parts, joined.
   if (bad) lds_bad = 1;
@@ -176,47 +248,69 @@ __global__ __launch_bounds__(64 * kWaves) void paged_attention_parts(PagedArgs a
   }
 }
 
-// Joins a row's parts: a wave a head of a text.
+// Joins a row's parts, a workgroup a head of a text: lane i of each wave has
+// parts i and i + 64's factors, wave w adds parts w, w + 4, ... of them.
+constexpr int kMostParts = 128;
+
 template <int T>
-__global__ __launch_bounds__(64) void paged_attention_join(PagedArgs a) {
+__global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
   typedef num_t<T> V;
-  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
+  __shared__ float lds_o[4][256], lds_f[kMostParts];
+  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int length = a.c.lengths[b];
   const Seen s = seen_of(length > a.c.table_width * a.c.page_size ? 0 : length, a.window, a.sinks,
                          T == PPOCR_F32 ? 16 : 32);
-  const int each = tiles_a_part(s.tiles, a.splits);
-  const int parts = max(1, (s.tiles + each - 1) / each), dim = a.c.dim;
-  const float *p = a.part + (long)(b * a.heads + head) * a.splits * (dim + 2);
-  float m = -INFINITY;
-  for (int i = 0; i < parts; i++) m = fmaxf(m, p[(long)i * (dim + 2)]);
-  float sum = 0.0f, o[4] = {0, 0, 0, 0};
-  for (int i = 0; i < parts; i++) {
-    const float *part = p + (long)i * (dim + 2);
-    // A part's maximum is -inf only where nothing of it is seen (or a seen
-    // page does not exist: then its sum is NaN, and so is the whole).
-    const float f = part[0] == -INFINITY ? (part[1] == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f((part[0] - m) * a.scale);
-    sum += f * part[1];
+  const int each = tiles_a_part(s.tiles, a.each, a.splits);
+  const int parts = max(1, (s.tiles + each - 1) / each), dim = a.c.dim, row = dim + 2;
+  const float *p = a.part + (long)(b * a.heads + head) * a.splits * row;
+  const float m0 = lane < parts ? p[(long)lane * row] : -INFINITY, l0 = lane < parts ? p[(long)lane * row + 1] : 0.0f;
+  const int far = lane + 64;
+  const float m1 = far < parts ? p[(long)far * row] : -INFINITY, l1 = far < parts ? p[(long)far * row + 1] : 0.0f;
+  float m = fmaxf(m0, m1);
+#pragma unroll
+  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  // A part's maximum is -inf only where nothing of it is seen (or a seen page
+  // does not exist: then its sum is NaN, and so is the whole).
+  auto factor = [&](float mi, float li) {
+    return mi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f((mi - m) * a.scale);
+  };
+  const float f0 = factor(m0, l0), f1 = factor(m1, l1);
+  float sum = f0 * l0 + f1 * l1;
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  if (wave == 0) lds_f[lane] = f0, lds_f[far] = f1;
+  __syncthreads();
+  float o[4] = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int i = wave; i < parts; i += 4) {
+    const float f = lds_f[i];
 #pragma unroll
     for (int j = 0; j < 4; j++)
-      if (lane + 64 * j < dim) o[j] += f * part[2 + lane + 64 * j];
+      if (lane + 64 * j < dim) o[j] = fmaf(f, p[(long)i * row + 2 + lane + 64 * j], o[j]);
   }
-  V *y = (V *)a.y + b * a.y_stride + (long)head * dim;
 #pragma unroll
-  for (int j = 0; j < 4; j++)
-    if (lane + 64 * j < dim) y[lane + 64 * j] = Num<T>::put(sum == 0.0f ? 0.0f : o[j] / sum);
+  for (int j = 0; j < 4; j++) lds_o[wave][lane + 64 * j] = o[j];
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d < dim) {
+    const float v = (lds_o[0][d] + lds_o[1][d]) + (lds_o[2][d] + lds_o[3][d]);
+    ((V *)a.y)[b * a.y_stride + (long)head * dim + d] = Num<T>::put(sum == 0.0f ? 0.0f : v / sum);
+  }
 }
 
 template <int T, int DP>
 void launch_parts(const PagedArgs &a, hipStream_t s) {
   const int per = a.heads / a.c.heads;
   const dim3 grid(a.splits, a.c.heads * ((per + 15) / 16), a.batch), block(64 * kWaves);
-  const bool even = a.c.dim % 8 == 0, paged16 = a.c.page_size % 16 == 0;
-  if (even && paged16)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, true, true>), grid, block, 0, s, a);
-  else if (even)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, true, false>), grid, block, 0, s, a);
+  const bool paged16 = a.c.page_size % 16 == 0;
+  if (a.c.dim == DP && paged16)
+    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, true>), grid, block, 0, s, a);
+  else if (a.c.dim == DP)
+    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, false>), grid, block, 0, s, a);
+  else if (a.c.dim % 8 == 0)
+    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_EVEN, false>), grid, block, 0, s, a);
   else
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, false, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_ANY, false>), grid, block, 0, s, a);
 }
 
 template <int T>
@@ -229,34 +323,43 @@ hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
     launch_parts<T, 256>(a, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((paged_attention_join<T>), dim3(a.heads, a.batch), dim3(64), 0, s, a);
+  hipLaunchKernelGGL((paged_attention_join<T>), dim3(a.heads, a.batch), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
-int paged_splits(int batch, int heads, int kv_heads, int type, long longest) {
-  // Enough workgroups to fill 256 CUs four times; a part has kLeastTiles
-  // tiles at least.
+PagedParts paged_parts(int batch, int heads, int kv_heads, int type, long longest) {
+  // Parts so long that, were all texts the longest, 4096 workgroups would come
+  // of it: eight times what the card holds at once, so that the last of them
+  // end together; but of 16 tiles (four a wave) at least, or of four where
+  // that leaves too few for the card. A text of 16 tiles is done without a
+  // join.
   const int keys = type == PPOCR_F32 ? 16 : 32, per = heads / kv_heads;
-  const long groups = (long)batch * kv_heads * ((per + 15) / 16);
-  const long most = (longest + (long)keys * kLeastTiles - 1) / ((long)keys * kLeastTiles);
-  const long want = (1024 + groups - 1) / groups;
-  const long n = want < most ? want : most;
-  return n < 1 ? 1 : n > 128 ? 128 : (int)n;
+  const long groups = (long)batch * kv_heads * ((per + 15) / 16), tiles = (longest + keys - 1) / keys + 2;
+  long each = (tiles * groups + 4095) / 4096;
+  if (each < 16) {
+    const long few = (tiles * groups + 511) / 512;
+    each = tiles <= 16 ? 16 : few < 4 ? 4 : few < 16 ? few : 16;
+  }
+  if (each < (tiles + kMostParts - 1) / kMostParts) each = (tiles + kMostParts - 1) / kMostParts;
+  const long splits = (tiles + each - 1) / each;
+  return {int(splits < 1 ? 1 : splits), int(each)};
 }
 
 hipError_t launch_kv_append(const AppendArgs &a, int type, hipStream_t s) {
-  // Waves: one a token where the texts' shares are even, up to 4096.
-  const long share = (a.rows + a.batch - 1) / a.batch;
-  long x = (share + 3) / 4;
-  const long most = 1024 / a.batch + 1;
-  if (x > most) x = most;
-  const dim3 grid(unsigned(x < 1 ? 1 : x), a.batch);
-  if (type == PPOCR_F32)
-    hipLaunchKernelGGL((kv_append_rows<uint32_t>), grid, dim3(256), 0, s, a);
+  // A token a wave where the texts' shares are even, up to 8192 waves.
+  const long share = (a.rows + a.batch - 1) / a.batch, most = 2048 / a.batch + 1;
+  const long x = std::min((share + 3) / 4, most);
+  const dim3 grid(unsigned(std::max(x, 1L)), a.batch);
+  if (type == PPOCR_F32 && a.c.dim % 4 == 0)
+    hipLaunchKernelGGL((kv_append_rows<uint32_t, true>), grid, dim3(256), 0, s, a);
+  else if (type == PPOCR_F32)
+    hipLaunchKernelGGL((kv_append_rows<uint32_t, false>), grid, dim3(256), 0, s, a);
+  else if (a.c.dim % 8 == 0)
+    hipLaunchKernelGGL((kv_append_rows<uint16_t, true>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((kv_append_rows<uint16_t>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv_append_rows<uint16_t, false>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -93,6 +93,7 @@ int cache_of(const Fail &fail, const char *what, const ppocr_kv_cache *k, const 
   }
   c.k = k->k, c.v = k->v;
   c.pages = int(k->pages), c.page_size = int(k->page_size), c.heads = int(k->heads), c.dim = int(k->dim);
+  c.by_page = Divide(c.page_size);
   c.table = table, c.table_width = long(table_width), c.lengths = lengths;
   return 0;
 }
@@ -125,7 +126,7 @@ int ppocr_hip_rms_norm(const void *x, size_t x_stride, const void *residual, siz
     return fail("rms norm: rows of %zu values with strides %zu, %zu, %zu, %zu", c, x_stride, residual_stride,
                 sum_stride, y_stride);
   a.x = x, a.residual = residual, a.weight = weight, a.sum = sum, a.y = y, a.scales = scales;
-  a.rows = long(rows), a.c = int(c), a.eps = eps;
+  a.rows = long(rows), a.c = int(c), a.eps = eps, a.inverse_c = float(1.0 / double(c));
   a.group = group && y8 ? int(group) : int(c);
   a.groups = int((c + a.group - 1) / a.group);
   const OnDevice on{hipStream_t(stream)};
@@ -196,7 +197,7 @@ size_t ppocr_hip_paged_attention_workspace(const ppocr_kv_cache *cache, size_t b
       batch > 65535 || !heads || heads > 65535 || heads % cache->heads)
     return 0;
   if (!longest || longest > (size_t(1) << 31)) longest = size_t(1) << 31;
-  const int n = paged_splits(int(batch), int(heads), int(cache->heads), cache->type, long(longest));
+  const int n = paged_parts(int(batch), int(heads), int(cache->heads), cache->type, long(longest)).splits;
   return n > 1 ? batch * heads * size_t(n) * (cache->dim + 2) * sizeof(float) : 0;
 }
 
@@ -219,12 +220,14 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
   if (!std::isfinite(scale)) return fail("paged attention: scale %g", double(scale));
   const size_t capacity = table_width * cache->page_size;
   if (!longest || longest > capacity) longest = capacity;
-  const size_t seen = window && window < longest ? window + sinks + 256 : longest;
-  int n = paged_splits(int(batch), int(heads), int(cache->heads), cache->type, long(seen < longest ? seen : longest));
+  const size_t seen = window && window < longest && sinks < longest ? window + sinks + 64 : longest;
+  const PagedParts parts =
+      paged_parts(int(batch), int(heads), int(cache->heads), cache->type, long(seen < longest ? seen : longest));
+  int n = parts.splits;
   const size_t a_part = batch * heads * (cache->dim + 2) * sizeof(float);
   const size_t most = workspace ? workspace_bytes / a_part : 0;
   if (size_t(n) > most) n = most > 1 ? int(most) : 1;
-  a.q = q, a.y = y, a.batch = int(batch), a.heads = int(heads), a.splits = n;
+  a.q = q, a.y = y, a.batch = int(batch), a.heads = int(heads), a.splits = n, a.each = parts.each;
   a.window = int(window < (size_t(1) << 31) - 1 ? window : 0);
   a.sinks = int(sinks < (size_t(1) << 30) ? sinks : size_t(1) << 30);
   a.scale = scale_of(scale), a.turn = scale < 0.0f;

@@ -80,7 +80,7 @@ struct NormArgs {
   long x_stride, residual_stride, sum_stride, y_stride;
   long rows;
   int c, groups, group;  // group: values a scale covers (c: the whole row)
-  float eps;
+  float eps, inverse_c;
 };
 hipError_t launch_rms_norm(const NormArgs &a, int type, int y_type, hipStream_t s);
 
@@ -102,10 +102,24 @@ hipError_t launch_q4_bf16(const Q4Args &a, int, hipStream_t s);
 hipError_t launch_q4_f16(const Q4Args &a, int, hipStream_t s);
 hipError_t launch_q4_i8(const Q4Args &a, int e4m3, hipStream_t s);
 
+// Division of 0 .. 2^31 - 1 by d: n / d = n mul >> shift.
+struct Divide {
+  uint32_t mul;
+  int shift, d;
+  Divide(int by = 1) : d(by) {
+    int l = 0;
+    while ((int64_t(1) << l) < by) l++;
+    shift = 31 + l;
+    mul = uint32_t(((uint64_t(1) << shift) + by - 1) / by);
+  }
+  __device__ __forceinline__ int operator()(int n) const { return int((uint64_t)(uint32_t)n * mul >> shift); }
+};
+
 struct CacheArgs {
   void *k, *v;
   long page_stride, token_stride, head_stride;
   int pages, page_size, heads, dim;
+  Divide by_page;
   const int *table;
   long table_width;
   const int *lengths;
@@ -126,14 +140,18 @@ struct PagedArgs {
   const void *q;
   void *y;
   long q_stride, y_stride;
-  int batch, heads, splits;
+  int batch, heads;
+  int splits, each;  // parts of a text at most, and tiles of one at least
   int window, sinks;  // window 0: every key is seen
   float scale;        // of 2-logarithms, positive
   bool turn;          // the given scale was negative: q turns its sign
   float *part;  // splits > 1: batch x heads x splits rows of dim + 2 floats
 };
-// The parts a text's cache of up to `longest` tokens is split into.
-int paged_splits(int batch, int heads, int kv_heads, int type, long longest);
+// The parts a text's cache of up to `longest` seen tokens is split into.
+struct PagedParts {
+  int splits, each;
+};
+PagedParts paged_parts(int batch, int heads, int kv_heads, int type, long longest);
 hipError_t launch_paged_attention(const PagedArgs &a, int type, hipStream_t s);
 
 struct PromptArgs {

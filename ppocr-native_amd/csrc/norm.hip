@@ -20,8 +20,19 @@ __device__ __forceinline__ float wave_sum(float v) {
   return v;
 }
 
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, false);
+}
+
+// The largest of each 4, 8, 16, 32 or 64 neighbouring lanes, in all of them.
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int lanes) {
-  for (int o = lanes >> 1; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  v = max(v, dpp<0xB1>(v));                    // lane ^ 1
+  v = max(v, dpp<0x4E>(v));                    // lane ^ 2
+  if (lanes >= 8) v = max(v, dpp<0x141>(v));   // lane i <-> 7 - i of 8
+  if (lanes >= 16) v = max(v, dpp<0x140>(v));  // lane i <-> 15 - i of 16
+  if (lanes >= 32) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  if (lanes >= 64) v = max(v, (uint32_t)__shfl_xor((int)v, 32));
   return v;
 }
 
@@ -53,7 +64,10 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t *lds) {
   return v;
 }
 
-constexpr float kTop8[2] = {448.0f, 127.0f};  // E4M3, I8
+// 1 / sqrt(v), to a step of f32 (the instruction takes normal numbers).
+__device__ __forceinline__ float inverse_root(float v) {
+  return v > 1e-37f ? __builtin_amdgcn_rsqf(v) : 1.0f / sqrtf(v);
+}
 
 // A group's scale from the bits of its largest |y|, and what to multiply y
 // with: 0 for a group whose scale would not be a normal number. Not finite:
@@ -63,36 +77,52 @@ __device__ __forceinline__ float scale8(uint32_t top, int i8, float &inverse) {
     inverse = 0.0f;
     return __uint_as_float(0x7fc00000u);
   }
-  const float s = __uint_as_float(top) / kTop8[i8];
-  inverse = s >= 1.17549435e-38f ? 1.0f / s : 0.0f;
-  return inverse != 0.0f ? s : 0.0f;
+  const float s = __uint_as_float(top) * (i8 ? 1.0f / 127.0f : 1.0f / 448.0f);
+  inverse = s >= 1.17549435e-38f ? __builtin_amdgcn_rcpf(s) : 0.0f;  // (a step of f32)
+  return s >= 1.17549435e-38f ? s : 0.0f;
 }
 
-// N values to their codes. `scale` NaN: the NaN code (E4M3) or 0 (I8).
+// N values to their codes, four a dword. `scale` NaN: the NaN code (E4M3) or 0.
 template <int N>
-__device__ __forceinline__ void codes8(const float (&y)[N], float inverse, float scale, int i8, uint8_t (&out)[N]) {
+__device__ __forceinline__ void codes8(const float (&y)[N], float inverse, float scale, int i8, uint32_t (&out)[N / 4]) {
   const bool bad = scale != scale;
-  if (i8) {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const float v = bad ? 0.0f : fminf(fmaxf(y[i] * inverse, -127.0f), 127.0f);
-      out[i] = (uint8_t)(int8_t)(int)rintf(v);
-    }
-  } else {
+  for (int i = 0; i < N; i += 4) {
+    uint32_t w;
+    if (i8) {
+      w = 0;
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float a = fminf(fmaxf(y[i] * inverse, -448.0f), 448.0f);
-      const float b = fminf(fmaxf(y[i + 1] * inverse, -448.0f), 448.0f);
-      const int p = bad ? 0x7f7f : __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-      out[i] = (uint8_t)p;
-      out[i + 1] = (uint8_t)(p >> 8);
+      for (int e = 0; e < 4; e++)
+        w |= (uint32_t)((int)rintf(__builtin_amdgcn_fmed3f(y[i + e] * inverse, -127.0f, 127.0f)) & 255) << 8 * e;
+      out[i / 4] = bad ? 0 : w;
+    } else {
+      float c[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_fmed3f(y[i + e] * inverse, -448.0f, 448.0f);
+      w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+      w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], (int)w, true);
+      out[i / 4] = bad ? 0x7f7f7f7fu : w;
     }
   }
 }
 
-// L lanes a row: 64 (four rows a workgroup) or the whole workgroup.
+template <int N>
+__device__ __forceinline__ void store_codes(uint8_t *p, long have, const uint32_t (&w)[N / 4]) {
+  if (have >= N) {
+    __builtin_memcpy(p, w, N);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+      if (i < have) p[i] = (uint8_t)(w[i / 4] >> 8 * (i % 4));
+  }
+}
+
+// L lanes a row: 64 (four rows a workgroup) or the whole workgroup. A vector a
+// lane (CH 1) wherever 1024 lanes hold a row: 8192 x 8192 of bf16 with the
+// residual ran at 4.2 TB/s with four vectors a lane, 4.7 with two, 5.2 with
+// one.
 template <int T, bool Y8, int L, int CH>
-__global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_rows(NormArgs a, int i8) {
+__global__ __launch_bounds__(L == 64 ? 256 : L) void rms_norm_rows(NormArgs a, int i8) {
   typedef num_t<T> V;
   constexpr int N = 16 / sizeof(V);
   __shared__ float lds[32];
@@ -132,7 +162,7 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_rows(NormArgs a, i
       q = fmaf(h[i][e], h[i][e], q);
     }
   q = row_sum<L>(q, lds);
-  const float r = 1.0f / sqrtf(q / (float)a.c + a.eps);
+  const float r = inverse_root(fmaf(q, a.inverse_c, a.eps));
 #pragma unroll
   for (int i = 0; i < CH; i++)
 #pragma unroll
@@ -154,8 +184,8 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_rows(NormArgs a, i
     for (int i = 0; i < CH; i++) {
       top[i] = 0;
 #pragma unroll
-      for (int e = 0; e < N; e++)  // values past the row's end are 0 (or NaN if r or the zeros' product is)
-        if ((i * L + lane) * N + e < a.c) top[i] = max(top[i], __float_as_uint(h[i][e]) & 0x7fffffffu);
+      for (int e = 0; e < N; e++)  // (past the row's end 0, or NaN where the whole row is)
+        top[i] = max(top[i], __float_as_uint(h[i][e]) & 0x7fffffffu);
       all = max(all, top[i]);
     }
     const bool whole = a.groups == 1;
@@ -166,9 +196,9 @@ __global__ __launch_bounds__(L < 256 ? 256 : L) void rms_norm_rows(NormArgs a, i
       float inverse;
       const float s = scale8(whole ? all : lanes_max(top[i], a.group / N), i8, inverse);
       if (whole ? i == 0 && lane == 0 : at < a.c && at % a.group == 0) scales[whole ? 0 : at / a.group] = s;
-      uint8_t o[N];
+      uint32_t o[N / 4];
       codes8(h[i], inverse, s, i8, o);
-      store_n(y + at, (long)a.c - at, o);
+      store_codes<N>(y + at, (long)a.c - at, o);
     }
   }
 }
@@ -210,7 +240,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long(NormArgs a, int i8) {
     for (int e = 0; e < N; e++) q = fmaf(Num<T>::get(v[e]), Num<T>::get(v[e]), q);
   }
   q = row_sum<L>(q, lds);
-  const float r = 1.0f / sqrtf(q / (float)a.c + a.eps);
+  const float r = inverse_root(fmaf(q, a.inverse_c, a.eps));
   auto load_y = [&](int at, float(&y)[N]) {
     V v[N], wv[N];
     load_h(at, v, false);
@@ -251,9 +281,9 @@ __global__ __launch_bounds__(1024) void rms_norm_long(NormArgs a, int i8) {
       const float s = scale8(whole ? all : lanes_max(top_of(at, y), a.group / N), i8, inverse);
       float *scales = a.scales + row * a.groups;
       if (whole ? at == 0 : at < a.c && at % a.group == 0) scales[whole ? 0 : at / a.group] = s;
-      uint8_t o[N];
+      uint32_t o[N / 4];
       codes8(y, inverse, s, i8, o);
-      store_n((uint8_t *)a.y + row * a.y_stride + at, (long)a.c - at, o);
+      store_codes<N>((uint8_t *)a.y + row * a.y_stride + at, (long)a.c - at, o);
     }
   }
 }
@@ -264,17 +294,17 @@ hipError_t launch(const NormArgs &a, int i8, hipStream_t s) {
   const int vecs = (a.c + N - 1) / N;  // 16-byte vectors a row
 #define NORM(L, CH)                                                                                          \
   hipLaunchKernelGGL((rms_norm_rows<T, Y8, L, CH>), dim3(unsigned(L == 64 ? (a.rows + 3) / 4 : a.rows)), \
-                     dim3(L < 256 ? 256 : L), 0, s, a, i8)
+                     dim3(L == 64 ? 256 : L), 0, s, a, i8)
   if (vecs <= 64)
     NORM(64, 1);
   else if (vecs <= 128)
-    NORM(64, 2);
+    NORM(128, 1);
   else if (vecs <= 256)
     NORM(256, 1);
   else if (vecs <= 512)
-    NORM(256, 2);
+    NORM(512, 1);
   else if (vecs <= 1024)
-    NORM(256, 4);
+    NORM(1024, 1);
   else if (vecs <= 2048)
     NORM(1024, 2);
   else if (vecs <= 4096)

@@ -102,9 +102,9 @@ __device__ __forceinline__ void attend_alone(const PromptArgs &a, const Block &b
 
 // 16 queries of one head, from the block's query `first` on, by one wave,
 // keys and values straight from memory (the caches): any type and dim.
-template <int T, int DP, bool EVEN>
+template <int T, int DP, int DIMS>
 __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl, int head, int first) {
-  typedef Attend<T, DP, EVEN> A;
+  typedef Attend<T, DP, DIMS> A;
   typedef typename A::V V;
   constexpr int K = A::KEYS;
   const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
@@ -134,10 +134,11 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
       const int j = k0 + i;
       return j <= last && (j >= low || j < a.sinks);
     };
-    bad |= at.template tile<true>(
-        [&](int i) -> const V * { return masked && !any(i) ? nullptr : k + (long)(k0 + i) * a.k_stride; },
-        [&](int i) -> const V * { return masked && !any(i) ? nullptr : v + (long)(k0 + i) * a.v_stride; }, seen,
-        masked, a.dim, a.scale, lane);
+    typename A::Tile tile;
+    A::load(
+        tile, [&](int i) { return k + (long)min(k0 + i, bl.nk - 1) * a.k_stride; },
+        [&](int i) { return v + (long)min(k0 + i, bl.nk - 1) * a.v_stride; }, a.dim, lane);
+    bad |= at.template use<true>(tile, seen, any, masked, a.dim, a.scale, lane);
   }
   if (__any(bad)) {
     attend_alone<T>(a, bl, head, first, rows);
@@ -157,14 +158,14 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
   }
 }
 
-template <int T, int DP, bool EVEN>
+template <int T, int DP, int DIMS>
 __global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
   Block bl;
   if (!find_block(a, blockIdx.y, 64, bl)) return;
   const int per = a.heads / a.kv_heads;
   const int first = bl.first + threadIdx.x / 64 * 16;
   if (first < bl.nq)
-    attend_rows<T, DP, EVEN>(a, bl, blockIdx.x % a.kv_heads * per + blockIdx.x / a.kv_heads, first);
+    attend_rows<T, DP, DIMS>(a, bl, blockIdx.x % a.kv_heads * per + blockIdx.x / a.kv_heads, first);
 }
 
 // ------------------------------------------------- 16-bit types, tiles in LDS
@@ -420,10 +421,12 @@ hipError_t launch_tiles(const PromptArgs &a, hipStream_t s) {
 template <int T, int DP>
 hipError_t launch_rows(const PromptArgs &a, hipStream_t s) {
   const dim3 grid(a.heads, a.rows_q / 64 + a.batch);
-  if (a.dim % 8 == 0)
-    hipLaunchKernelGGL((window_attention_rows<T, DP, true>), grid, dim3(256), 0, s, a);
+  if (a.dim == DP)
+    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_WHOLE>), grid, dim3(256), 0, s, a);
+  else if (a.dim % 8 == 0)
+    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_EVEN>), grid, dim3(256), 0, s, a);
   else
-    hipLaunchKernelGGL((window_attention_rows<T, DP, false>), grid, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_ANY>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 

@@ -11,6 +11,7 @@ a refused call raises `GpuError` with the library's reason.
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 from . import GpuError, lib
 
@@ -18,6 +19,16 @@ F32, BF16, F16, E4M3, I8 = range(5)
 
 _fns: dict = {}
 _ERR = 512
+
+
+class _Reason(threading.local):
+    """A thread's buffer for the reason of a refusal (made once: making it is a good part of a short call)."""
+
+    def __init__(self):
+        self.buffer = C.create_string_buffer(_ERR)
+
+
+_reason = _Reason()
 
 
 class KvCache(C.Structure):
@@ -57,9 +68,8 @@ def _functions() -> dict:
 
 
 def _call(name: str, *args) -> None:
-    fn = (_fns or _functions())[name]
-    err = C.create_string_buffer(_ERR)
-    if fn(*args, err, _ERR):
+    err = _reason.buffer
+    if (_fns or _functions())[name](*args, err, _ERR):
         raise GpuError(err.value.decode(errors="replace"))
 
 
