@@ -166,11 +166,14 @@ struct Attend {
 #pragma unroll
     for (int h = 0; h < H; h++) {
       s[h] = v4f{0, 0, 0, 0};
+      v4f s2[3] = {};  // F32: four sums, each of a quarter of the roundings
 #pragma unroll
       for (int c = 0; c < QC; c++) {
         if constexpr (F32) {
+          s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[h][c][0], q[c][0], s[h], 0, 0, 0);
 #pragma unroll
-          for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[h][c][j], q[c][j], s[h], 0, 0, 0);
+          for (int j = 0; j < 3; j++)
+            s2[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[h][c][j + 1], q[c][j + 1], s2[j], 0, 0, 0);
         } else {
           v4u a, b;
           __builtin_memcpy(&a, k[h][c], 16);
@@ -178,6 +181,7 @@ struct Attend {
           s[h] = Tile16<T>::mfma(a, b, s[h]);
         }
       }
+      if constexpr (F32) s[h] = (s[h] + s2[0]) + (s2[1] + s2[2]);
     }
     float top = -INFINITY;
 #pragma unroll

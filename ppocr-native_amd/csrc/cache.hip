@@ -252,7 +252,8 @@ __global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attent
 // parts i and i + 64's factors, wave w adds parts w, w + 4, ... of them.
 constexpr int kMostParts = 128;
 
-template <int T>
+// J: 64s of dim, rounded up to a power of two.
+template <int T, int J>
 __global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
   typedef num_t<T> V;
   __shared__ float lds_o[4][256], lds_f[kMostParts];
@@ -280,16 +281,16 @@ __global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
   if (wave == 0) lds_f[lane] = f0, lds_f[far] = f1;
   __syncthreads();
-  float o[4] = {0, 0, 0, 0};
-#pragma unroll 4
+  float o[J] = {};
+#pragma unroll 8
   for (int i = wave; i < parts; i += 4) {
     const float f = lds_f[i];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (lane + 64 * j < dim) o[j] = fmaf(f, p[(long)i * row + 2 + lane + 64 * j], o[j]);
+    for (int j = 0; j < J; j++)  // (past dim: its last value, not kept)
+      o[j] = fmaf(f, p[i * row + 2 + min(lane + 64 * j, dim - 1)], o[j]);
   }
 #pragma unroll
-  for (int j = 0; j < 4; j++) lds_o[wave][lane + 64 * j] = o[j];
+  for (int j = 0; j < J; j++) lds_o[wave][lane + 64 * j] = o[j];
   __syncthreads();
   const int d = threadIdx.x;
   if (d < dim) {
@@ -315,7 +316,9 @@ void launch_parts(const PagedArgs &a, hipStream_t s) {
 
 template <int T>
 hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
-  if (a.c.dim <= 64)
+  if (a.c.dim <= 32)
+    launch_parts<T, 32>(a, s);
+  else if (a.c.dim <= 64)
     launch_parts<T, 64>(a, s);
   else if (a.c.dim <= 128)
     launch_parts<T, 128>(a, s);
@@ -323,7 +326,13 @@ hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
     launch_parts<T, 256>(a, s);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((paged_attention_join<T>), dim3(a.heads, a.batch), dim3(256), 0, s, a);
+  const dim3 grid(a.heads, a.batch), block(256);
+  if (a.c.dim <= 64)
+    hipLaunchKernelGGL((paged_attention_join<T, 1>), grid, block, 0, s, a);
+  else if (a.c.dim <= 128)
+    hipLaunchKernelGGL((paged_attention_join<T, 2>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_attention_join<T, 4>), grid, block, 0, s, a);
   return hipGetLastError();
 }
 

@@ -122,9 +122,16 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
   const int sinks = min(a.sinks, low);                       // sinks before every window
   const int start = low / K * K, sink_tiles = min((sinks + K - 1) / K, start / K);
   const int tiles = sink_tiles + (last >= start ? (last - start) / K + 1 : 0);
+  auto tile_key = [&](int t) { return t < sink_tiles ? t * K : start + (t - sink_tiles) * K; };
+  auto load = [&](typename A::Tile &tile, int t) {
+    const int k0 = tile_key(t);
+    A::load(
+        tile, [&](int i) { return k + (long)min(k0 + i, bl.nk - 1) * a.k_stride; },
+        [&](int i) { return v + (long)min(k0 + i, bl.nk - 1) * a.v_stride; }, a.dim, lane);
+  };
   bool bad = false;
-  for (int t = 0; t < tiles; t++) {
-    const int k0 = t < sink_tiles ? t * K : start + (t - sink_tiles) * K;
+  auto use = [&](typename A::Tile &tile, int t) {
+    const int k0 = tile_key(t);
     const bool masked = k0 + K - 1 > p0 || (a.window && k0 <= last - a.window);
     auto seen = [&](int i) {
       const int j = k0 + i;
@@ -134,11 +141,16 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
       const int j = k0 + i;
       return j <= last && (j >= low || j < a.sinks);
     };
-    typename A::Tile tile;
-    A::load(
-        tile, [&](int i) { return k + (long)min(k0 + i, bl.nk - 1) * a.k_stride; },
-        [&](int i) { return v + (long)min(k0 + i, bl.nk - 1) * a.v_stride; }, a.dim, lane);
     bad |= at.template use<true>(tile, seen, any, masked, a.dim, a.scale, lane);
+  };
+  typename A::Tile ta, tb;
+  if (tiles > 0) load(ta, 0);
+  for (int t = 0; t < tiles; t += 2) {
+    if (t + 1 < tiles) load(tb, t + 1);
+    use(ta, t);
+    if (t + 1 >= tiles) break;
+    if (t + 2 < tiles) load(ta, t + 2);
+    use(tb, t + 1);
   }
   if (__any(bad)) {
     attend_alone<T>(a, bl, head, first, rows);
@@ -159,7 +171,7 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
 }
 
 template <int T, int DP, int DIMS>
-__global__ __launch_bounds__(256) void window_attention_rows(PromptArgs a) {
+__global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void window_attention_rows(PromptArgs a) {
   Block bl;
   if (!find_block(a, blockIdx.y, 64, bl)) return;
   const int per = a.heads / a.kv_heads;
@@ -443,6 +455,7 @@ hipError_t launch(const PromptArgs &a, hipStream_t s) {
       return launch_tiles<T, 256>(a, s);
     }
   }
+  if (a.dim <= 32) return launch_rows<T, 32>(a, s);
   if (a.dim <= 64) return launch_rows<T, 64>(a, s);
   if (a.dim <= 128) return launch_rows<T, 128>(a, s);
   return launch_rows<T, 256>(a, s);
