@@ -180,14 +180,18 @@ __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void window_attention_row
     attend_rows<T, DP, DIMS>(a, bl, blockIdx.x % a.kv_heads * per + blockIdx.x / a.kv_heads, first);
 }
 
-// ------------------------------------------------- 16-bit types, tiles in LDS
+// ------------------------------------------------------------- tiles in LDS
 
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-constexpr int kTileKeys = 64;
 constexpr int kTileWaves = 4;
+template <int T>
+constexpr int kTileKeys = T == PPOCR_F32 ? 32 : 64;
+// 16-byte pieces that a row of a tile has room for.
+template <int T, int DP>
+constexpr int kPieces = (DP <= 64 ? 8 : DP <= 128 ? 16 : 32) * (T == PPOCR_F32 ? 2 : 1);
 
 // Where a key's row of a tile keeps its 16-byte piece c: place c ^ turn(key),
 // so that both the 16 rows that a read of K touches at one piece and the four
@@ -198,29 +202,35 @@ __device__ __forceinline__ int turn(int key) {
   return C == 8 ? (key >> 1 & 1) << 2 | (key >> 2 & 3) : (key & 3) << 2 | (key >> 2 & 3);
 }
 
-// Whether a dword holds a 16-bit infinity or NaN.
+// Whether a dword holds an infinity or NaN.
 template <int T>
 __device__ __forceinline__ int not_finite2(uint32_t x) {
+  if constexpr (T == PPOCR_F32) return (x & 0x7f800000u) == 0x7f800000u;
   constexpr uint32_t lo = T == PPOCR_F16 ? 0x7c00u : 0x7f80u, hi = lo << 16;
   return ((x & lo) == lo ? 1 : 0) + ((x & hi) == hi ? 1 : 0);
 }
 
 // Four waves, each 32 queries of one head; `hg` heads of one key head (1, 2 or
-// 4) share the workgroup's tiles of 64 keys and values, which go straight from
-// memory to LDS, the next tile's while this one's are used. The products are
-// 32x32x16, the 32 queries the columns of each:
+// 4) share the workgroup's tiles of 64 keys and values (32 in f32), which go
+// straight from memory to LDS, the next tile's while this one's are used. The
+// 32 queries are the columns of each product:
 //   S^T[key][query] = K Q^T, O^T[d][query] += V^T P^T,
 // so that a lane holds one query's numbers: row maxima and sums need one
 // exchange between the wave's halves, and P goes from the first product's
-// result to the second's operand in its own lane, rounded to T, its keys in
-// the order 4 (lane / 32) + {0..3, 8..11}; V is read to match, transposed on
-// its way out of LDS.
+// result to the second's operand in its own lane, in 16 bits rounded to T, its
+// keys in the order 4 (lane / 32) + {0..3, 8..11}; V is read to match, in 16
+// bits transposed on its way out of LDS. In f32 the products take two inner
+// values at a time, and V's column d = E (lane % 32) + e is row lane % 32 of
+// product e. (With the keys of each wave's 16 queries read from memory in the
+// operand's order instead, f32 ran at 60 TFLOP/s: the address unit takes a
+// cycle a lane.)
 template <int T, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_attention_tiles(PromptArgs a, int hg) {
   typedef num_t<T> V;
-  constexpr int C = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;  // pieces of a row
-  constexpr int TILE = kTileKeys * C * 16;               // bytes
-  constexpr int KS = DP / 16, DB = DP / 32, PIECES = kTileKeys * C / (64 * kTileWaves);
+  constexpr bool F32 = T == PPOCR_F32;
+  constexpr int C = kPieces<T, DP>, KEYS = kTileKeys<T>, PN = 16 / sizeof(V);
+  constexpr int TILE = KEYS * C * 16;  // bytes
+  constexpr int KS = F32 ? DP / 8 : DP / 16, DB = DP / 32, PIECES = KEYS * C / (64 * kTileWaves), SB = KEYS / 32;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // [2][K, V][TILE]
   const int index = gridDim.y - 1 - blockIdx.y;  // the last block of a text, which sees most, first
   const int size = 32 * kTileWaves / hg;
@@ -239,12 +249,12 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
 
   // The tiles that the block sees: of sinks, then of the windows.
   const int low = a.window ? max(p_first - a.window + 1, 0) : 0;
-  const int sinks = min(a.sinks, low), start = low / kTileKeys * kTileKeys;
-  const int sink_tiles = min((sinks + kTileKeys - 1) / kTileKeys, start / kTileKeys);
-  const int tiles = sink_tiles + (p_last >= start ? (p_last - start) / kTileKeys + 1 : 0);
-  auto tile_key = [&](int t) { return t < sink_tiles ? t * kTileKeys : start + (t - sink_tiles) * kTileKeys; };
+  const int sinks = min(a.sinks, low), start = low / KEYS * KEYS;
+  const int sink_tiles = min((sinks + KEYS - 1) / KEYS, start / KEYS);
+  const int tiles = sink_tiles + (p_last >= start ? (p_last - start) / KEYS + 1 : 0);
+  auto tile_key = [&](int t) { return t < sink_tiles ? t * KEYS : start + (t - sink_tiles) * KEYS; };
 
-  const int pieces = a.dim / 8;  // WHOLE: C
+  const int pieces = a.dim / PN;  // WHOLE: C
   if (!WHOLE) {  // pieces past dim stay zero
     for (int i = tid; i < 4 * TILE / 16; i += 64 * kTileWaves) ((v4u *)lds)[i] = v4u{0, 0, 0, 0};
     __syncthreads();
@@ -256,24 +266,25 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
 #pragma unroll
     for (int i = 0; i < PIECES; i++) {
       const int e = (i * kTileWaves + wave) * 64 + lane, row = e / C, piece = (e % C) ^ turn<C>(row);
+      const int v_piece = F32 ? e % C : piece;  // (f32 rows of V are read along the row)
       const long key = min(k0 + row, bl.nk - 1);
       char *to = lds + buffer * 2 * TILE + (i * kTileWaves + wave) * 1024;
-      if (WHOLE || piece < pieces) {
-        __builtin_amdgcn_global_load_lds((const void *)(k_base + key * a.k_stride * 2 + piece * 16),
+      if (WHOLE || piece < pieces)
+        __builtin_amdgcn_global_load_lds((const void *)(k_base + key * a.k_stride * (long)sizeof(V) + piece * 16),
                                          (lds_void *)to, 16, 0, 0);
-        __builtin_amdgcn_global_load_lds((const void *)(v_base + key * a.v_stride * 2 + piece * 16),
+      if (WHOLE || v_piece < pieces)
+        __builtin_amdgcn_global_load_lds((const void *)(v_base + key * a.v_stride * (long)sizeof(V) + v_piece * 16),
                                          (lds_void *)(to + TILE), 16, 0, 0);
-      }
     }
   };
 
   v4u q[KS];
   {
     const V *row = (const V *)a.q + (long)(bl.q0 + query) * a.q_stride + (long)head * a.dim;
-    const uint32_t sign = a.turn ? 0x80008000u : 0u;
+    const uint32_t sign = a.turn ? (F32 ? 0x80000000u : 0x80008000u) : 0u;
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-      const int d = 16 * s + 8 * half;
+      const int d = PN * (2 * s + half);
       q[s] = v4u{0, 0, 0, 0};
       if (d < a.dim) __builtin_memcpy(&q[s], row + d, 16);
 #pragma unroll
@@ -297,27 +308,31 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
     if (t + 1 < tiles) load(t + 1, (t + 1) & 1);
     // Where some query does not see some key of the tile, an infinity or NaN
     // in V would reach it through its weight of 0.
-    if (k0 + kTileKeys - 1 > p_first || (a.window && k0 <= p_last - a.window)) {
+    if (k0 + KEYS - 1 > p_first || (a.window && k0 <= p_last - a.window)) {
 #pragma unroll
       for (int i = 0; i < PIECES; i++) {
         const v4u x = *(const v4u *)(vt + (i * 64 * kTileWaves + tid) * 16);
         bad |= not_finite2<T>(x[0]) + not_finite2<T>(x[1]) + not_finite2<T>(x[2]) + not_finite2<T>(x[3]);
       }
     }
-    const bool none = k0 > pw_last || (a.window && k0 + kTileKeys - 1 <= pw_first - a.window && k0 >= a.sinks);
+    const bool none = k0 > pw_last || (a.window && k0 + KEYS - 1 <= pw_first - a.window && k0 >= a.sinks);
     if (none || w0 >= bl.nq) continue;
-    const bool masked = k0 + kTileKeys - 1 > pw_first || (a.window && k0 <= pw_last - a.window);
+    const bool masked = k0 + KEYS - 1 > pw_first || (a.window && k0 <= pw_last - a.window);
 
-    v16f s[2];
+    v16f s[SB];
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < SB; b++) {
 #pragma unroll
       for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
       const char *row = kt + (32 * b + col) * C * 16;
 #pragma unroll
       for (int c = 0; c < KS; c++) {
         const v4u f = *(const v4u *)(row + ((2 * c + half) ^ turn<C>(col)) * 16);
-        if constexpr (T == PPOCR_F16)
+        if constexpr (F32) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+            s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(f[j]), __uint_as_float(q[c][j]), s[b], 0, 0, 0);
+        } else if constexpr (T == PPOCR_F16)
           s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f), __builtin_bit_cast(v8h, q[c]), s[b],
                                                         0, 0, 0);
         else
@@ -328,7 +343,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
     if (masked) {
       const int here = k0 + 4 * half, last = p - here, from = p_low - here, sunk = a.sinks - here;
 #pragma unroll
-      for (int b = 0; b < 2; b++)
+      for (int b = 0; b < SB; b++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
           const int j = 32 * b + 8 * (i / 4) + i % 4;
@@ -338,7 +353,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
     }
     float top = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+    for (int b = 0; b < SB; b++)
 #pragma unroll
       for (int i = 0; i < 16; i++) top = fmaxf(top, s[b][i]);
     top = fmaxf(top, __shfl_xor(top, 32));
@@ -355,38 +370,53 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
         for (int i = 0; i < 16; i++) o[b][i] *= shrink;
     }
     const float base = m == -INFINITY ? 0.0f : m * a.scale;
-    v4u pf[4];
+    if constexpr (F32) {
 #pragma unroll
-    for (int b = 0; b < 2; b++)
+      for (int i = 0; i < 16; i++) {
+        const float w = __builtin_amdgcn_exp2f(fmaf(s[0][i], a.scale, -base));
+        l += w;
+        float f[DB];
+        const float *at = (const float *)(vt + (8 * (i / 4) + 4 * half + i % 4) * C * 16) + DB * col;
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -base));
-        const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale, -base));
-        l += x + y;
-        pf[2 * b + i / 8][i / 2 % 4] = Tile16<T>::pack(x, y);
+        for (int b = 0; b < DB; b++) f[b] = at[b];
+#pragma unroll
+        for (int b = 0; b < DB; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(f[b], w, o[b], 0, 0, 0);
       }
+      continue;
+    } else {
+      v4u pf[4];
 #pragma unroll
-    for (int b = 0; b < DB; b++) {
+      for (int b = 0; b < SB; b++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        // Lane s of 16 names keys s / 4 of four and values 4 (s % 4) .. + 3 of
-        // 16, and gets value s of the four keys.
-        v4u f;
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-          const int key = 16 * c + 8 * g + 4 * half + lane % 16 / 4;
-          const int piece = 4 * b + 2 * (lane / 16 % 2) + lane % 4 / 2;
-          const char *at = vt + (key * C + (piece ^ turn<C>(key))) * 16 + lane % 2 * 8;
-          const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
-          f[2 * g] = __builtin_bit_cast(v2u, r)[0];
-          f[2 * g + 1] = __builtin_bit_cast(v2u, r)[1];
+        for (int i = 0; i < 16; i += 2) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -base));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale, -base));
+          l += x + y;
+          pf[2 * b + i / 8][i / 2 % 4] = Tile16<T>::pack(x, y);
         }
-        if constexpr (T == PPOCR_F16)
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f), __builtin_bit_cast(v8h, pf[c]),
-                                                        o[b], 0, 0, 0);
-        else
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, f), __builtin_bit_cast(v8bf, pf[c]),
-                                                         o[b], 0, 0, 0);
+#pragma unroll
+      for (int b = 0; b < DB; b++) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          // Lane s of 16 names keys s / 4 of four and values 4 (s % 4) .. + 3 of
+          // 16, and gets value s of the four keys.
+          v4u f;
+#pragma unroll
+          for (int g = 0; g < 2; g++) {
+            const int key = 16 * c + 8 * g + 4 * half + lane % 16 / 4;
+            const int piece = 4 * b + 2 * (lane / 16 % 2) + lane % 4 / 2;
+            const char *at = vt + (key * C + (piece ^ turn<C>(key))) * 16 + lane % 2 * 8;
+            const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)at);
+            f[2 * g] = __builtin_bit_cast(v2u, r)[0];
+            f[2 * g + 1] = __builtin_bit_cast(v2u, r)[1];
+          }
+          if constexpr (T == PPOCR_F16)
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, f), __builtin_bit_cast(v8h, pf[c]),
+                                                          o[b], 0, 0, 0);
+          else
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, f), __builtin_bit_cast(v8bf, pf[c]),
+                                                           o[b], 0, 0, 0);
+        }
       }
     }
   }
@@ -398,23 +428,34 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
   if (w0 + col >= bl.nq) return;
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   V *y = (V *)a.y + (long)(bl.q0 + query) * a.y_stride + (long)head * a.dim;
+  if constexpr (F32) {
 #pragma unroll
-  for (int b = 0; b < DB; b++)
+    for (int i = 0; i < 16; i++) {
+      float out[DB];
 #pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int d = 32 * b + 2 * i + 4 * half;
-      V out[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) out[e] = Num<T>::put(l == 0.0f ? 0.0f : o[b][i + e] * f);
+      for (int b = 0; b < DB; b++) out[b] = l == 0.0f ? 0.0f : o[b][i] * f;
+      const int d = DB * (8 * (i / 4) + 4 * half + i % 4);
       store_n(y + d, (long)a.dim - d, out);
     }
+  } else {
+#pragma unroll
+    for (int b = 0; b < DB; b++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = 32 * b + 2 * i + 4 * half;
+        V out[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) out[e] = Num<T>::put(l == 0.0f ? 0.0f : o[b][i + e] * f);
+        store_n(y + d, (long)a.dim - d, out);
+      }
+  }
 }
 
 template <int T, int DP, bool WHOLE>
 hipError_t launch_tiles_of(const PromptArgs &a, hipStream_t s) {
   const int per = a.heads / a.kv_heads, hg = per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1;
   const int size = 32 * kTileWaves / hg;
-  constexpr int bytes = 4 * kTileKeys * (DP <= 64 ? 8 : DP <= 128 ? 16 : 32) * 16;
+  constexpr int bytes = 4 * kTileKeys<T> * kPieces<T, DP> * 16;
   const void *kernel = (const void *)&window_attention_tiles<T, DP, WHOLE>;
   const hipError_t e = allow_lds(kernel, bytes);
   if (e != hipSuccess) return e;
@@ -444,16 +485,15 @@ hipError_t launch_rows(const PromptArgs &a, hipStream_t s) {
 
 template <int T>
 hipError_t launch(const PromptArgs &a, hipStream_t s) {
-  if constexpr (T != PPOCR_F32) {
-    // Loads to LDS move 16 aligned bytes.
-    auto a16 = [](const void *p, long stride) { return uintptr_t(p) % 16 == 0 && stride % 8 == 0; };
-    if (a.dim % 8 == 0 && a16(a.k, a.k_stride) && a16(a.v, a.v_stride)) {
-      if (a.dim <= 64) return launch_tiles<T, 64>(a, s);
-      if (a.dim <= 96) return launch_tiles<T, 96>(a, s);
-      if (a.dim <= 128) return launch_tiles<T, 128>(a, s);
-      if (a.dim <= 192) return launch_tiles<T, 192>(a, s);
-      return launch_tiles<T, 256>(a, s);
-    }
+  // Loads to LDS move 16 aligned bytes.
+  constexpr int N = 16 / sizeof(num_t<T>);
+  auto a16 = [](const void *p, long stride) { return uintptr_t(p) % 16 == 0 && stride % N == 0; };
+  if (a.dim % N == 0 && a.dim > 16 && a16(a.k, a.k_stride) && a16(a.v, a.v_stride)) {
+    if (a.dim <= 64) return launch_tiles<T, 64>(a, s);
+    if (a.dim <= 96) return launch_tiles<T, 96>(a, s);
+    if (a.dim <= 128) return launch_tiles<T, 128>(a, s);
+    if (a.dim <= 192) return launch_tiles<T, 192>(a, s);
+    return launch_tiles<T, 256>(a, s);
   }
   if (a.dim <= 32) return launch_rows<T, 32>(a, s);
   if (a.dim <= 64) return launch_rows<T, 64>(a, s);
