@@ -308,6 +308,8 @@ void launch_parts(const PagedArgs &a, hipStream_t s) {
     hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, true>), grid, block, 0, s, a);
   else if (a.c.dim == DP)
     hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, false>), grid, block, 0, s, a);
+  else if (a.c.dim % 8 == 0 && paged16)
+    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_EVEN, true>), grid, block, 0, s, a);
   else if (a.c.dim % 8 == 0)
     hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_EVEN, false>), grid, block, 0, s, a);
   else

@@ -130,7 +130,7 @@ constexpr int kRing = 3;
 // than there are), piece (quarter, row) at quarter * rows + (row ^ turn), turn
 // = the 8 inputs' number: so that neighbouring pieces of a row, written
 // together, lie in different banks; the weights' scales and 16 + zero points,
-// [group][output][2]; and 8-bit x's scales a group, [group][row].
+// [output][group][2]; and 8-bit x's scales a group, [group][row].
 struct Chunk {
   int stretches, log_stretches;  // a power of two, not fewer than the waves (one, too)
   int rows;
@@ -157,21 +157,23 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
   const int frag = 4 * ch.rows * 16, a_stretch = 4 * P * frag;  // bytes
   uint8_t *ring = lds + wave * kRing * 1024, *lds_x = lds + waves * kRing * 1024;
   v2f *lds_s = (v2f *)(lds_x + ch.stretches * a_stretch);
-  float *lds_xs = (float *)(lds_s + ch.stretches * SG * N);
+  const int s_row = ch.stretches * SG + 1;  // (one more: 16 outputs' scales lie in different banks)
+  float *lds_xs = (float *)(lds_s + N * s_row);
 
   // The ring's loads: the wave's next unit is tile l_tile of stretch l_step.
   // Piece p of row r has place 4 r + (p ^ turn), turn = r / 4 % 4: a read of 16
   // rows' pieces p touches every bank once. (Past a row's end or the last row
   // something else is read, which meets zeros of x or is not stored.)
   int l_step = wave, l_tile = 0, l_slot = 0;
-  const int l_at = 16 * ((lane ^ lane >> 4) & 3);
+  const int l_at = 16 * ((lane ^ lane >> 4) & 3), tile_bytes = 16 * row_bytes;  // (k is at most 2^24)
+  const uint8_t *l_from = q0 + wave * (kStretch / 2);  // of its row 0, in the common case
   const uint32_t l_off = (uint32_t)(lane / 4) * row_bytes + l_at;
+  const bool common = ch.align == 16 && n_here == N;
   auto load = [&] {
-    const int k2 = l_step * kStretch / 2;
+    const int k2 = l_step * (kStretch / 2);
     uint8_t *to = ring + l_slot * 1024;
-    if (ch.align == 16 && 16 * l_tile + 16 <= n_here && k2 + kStretch / 2 <= row_bytes) {
-      __builtin_amdgcn_global_load_lds((const void *)(q0 + ((long)(16 * l_tile) * row_bytes + k2) + l_off),
-                                       (lds_void *)to, 16, 0, 0);
+    if (common && k2 + kStretch / 2 <= row_bytes) {
+      __builtin_amdgcn_global_load_lds((const void *)(l_from + l_off), (lds_void *)to, 16, 0, 0);
     } else if (ch.align == 16) {
       const long row = min(16 * l_tile + lane / 4, n_here - 1);
       __builtin_amdgcn_global_load_lds((const void *)(q0 + row * row_bytes + (k2 + l_at < row_bytes ? k2 + l_at : 0)),
@@ -191,14 +193,17 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
       __builtin_memcpy(to + 16 * lane, b, 16);
     }
     l_slot = l_slot + 1 == kRing ? 0 : l_slot + 1;
-    if (++l_tile == NT) l_tile = 0, l_step += waves;
+    l_from += tile_bytes;
+    if (++l_tile == NT) l_tile = 0, l_step += waves, l_from += waves * (kStretch / 2) - (long)NT * tile_bytes;
   };
   // Waits until at most `ahead` later units are on their way.
   auto arrived = [&](int ahead) {
-    if (ch.align == 16)
-      ring_wait_chunks<1, kRing - 1>(ahead);
+    if (ch.align == 16 && ahead >= kRing - 1)
+      ring_wait<kRing - 1>();
+    else if (ch.align == 16)
+      ring_wait_chunks<1, kRing - 2>(ahead);
     else if (ch.align == 4)
-      ring_wait_chunks<4, kRing - 1>(ahead);
+      ring_wait_chunks<4, kRing - 1>(min(ahead, kRing - 1));
     asm volatile("" ::: "memory");
   };
 
@@ -250,7 +255,7 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
                         : a.scale_type == PPOCR_BF16 ? __uint_as_float(raw << 16)
                                                      : (float)__builtin_bit_cast(_Float16, (uint16_t)raw);
         if (j < sums)
-          lds_s[g * N + (j >> log_g)] = v2f{g0 + g < a.groups ? f : 0.0f, 16.0f + (float)(a.zeros ? z[u] : 8)};
+          lds_s[(j >> log_g) * s_row + g] = v2f{g0 + g < a.groups ? f : 0.0f, 16.0f + (float)(a.zeros ? z[u] : 8)};
       }
     }
     const int cut = a.k / 8 - first * 16;  // the piece that x's rows end in
@@ -312,13 +317,13 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
 #pragma unroll
       for (int j = 0; j < NT; j++) {
         units--;
-        arrived(min(units, kRing - 1));
+        arrived(units);
         uint32_t w[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) w[c] = *(const uint32_t *)(my_w + slot * 1024 + 16 * (c ^ col >> 2));
         v2f sz[SG];
 #pragma unroll
-        for (int g = 0; g < SG; g++) sz[g] = lds_s[(at * SG + g) * N + 16 * j + col];
+        for (int g = 0; g < SG; g++) sz[g] = lds_s[(16 * j + col) * s_row + at * SG + g];
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the slot has been read
         asm volatile("" ::: "memory");
         slot = slot + 1 == kRing ? 0 : slot + 1;
@@ -393,18 +398,19 @@ hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   while (ch.rows < 16 && ch.rows < a.m) ch.rows *= 2;
   constexpr int SG = kStretch / GROUP;
   const int a_stretch = 4 * XRow<X>::parts * 64 * ch.rows + SG * 16 * NT * 8 + (a.x_group ? SG * 64 : 0);
+  constexpr int once = 16 * NT * 8;  // the scales' extra column
   // Eight waves and two workgroups a CU, each with half its LDS; all of it
   // where there are not more workgroups than CUs. At least a stretch a wave.
   int waves = kWaves;
   const int room = (strips * (long)m_blocks <= 256 ? 152 : 76) * 1024;
-  while (waves > 1 && (waves / 2 >= steps || waves * (a_stretch + kRing * 1024) > 152 * 1024)) waves /= 2;
+  while (waves > 1 && (waves / 2 >= steps || waves * (a_stretch + kRing * 1024) + once > 152 * 1024)) waves /= 2;
   ch.stretches = waves;
-  while (ch.stretches < steps && waves * kRing * 1024 + 2 * ch.stretches * a_stretch <= room) ch.stretches *= 2;
+  while (ch.stretches < steps && waves * kRing * 1024 + 2 * ch.stretches * a_stretch + once <= room) ch.stretches *= 2;
   ch.log_stretches = __builtin_ctz(ch.stretches);
   auto kernel = &q4_rows<X, NT, GROUP, SB>;
   const hipError_t e = allow_lds((const void *)kernel, 160 * 1024);
   if (e != hipSuccess) return e;
-  const int bytes = std::max(waves * kRing * 1024 + ch.stretches * a_stretch, waves * 4096);
+  const int bytes = std::max(waves * kRing * 1024 + ch.stretches * a_stretch + once, waves * 4096);
   hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), bytes, s, a, e4m3, ch);
   return hipGetLastError();
 }
