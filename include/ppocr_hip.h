@@ -269,8 +269,8 @@ int ppocr_hip_rms_norm(const void *x, size_t x_stride, const void *residual, siz
  * E4M3 or I8; 8-bit x has x_scales: [m] (`x_group` 0) or
  * [m][ceil(k / group)] (`x_group` == group), as ppocr_hip_rms_norm writes
  * them. y_type F32, BF16 or F16. The weights' integers are multiplied exactly
- * and scaled in f32. k and x_stride up to 2^24. Made for up to 64 rows: more
- * read the weights again for every 64. An infinity in x gives NaN in its row. */
+ * and scaled in f32. k and x_stride up to 2^24. Made for up to 64 rows: every
+ * 16 read the weights again (from the L2 cache, where they fit). An infinity in x gives NaN in its row. */
 int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, size_t x_group, const uint8_t *q,
                          const void *scales, const uint8_t *zeros, const void *bias, void *y, size_t y_stride,
                          size_t m, size_t n, size_t k, size_t group, int x_type, int scale_type, int y_type,
@@ -327,7 +327,8 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
  * j <= p with j > p - window (`window` 0: all) or j < sinks; y is as above.
  * A query that sees no key gives zeros. Rows outside every text are left as
  * they were. `rows_q`, `rows_k`: the rows there are; starts are int32, not
- * decreasing, within them (rows past them are not touched). q and y: heads x
+ * decreasing, within them (rows past them are not touched), at most 2^24 rows of
+ * q, and heads x (rows_q / 32 + batch) below 2^24. q and y: heads x
  * dim a row, k and v: kv_heads x dim, dim up to 256, type F32, BF16 or F16.
  * What lies in keys that a query does not see does not matter to it. In BF16
  * and F16 the softmax's weights are rounded to the type before the product

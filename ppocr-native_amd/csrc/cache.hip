@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attent
     }
     if (lds_bad) sum = o = __uint_as_float(0x7fc00000u);
     if (split) {
-      float *p = a.part + ((long)(b * a.heads + h0 + row) * a.splits + blockIdx.x) * (a.c.dim + 2);
+      float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + blockIdx.x) * (a.c.dim + 2);
       p[d + 2] = o;
       if (d == 0) p[0] = m, p[1] = sum;
     } else {
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
                          T == PPOCR_F32 ? 16 : 32);
   const int each = tiles_a_part(s.tiles, a.each, a.splits);
   const int parts = max(1, (s.tiles + each - 1) / each), dim = a.c.dim, row = dim + 2;
-  const float *p = a.part + (long)(b * a.heads + head) * a.splits * row;
+  const float *p = a.part + ((long)b * a.heads + head) * a.splits * row;
   const float m0 = lane < parts ? p[(long)lane * row] : -INFINITY, l0 = lane < parts ? p[(long)lane * row + 1] : 0.0f;
   const int far = lane + 64;
   const float m1 = far < parts ? p[(long)far * row] : -INFINITY, l1 = far < parts ? p[(long)far * row + 1] : 0.0f;

@@ -50,7 +50,7 @@ struct OnDevice {
   }
 };
 
-constexpr size_t kMost = size_t(1) << 30;     // most rows, values a row and the like
+constexpr size_t kMost = size_t(1) << 30;  // most rows, values a row and the like
 constexpr size_t kMostStride = size_t(1) << 40;
 
 bool is_real(int t) { return t == PPOCR_F32 || t == PPOCR_BF16 || t == PPOCR_F16; }
@@ -146,7 +146,7 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
   if (group != 32 && group != 64 && group != 128)
     return fail("4-bit product: groups of %zu inputs: 32, 64 or 128 are taken", group);
   if (m == 0 || n == 0) return 0;
-  if (!k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20 || (n + 15) / 16 * ((m + 15) / 16) > size_t(1) << 26)
+  if (!k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20 || (n + 15) / 16 * ((m + 15) / 16) > size_t(1) << 24)
     return fail("4-bit product: %zu rows of %zu inputs to %zu outputs", m, k, n);
   if (!x || !q || !scales || !y || (x8 && !x_scales))
     return fail("4-bit product: x, q, scales, y and (for 8-bit x) x_scales are needed");
@@ -248,7 +248,8 @@ int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, si
     return fail("window attention: %zu query heads over %zu", heads, kv_heads);
   if (!dim || dim > 256) return fail("window attention: heads of %zu values: 1 to 256 are taken", dim);
   if (batch == 0 || rows_q == 0) return 0;
-  if (batch > 32768 || rows_q > (size_t(1) << 20) * 2 || rows_k > kMost)
+  // (A launch has fewer than 2^24 workgroups of 32 or more queries of a head.)
+  if (batch > 32768 || rows_q > size_t(1) << 24 || rows_k > kMost || heads * (rows_q / 32 + batch) >= size_t(1) << 24)
     return fail("window attention: %zu queries and %zu keys of %zu texts", rows_q, rows_k, batch);
   if (!q || !y || !starts_q || !starts_k || (rows_k && (!k || !v)))
     return fail("window attention: q, k, v, y and starts are needed");

@@ -289,7 +289,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long(NormArgs a, int i8) {
 }
 
 template <int T, bool Y8>
-hipError_t launch(const NormArgs &a, int i8, hipStream_t s) {
+hipError_t launch_some(const NormArgs &a, int i8, hipStream_t s) {
   constexpr int N = 16 / sizeof(num_t<T>);
   const int vecs = (a.c + N - 1) / N;  // 16-byte vectors a row
 #define NORM(L, CH)                                                                                          \
@@ -313,6 +313,23 @@ hipError_t launch(const NormArgs &a, int i8, hipStream_t s) {
     hipLaunchKernelGGL((rms_norm_long<T, Y8>), dim3(unsigned(a.rows)), dim3(1024), 0, s, a, i8);
 #undef NORM
   return hipGetLastError();
+}
+
+// A launch has fewer than 2^32 threads: 2^21 rows at a time.
+template <int T, bool Y8>
+hipError_t launch(NormArgs a, int i8, hipStream_t s) {
+  constexpr long most = 1L << 21;
+  constexpr size_t size = sizeof(num_t<T>), y_size = Y8 ? 1 : size;
+  auto on = [](auto *p, long rows, long stride, size_t each) { return p ? (char *)p + rows * stride * (long)each : nullptr; };
+  for (long left = a.rows; left > 0; left -= most) {
+    a.rows = left < most ? left : most;
+    const hipError_t e = launch_some<T, Y8>(a, i8, s);
+    if (e != hipSuccess || left <= most) return e;
+    a.x = on(a.x, most, a.x_stride, size), a.residual = on(a.residual, most, a.residual_stride, size);
+    a.sum = on(a.sum, most, a.sum_stride, size), a.y = on(a.y, most, a.y_stride, y_size);
+    a.scales = (float *)on(a.scales, most, a.groups, 4);
+  }
+  return hipSuccess;
 }
 
 }  // namespace

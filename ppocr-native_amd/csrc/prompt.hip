@@ -173,11 +173,10 @@ __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl
 template <int T, int DP, int DIMS>
 __global__ __launch_bounds__(256, (DP <= 128 ? 2 : 1)) void window_attention_rows(PromptArgs a) {
   Block bl;
-  if (!find_block(a, blockIdx.y, 64, bl)) return;
-  const int per = a.heads / a.kv_heads;
+  if (!find_block(a, blockIdx.x / a.heads, 64, bl)) return;
+  const int per = a.heads / a.kv_heads, x = blockIdx.x % a.heads;
   const int first = bl.first + threadIdx.x / 64 * 16;
-  if (first < bl.nq)
-    attend_rows<T, DP, DIMS>(a, bl, blockIdx.x % a.kv_heads * per + blockIdx.x / a.kv_heads, first);
+  if (first < bl.nq) attend_rows<T, DP, DIMS>(a, bl, x % a.kv_heads * per + x / a.kv_heads, first);
 }
 
 // ------------------------------------------------------------- tiles in LDS
@@ -232,14 +231,17 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
   constexpr int TILE = KEYS * C * 16;  // bytes
   constexpr int KS = F32 ? DP / 8 : DP / 16, DB = DP / 32, PIECES = KEYS * C / (64 * kTileWaves), SB = KEYS / 32;
   extern __shared__ __attribute__((aligned(1024))) char lds[];  // [2][K, V][TILE]
-  const int index = gridDim.y - 1 - blockIdx.y;  // the last block of a text, which sees most, first
+  // Workgroups in a row are a block's key heads (and the query heads of each,
+  // hg at a time): with eight, each XCD has its own, whose keys stay in its L2.
+  // The last block of a text, which sees most, comes first.
+  const int across = a.heads / hg, index = (gridDim.x - 1 - blockIdx.x) / across, x = blockIdx.x % across;
   const int size = 32 * kTileWaves / hg;
   Block bl;
   if (!find_block(a, index, size, bl)) return;
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int half = lane / 32, col = lane % 32;
-  const int per = a.heads / a.kv_heads, kv = blockIdx.x % a.kv_heads;
-  const int head = kv * per + blockIdx.x / a.kv_heads * hg + wave % hg;
+  const int per = a.heads / a.kv_heads, kv = x % a.kv_heads;
+  const int head = kv * per + x / a.kv_heads * hg + wave % hg;
   const int w0 = bl.first + wave / hg * 32;  // this wave's first query
   const int p_first = bl.nk - bl.nq + bl.first, p_last = bl.nk - bl.nq + min(bl.first + size, bl.nq) - 1;
   const int query = min(w0 + col, bl.nq - 1), p = bl.nk - bl.nq + query;
@@ -459,8 +461,10 @@ hipError_t launch_tiles_of(const PromptArgs &a, hipStream_t s) {
   const void *kernel = (const void *)&window_attention_tiles<T, DP, WHOLE>;
   const hipError_t e = allow_lds(kernel, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((window_attention_tiles<T, DP, WHOLE>), dim3(a.heads / hg, a.rows_q / size + a.batch),
-                     dim3(64 * kTileWaves), bytes, s, a, hg);
+  const long blocks = (a.heads / hg) * (a.rows_q / size + (long)a.batch);
+  if (blocks >= 1L << 24) return hipErrorInvalidConfiguration;
+  hipLaunchKernelGGL((window_attention_tiles<T, DP, WHOLE>), dim3(unsigned(blocks)), dim3(64 * kTileWaves), bytes, s, a,
+                     hg);
   return hipGetLastError();
 }
 
@@ -473,7 +477,9 @@ hipError_t launch_tiles(const PromptArgs &a, hipStream_t s) {
 
 template <int T, int DP>
 hipError_t launch_rows(const PromptArgs &a, hipStream_t s) {
-  const dim3 grid(a.heads, a.rows_q / 64 + a.batch);
+  const long blocks = a.heads * (a.rows_q / 64 + (long)a.batch);
+  if (blocks >= 1L << 24) return hipErrorInvalidConfiguration;
+  const dim3 grid{unsigned(blocks)};
   if (a.dim == DP)
     hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_WHOLE>), grid, dim3(256), 0, s, a);
   else if (a.dim % 8 == 0)

@@ -102,6 +102,10 @@ def prompt(**k):
     (prompt, dict(scale=float("nan")), "scale nan"),
     (prompt, dict(v_stride=100), "strides"),
     (prompt, dict(batch=40000), "40000 texts"),
+    (prompt, dict(rows_q=1 << 25), "queries"),
+    (product, dict(k=1 << 25), "inputs"),
+    (product, dict(x_stride=1 << 25), "strides"),
+    (product, dict(m=1 << 20, n=1 << 20), "outputs"),
 ])
 def test_refused(call, args, reason):
     with pytest.raises(GpuError, match=reason):

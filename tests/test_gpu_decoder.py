@@ -147,6 +147,35 @@ def test_product(x_type, m, n, k):
             run_product(rng, m, n, k, group, x_type, scale_type, D.F32, zeros, bias, x_group=group)
 
 
+@pytest.mark.parametrize("x_type", [D.F32, D.BF16, D.F16, D.E4M3])
+@pytest.mark.parametrize("m,n,k,group", [(3, 9000, 96, 32), (17, 8300, 200, 128), (2, 16500, 130, 64), (40, 5000, 64, 32),
+                                         (16, 32, 4160, 32), (16, 1000, 2100, 32)])
+def test_product_many_tiles(x_type, m, n, k, group):
+    # Two and four tiles a workgroup, blocks of rows, several chunks of x.
+    y_type = x_type if x_type in R.REAL else D.F16
+    run_product(np.random.default_rng(n), m, n, k, group, x_type, D.F16, y_type, True, False,
+                x_group=group if x_type == D.E4M3 else 0)
+
+
+def test_product_at_any_address():
+    # Weights, scales and x that start at any address of their own type's alignment.
+    m, n, k = 3, 50, 512
+    rng = np.random.default_rng(6)
+    q, x = rng.integers(0, 16, (n, k)), R.stored(rng.normal(0, 1, (m, k)), D.F16)
+    s = R.stored(rng.uniform(0.5, 1.5, (n, 8)) / 64, D.BF16)
+    for off in (1, 2, 4, 16):
+        dq = R.on_gpu(np.concatenate([np.zeros(off, np.uint8), R.packed(q).reshape(-1)]))
+        ds, dx = (R.on_gpu(np.concatenate([np.zeros(1, a.dtype), a.reshape(-1)])) for a in (s, x))
+        dy = R.on_gpu(np.zeros((m, n), np.float32))
+        print(f"product with weights {off} bytes off", flush=True)
+        D.q4_product(dx.addr + 2, dq.addr + off, ds.addr + 2, dy.addr, m, n, k, group=64, x_type=D.F16,
+                     scale_type=D.BF16, y_type=D.F32)
+        synchronize()
+        want, size = R.product(R.values(x, D.F16), q, R.values(s, D.BF16), None, 64)
+        R.close(R.back(dy, np.float32, (m, n)).astype(np.float64), want,
+                R.half_step(want, D.F32) + 16 * STEP * size)
+
+
 def test_product_keeps_rows_apart():
     # A NaN or infinity in one row of x leaves the others' results alone, and q's bytes past an odd row's end do not matter.
     m, n, k = 5, 40, 131
@@ -243,10 +272,10 @@ def test_append_leaves_what_is_out_of_range():
 # ------------------------------------------------------ the decode attention
 
 def run_paged(rng, lengths, page, heads, kv_heads, dim, t, window=0, sinks=0, layout="tokens", work=1 << 22, gap=0,
-              longest=0):
+              longest=0, scale=None):
     p = pages_of(rng, lengths, page, kv_heads, dim, t, layout)
     cache = p.upload()
-    batch, scale = len(lengths), 1.3 * dim ** -0.5
+    batch, scale = len(lengths), 1.3 * dim ** -0.5 if scale is None else scale
     q = R.stored(rng.normal(0, 2, (batch, heads * dim + gap)), t)
     dq, dl = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32))
     dy, dw = R.on_gpu(np.zeros((batch, heads * dim + gap), R.dtype(t))), R.on_gpu(np.full(max(work, 4), 0xFF, np.uint8))
@@ -314,6 +343,31 @@ def test_paged_window_over_evicted_pages():
         R.close(R.values(R.back(dy, np.float16, (1, 64)), D.F16), y, R.attention_bound(y, size, reach, D.F16, False))
 
 
+@pytest.mark.parametrize("t", [D.F32, D.F16])
+def test_cache_far_offsets(t):
+    # Pages further apart than 32 bits of values: append and attention.
+    heads, dim, page, stride = 2, 64, 16, (1 << 30) + 64
+    rng = np.random.default_rng(1)
+    size = np.dtype(R.dtype(t)).itemsize
+    far = [R.DeviceArray(size * (4 * stride + 65536)) for _ in range(2)]
+    cache = D.KvCache(far[0].addr, far[1].addr, 5, page, heads, dim, t, stride, heads * dim, dim)
+    table = np.array([[4, 2, 3]], np.int32)
+    k, v = (R.stored(rng.normal(0, 1, (40, heads, dim)), t) for _ in range(2))
+    q = R.stored(rng.normal(0, 2, (1, heads, dim)), t)
+    dk, dv, dq, dt = R.on_gpu(k), R.on_gpu(v), R.on_gpu(q), R.on_gpu(table)
+    dl, ds = R.on_gpu(np.array([40], np.int32)), R.on_gpu(np.array([0, 40], np.int32))
+    dy = R.on_gpu(np.zeros((heads, dim), R.dtype(t)))
+    print("a cache past 32 bits", flush=True)
+    D.kv_append(dk.addr, dv.addr, cache, dt.addr, 3, dl.addr, 1, 40, starts=ds.addr)
+    D.paged_attention(dq.addr, cache, dt.addr, 3, dl.addr, dy.addr, 1, heads, scale=0.125)
+    synchronize()
+    got = R.values(R.back(dy, R.dtype(t), (heads, dim)), t)
+    for h in range(heads):
+        y, s, reach = R.attend(R.values(q[:, h], t), R.values(k[:, h], t), R.values(v[:, h], t),
+                               np.ones((1, 40), bool), 0.125)
+        R.close(got[h:h + 1], y, R.attention_bound(y, s, reach, t, False))
+
+
 @pytest.mark.parametrize("page", [16, 10])
 @pytest.mark.parametrize("work", [0, 1 << 22])
 def test_paged_bad_pages(page, work):
@@ -337,10 +391,11 @@ def test_paged_bad_pages(page, work):
 
 # ------------------------------------------------------ the prompt attention
 
-def run_prompt(rng, nq, nk, heads, kv_heads, dim, t, window, sinks, fused=False, poison=()):
-    """`fused`: q, k and v in one buffer, a row's behind one another. `poison`: (text, key) whose k and v are NaN."""
-    rows_q, rows_k = sum(nq), sum(nk)
-    scale = 1.2 * dim ** -0.5
+def run_prompt(rng, nq, nk, heads, kv_heads, dim, t, window, sinks, fused=False, poison=(), scale=None, odd=0):
+    """`fused`: q, k and v in one buffer, a row's behind one another, `odd` values more. `poison`: (text, key) whose k
+    and v are NaN."""
+    rows_q, rows_k = int(sum(nq)), int(sum(nk))
+    scale = 1.2 * dim ** -0.5 if scale is None else scale
     q, k, v = (R.stored(rng.normal(0, s, (n + 3, h, dim)), t)
                for n, h, s in ((rows_q, heads, 2), (rows_k, kv_heads, 1), (rows_k, kv_heads, 1)))
     nan = R.stored(np.full(dim, np.nan, np.float32), t)
@@ -353,7 +408,7 @@ def run_prompt(rng, nq, nk, heads, kv_heads, dim, t, window, sinks, fused=False,
     print(f"prompt {nq} of {nk} heads {heads}/{kv_heads} dim {dim} type {t} window {window} sinks {sinks} "
           f"fused {fused}", flush=True)
     if fused:
-        both = np.concatenate([a.reshape(a.shape[0], -1) for a in (q, k, v)], 1)
+        both = np.concatenate([a.reshape(a.shape[0], -1) for a in (q, k, v)] + [np.zeros((rows_q + 3, odd), R.dtype(t))], 1)
         d, width, size = R.on_gpu(both), both.shape[1], np.dtype(R.dtype(t)).itemsize
         at = [d.addr, d.addr + heads * dim * size, d.addr + (heads + kv_heads) * dim * size]
         strides = dict(q_stride=width, k_stride=width, v_stride=width)
@@ -395,6 +450,30 @@ def test_prompt(t, heads, kv_heads, dim, nq, nk):
                                           (5000, 2)])
 def test_prompt_window(t, window, sinks):
     run_prompt(np.random.default_rng(window), [290, 70], [400, 70], 2, 1, 64, t, window, sinks)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [8, 20, 32, 64, 96, 128, 256])
+def test_prompt_any_stride(t, dim):
+    # Rows that do not start at 16 bytes, and rows that do.
+    for odd in (1, 0):
+        run_prompt(np.random.default_rng(dim), [100, 40], [100, 40], 4, 2, dim, t, 30, 3, fused=True, odd=odd)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_scales_below_0_and_0(t, scale):
+    for dim in (64, 15):
+        run_prompt(np.random.default_rng(dim), [70, 5], [70, 9], 2, 1, dim, t, 20, 2, scale=scale)
+    run_paged(np.random.default_rng(3), [90, 1, 0], 16, 2, 1, 64, t, scale=scale)
+    run_paged(np.random.default_rng(3), [90, 1, 0], 16, 2, 1, 64, t, 20, 2, scale=scale)
+
+
+def test_prompt_many_texts():
+    # More texts than a wave has lanes, some of them empty.
+    rng = np.random.default_rng(7)
+    nq = rng.integers(0, 9, 200).tolist()
+    run_prompt(rng, nq, nq, 2, 1, 64, D.F16, 4, 1)
 
 
 @pytest.mark.parametrize("t", R.REAL)
@@ -543,6 +622,29 @@ def test_a_step_captured():
         synchronize()
         for x, y in zip(a.outputs(), b.outputs()):
             assert np.array_equal(x.view(np.uint8), y.view(np.uint8))
+
+
+def test_two_threads_at_once():
+    # Calls and refusals from two threads: each its own results and reasons.
+    import threading
+    steps, said = [Step(np.random.default_rng(40 + i), held=100 + 200 * i) for i in range(2)], [[], []]
+
+    def work(i):
+        for n in range(20):
+            steps[i].run()
+            try:
+                D.q4_product(16, 16, 16, 16, 1, 1, 1, group=1000 + i)
+            except Exception as e:
+                said[i].append(str(e))
+
+    print("two threads", flush=True)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    synchronize()
+    for i in range(2):
+        steps[i].check()
+        assert len(said[i]) == 20 and all(f"groups of {1000 + i} " in s for s in said[i])
 
 
 def test_two_streams_at_once():
