@@ -51,8 +51,6 @@ __device__ __forceinline__ void cut_dims(int d, int dim, V (&v)[N]) {
 // 16-bit types: 32 keys a tile, inner index 32.
 template <int T>
 struct Tile16 {
-  typedef num_t<T> V;
-  static constexpr int keys = 32;
   static __device__ __forceinline__ v4f mfma(v4u a, v4u b, v4f c) {
     if constexpr (T == PPOCR_F16)
       return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0,

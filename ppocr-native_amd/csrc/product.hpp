@@ -26,8 +26,15 @@
 // x, the scales and the zero points are the same for all of a workgroup's
 // waves, or come in rows too short to load well: they go to LDS a chunk of
 // stretches at a time, x as finished operands.
+//
+// 4096 inputs to 28672 outputs (59 to 71 MB): one row of bf16, groups of 128,
+// 17.5 us, 3.5 TB/s; 16 rows of f16, groups of 32 with zero points, 26 us, 2.7
+// TB/s, of which the vector units are busy half; 5 rows of f32 40 us. What is
+// left is the wait at each chunk's start. Fetching a chunk's x ahead into
+// registers spilled (43 us); tiles of 32 and 64 rows of x were slower than
+// blocks of 16 that share the weights through L2 (64 rows of f32: 715 us
+// against 171).
 #include <algorithm>
-#include <type_traits>
 
 #include "decoder.hpp"
 #include "kernels.hpp"
