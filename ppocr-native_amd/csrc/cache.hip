@@ -36,9 +36,10 @@ __global__ __launch_bounds__(256) void kv_append_rows(AppendArgs a) {
   const long count = last - first;
   const int end = a.c.lengths[b];
   const int pieces = (a.c.dim + N - 1) / N, all = a.c.heads * pieces;
-  for (long i = wave; i < count; i += waves) {
+  // Those that have a row and a place: starts and lengths may say anything.
+  const long begin = max(max(0L, -first), count - end), stop = min(count, a.rows - first);
+  for (long i = begin + wave; i < stop; i += waves) {
     const long row = first + i, at = end - count + i;
-    if (row < 0 || row >= a.rows || at < 0) continue;
     const int slot = a.c.by_page((int)at);  // (at < end, an int)
     if (slot >= a.c.table_width) continue;
     const int page = a.c.table[b * a.c.table_width + slot];
@@ -304,42 +305,28 @@ __global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
 }
 
 template <int T, int DP>
-void launch_parts(const PagedArgs &a, hipStream_t s) {
+hipError_t launch_parts(const PagedArgs &a, hipStream_t s) {
   const int per = a.heads / a.c.heads;
   const dim3 grid(a.splits, a.c.heads * ((per + 15) / 16), a.batch), block(64 * kWaves);
   const bool paged16 = a.c.page_size % 16 == 0;
-  if (a.c.dim == DP && paged16)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, true>), grid, block, 0, s, a);
-  else if (a.c.dim == DP)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_WHOLE, false>), grid, block, 0, s, a);
-  else if (a.c.dim % 8 == 0 && paged16)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_EVEN, true>), grid, block, 0, s, a);
-  else if (a.c.dim % 8 == 0)
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_EVEN, false>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((paged_attention_parts<T, DP, DIMS_ANY, false>), grid, block, 0, s, a);
+  if (a.c.dim == DP && paged16) return launch_kernel(paged_attention_parts<T, DP, DIMS_WHOLE, true>, grid, block, 0, s, a);
+  if (a.c.dim == DP) return launch_kernel(paged_attention_parts<T, DP, DIMS_WHOLE, false>, grid, block, 0, s, a);
+  if (a.c.dim % 8 == 0 && paged16) return launch_kernel(paged_attention_parts<T, DP, DIMS_EVEN, true>, grid, block, 0, s, a);
+  if (a.c.dim % 8 == 0) return launch_kernel(paged_attention_parts<T, DP, DIMS_EVEN, false>, grid, block, 0, s, a);
+  return launch_kernel(paged_attention_parts<T, DP, DIMS_ANY, false>, grid, block, 0, s, a);
 }
 
 template <int T>
 hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
-  if (a.c.dim <= 32)
-    launch_parts<T, 32>(a, s);
-  else if (a.c.dim <= 64)
-    launch_parts<T, 64>(a, s);
-  else if (a.c.dim <= 128)
-    launch_parts<T, 128>(a, s);
-  else
-    launch_parts<T, 256>(a, s);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = a.c.dim <= 32    ? launch_parts<T, 32>(a, s)
+                       : a.c.dim <= 64  ? launch_parts<T, 64>(a, s)
+                       : a.c.dim <= 128 ? launch_parts<T, 128>(a, s)
+                                        : launch_parts<T, 256>(a, s);
   if (e != hipSuccess || a.splits == 1) return e;
   const dim3 grid(a.heads, a.batch), block(256);
-  if (a.c.dim <= 64)
-    hipLaunchKernelGGL((paged_attention_join<T, 1>), grid, block, 0, s, a);
-  else if (a.c.dim <= 128)
-    hipLaunchKernelGGL((paged_attention_join<T, 2>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((paged_attention_join<T, 4>), grid, block, 0, s, a);
-  return hipGetLastError();
+  if (a.c.dim <= 64) return launch_kernel(paged_attention_join<T, 1>, grid, block, 0, s, a);
+  if (a.c.dim <= 128) return launch_kernel(paged_attention_join<T, 2>, grid, block, 0, s, a);
+  return launch_kernel(paged_attention_join<T, 4>, grid, block, 0, s, a);
 }
 
 }  // namespace
@@ -367,15 +354,12 @@ hipError_t launch_kv_append(const AppendArgs &a, int type, hipStream_t s) {
   const long share = (a.rows + a.batch - 1) / a.batch, most = 2048 / a.batch + 1;
   const long x = std::min((share + 3) / 4, most);
   const dim3 grid(unsigned(std::max(x, 1L)), a.batch);
+  const dim3 block(256);
   if (type == PPOCR_F32 && a.c.dim % 4 == 0)
-    hipLaunchKernelGGL((kv_append_rows<uint32_t, true>), grid, dim3(256), 0, s, a);
-  else if (type == PPOCR_F32)
-    hipLaunchKernelGGL((kv_append_rows<uint32_t, false>), grid, dim3(256), 0, s, a);
-  else if (a.c.dim % 8 == 0)
-    hipLaunchKernelGGL((kv_append_rows<uint16_t, true>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((kv_append_rows<uint16_t, false>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+    return launch_kernel(kv_append_rows<uint32_t, true>, grid, block, 0, s, a);
+  if (type == PPOCR_F32) return launch_kernel(kv_append_rows<uint32_t, false>, grid, block, 0, s, a);
+  if (a.c.dim % 8 == 0) return launch_kernel(kv_append_rows<uint16_t, true>, grid, block, 0, s, a);
+  return launch_kernel(kv_append_rows<uint16_t, false>, grid, block, 0, s, a);
 }
 
 hipError_t launch_paged_attention(const PagedArgs &a, int type, hipStream_t s) {

@@ -266,7 +266,7 @@ int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, si
   a.q = q, a.k = k, a.v = v, a.y = y, a.starts_q = starts_q, a.starts_k = starts_k;
   a.batch = int(batch), a.rows_q = int(rows_q), a.rows_k = int(rows_k);
   a.heads = int(heads), a.kv_heads = int(kv_heads), a.dim = int(dim);
-  a.window = int(window < (size_t(1) << 31) - 1 ? window : 0);
+  a.window = int(window < rows_k ? window : 0);  // (no text has more keys)
   a.sinks = int(sinks < (size_t(1) << 30) ? sinks : size_t(1) << 30);
   a.scale = scale_of(scale), a.turn = scale < 0.0f;
   const OnDevice on{hipStream_t(stream)};

@@ -9,9 +9,34 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "ppocr_hip.h"
 
 namespace ppocr {
+
+// A launch whose own status is returned: the thread's last error may be that
+// of another call.
+template <class... P>
+hipError_t launch_kernel(void (*kernel)(P...), dim3 grid, dim3 block, int lds, hipStream_t s, P... args) {
+  void *at[] = {&args...};
+  return hipLaunchKernel((const void *)kernel, grid, block, at, size_t(lds), s);
+}
+
+// Allows `bytes` of LDS to a kernel on the current device: once, for always the
+// same number.
+template <auto Kernel>
+hipError_t allow_lds_of(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int dev = 0;
+  hipError_t e = hipGetDevice(&dev);
+  if (e != hipSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if (done.load(std::memory_order_acquire) & bit) return hipSuccess;
+  e = hipFuncSetAttribute((const void *)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == hipSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
 
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));

@@ -294,27 +294,18 @@ template <int T, bool Y8>
 hipError_t launch_some(const NormArgs &a, int i8, hipStream_t s) {
   constexpr int N = 16 / sizeof(num_t<T>);
   const int vecs = (a.c + N - 1) / N;  // 16-byte vectors a row
-#define NORM(L, CH)                                                                                          \
-  hipLaunchKernelGGL((rms_norm_rows<T, Y8, L, CH>), dim3(unsigned(L == 64 ? (a.rows + 3) / 4 : a.rows)), \
-                     dim3(L == 64 ? 256 : L), 0, s, a, i8)
-  if (vecs <= 64)
-    NORM(64, 1);
-  else if (vecs <= 128)
-    NORM(128, 1);
-  else if (vecs <= 256)
-    NORM(256, 1);
-  else if (vecs <= 512)
-    NORM(512, 1);
-  else if (vecs <= 1024)
-    NORM(1024, 1);
-  else if (vecs <= 2048)
-    NORM(1024, 2);
-  else if (vecs <= 4096)
-    NORM(1024, 4);
-  else
-    hipLaunchKernelGGL((rms_norm_long<T, Y8>), dim3(unsigned(a.rows)), dim3(1024), 0, s, a, i8);
+#define NORM(L, CH)                                                                                         \
+  return launch_kernel(rms_norm_rows<T, Y8, L, CH>, dim3(unsigned(L == 64 ? (a.rows + 3) / 4 : a.rows)), \
+                       dim3(L == 64 ? 256 : L), 0, s, a, i8)
+  if (vecs <= 64) NORM(64, 1);
+  if (vecs <= 128) NORM(128, 1);
+  if (vecs <= 256) NORM(256, 1);
+  if (vecs <= 512) NORM(512, 1);
+  if (vecs <= 1024) NORM(1024, 1);
+  if (vecs <= 2048) NORM(1024, 2);
+  if (vecs <= 4096) NORM(1024, 4);
 #undef NORM
-  return hipGetLastError();
+  return launch_kernel(rms_norm_long<T, Y8>, dim3(unsigned(a.rows)), dim3(1024), 0, s, a, i8);
 }
 
 // A launch has fewer than 2^32 threads: 2^21 rows at a time.

@@ -414,12 +414,10 @@ hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   ch.stretches = waves;
   while (ch.stretches < steps && waves * kRing * 1024 + 2 * ch.stretches * a_stretch + once <= room) ch.stretches *= 2;
   ch.log_stretches = __builtin_ctz(ch.stretches);
-  auto kernel = &q4_rows<X, NT, GROUP, SB>;
-  const hipError_t e = allow_lds((const void *)kernel, 160 * 1024);
+  const hipError_t e = allow_lds_of<&q4_rows<X, NT, GROUP, SB>>(160 * 1024);
   if (e != hipSuccess) return e;
   const int bytes = std::max(waves * kRing * 1024 + ch.stretches * a_stretch + once, waves * 4096);
-  hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), bytes, s, a, e4m3, ch);
-  return hipGetLastError();
+  return launch_kernel(q4_rows<X, NT, GROUP, SB>, grid, dim3(64 * waves), bytes, s, a, e4m3, ch);
 }
 
 template <int X, int NT, int GROUP>

@@ -472,14 +472,12 @@ hipError_t launch_tiles_of(const PromptArgs &a, hipStream_t s) {
   const int per = a.heads / a.kv_heads, hg = per % 4 == 0 ? 4 : per % 2 == 0 ? 2 : 1;
   const int size = 32 * kTileWaves / hg;
   constexpr int bytes = 4 * kTileKeys<T> * kPieces<T, DP> * 16;
-  const void *kernel = (const void *)&window_attention_tiles<T, DP, WHOLE>;
-  const hipError_t e = allow_lds(kernel, bytes);
+  const hipError_t e = allow_lds_of<&window_attention_tiles<T, DP, WHOLE>>(bytes);
   if (e != hipSuccess) return e;
   const long blocks = (a.heads / hg) * (a.rows_q / size + (long)a.batch);
   if (blocks >= 1L << 24) return hipErrorInvalidConfiguration;
-  hipLaunchKernelGGL((window_attention_tiles<T, DP, WHOLE>), dim3(unsigned(blocks)), dim3(64 * kTileWaves), bytes, s, a,
-                     hg);
-  return hipGetLastError();
+  return launch_kernel(window_attention_tiles<T, DP, WHOLE>, dim3(unsigned(blocks)), dim3(64 * kTileWaves), bytes, s, a,
+                       hg);
 }
 
 template <int T, int DP>
@@ -493,14 +491,10 @@ template <int T, int DP>
 hipError_t launch_rows(const PromptArgs &a, hipStream_t s) {
   const long blocks = a.heads * (a.rows_q / 64 + (long)a.batch);
   if (blocks >= 1L << 24) return hipErrorInvalidConfiguration;
-  const dim3 grid{unsigned(blocks)};
-  if (a.dim == DP)
-    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_WHOLE>), grid, dim3(256), 0, s, a);
-  else if (a.dim % 8 == 0)
-    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_EVEN>), grid, dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((window_attention_rows<T, DP, DIMS_ANY>), grid, dim3(256), 0, s, a);
-  return hipGetLastError();
+  const dim3 grid{unsigned(blocks)}, block(256);
+  if (a.dim == DP) return launch_kernel(window_attention_rows<T, DP, DIMS_WHOLE>, grid, block, 0, s, a);
+  if (a.dim % 8 == 0) return launch_kernel(window_attention_rows<T, DP, DIMS_EVEN>, grid, block, 0, s, a);
+  return launch_kernel(window_attention_rows<T, DP, DIMS_ANY>, grid, block, 0, s, a);
 }
 
 template <int T>

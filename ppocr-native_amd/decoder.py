@@ -48,7 +48,7 @@ class KvCache(C.Structure):
 
 def _functions() -> dict:
     if not _fns:
-        L = lib()
+        L, fns = lib(), {}
         p, n, i, f = C.c_void_p, C.c_size_t, C.c_int, C.c_float
         cache, end = C.POINTER(KvCache), [p, C.c_char_p, n]
         for name, args in {
@@ -60,10 +60,11 @@ def _functions() -> dict:
         }.items():
             fn = getattr(L, "ppocr_hip_" + name)
             fn.argtypes, fn.restype = args, i
-            _fns[name] = fn
+            fns[name] = fn
         fn = L.ppocr_hip_paged_attention_workspace
         fn.argtypes, fn.restype = [cache, n, n, n], n
-        _fns["workspace"] = fn
+        fns["workspace"] = fn
+        _fns.update(fns)  # all at once: another thread may be looking
     return _fns
 
 

@@ -127,3 +127,28 @@ def test_workspace():
     assert n > 0 and n % (32 * 130 * 4) == 0
     assert D.paged_attention_workspace(c, 4096, 32, 16384) == 0  # enough texts
     assert D.paged_attention_workspace(c, 1, 33, 16384) == 0 and D.paged_attention_workspace(None, 1, 1, 1) == 0
+
+
+def test_first_calls_of_two_threads(monkeypatch):
+    # The functions are looked up by the first call; one made meanwhile finds all of them or none.
+    import threading
+    import time
+    real = D.lib()
+
+    class Slow:
+        def __getattr__(self, name):
+            time.sleep(0.02)
+            return getattr(real, name)
+
+    monkeypatch.setattr(D, "_fns", {})
+    monkeypatch.setattr(D, "lib", Slow)
+    got = []
+
+    def call(wait):
+        time.sleep(wait)
+        got.append(D.paged_attention_workspace(cache(heads=8, dim=128), 1, 32, 16384))
+
+    threads = [threading.Thread(target=call, args=(w,)) for w in (0, 0.05, 0.09)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert len(got) == 3 and got[0] > 0 and len(set(got)) == 1

@@ -269,6 +269,25 @@ def test_append_leaves_what_is_out_of_range():
     assert np.array_equal(R.back(p.gpu[1], np.float32, p.host[1].shape), p.host[1], equal_nan=True)
 
 
+@pytest.mark.parametrize("starts", [(0, 2 ** 31 - 1), (-2 ** 31, 2 ** 31 - 1), (3, 2)])
+def test_append_starts_far_out(starts):
+    # Only the rows there are count, however many the starts tell of; and a
+    # length that all those would have puts row 0 at place 0 again.
+    p = R.Pages(np.random.default_rng(4), [20], 16, 1, 8, D.F32)
+    cache = p.upload()
+    k = np.random.default_rng(5).normal(0, 1, (6, 1, 8)).astype(np.float32)
+    dk, ds = R.on_gpu(k), R.on_gpu(np.array(starts, np.int32))
+    dl = R.on_gpu(np.array([2 ** 31 - 1], np.int32))
+    print(f"append, starts {starts}", flush=True)
+    D.kv_append(dk.addr, dk.addr, cache, p.gpu_table.addr, p.width, dl.addr, 1, 6, starts=ds.addr)
+    synchronize()
+    if starts[1] > starts[0]:
+        for i in range(6):
+            p.put(0, i, k[i], k[i])
+    for gpu, want in zip(p.gpu, p.host):
+        assert np.array_equal(R.back(gpu, np.float32, want.shape), want, equal_nan=True)
+
+
 # ------------------------------------------------------ the decode attention
 
 def run_paged(rng, lengths, page, heads, kv_heads, dim, t, window=0, sinks=0, layout="tokens", work=1 << 22, gap=0,
@@ -450,6 +469,14 @@ def test_prompt(t, heads, kv_heads, dim, nq, nk):
                                           (5000, 2)])
 def test_prompt_window(t, window, sinks):
     run_prompt(np.random.default_rng(window), [290, 70], [400, 70], 2, 1, 64, t, window, sinks)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("window", [149, 150, 151, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 40])
+def test_prompt_window_of_all(t, window):
+    # A window as long as the text, or longer, is none.
+    rng = np.random.default_rng(12)
+    run_prompt(rng, [150, 20], [150, 3], 4, 2, 64, t, window, 0)
 
 
 @pytest.mark.parametrize("t", R.REAL)
@@ -663,3 +690,14 @@ def test_two_streams_at_once():
         one.check()
         for x, y in zip(outs, one.outputs()):
             assert np.array_equal(x.view(np.uint8), y.view(np.uint8))
+
+
+def test_after_another_calls_error():
+    # What another call of the thread's failed at is not these calls' failure.
+    step = Step(np.random.default_rng(31))
+    print("after an error", flush=True)
+    assert hip().hipSetDevice(10 ** 6) != 0
+    step.run()
+    synchronize()
+    step.check()
+    hip().hipGetLastError()
