@@ -65,6 +65,13 @@ struct Tile16 {
     else
       return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
   }
+  // Adds the two values to a sum.
+  static __device__ __forceinline__ float sum(uint32_t p, float to) {
+    if constexpr (T == PPOCR_F16)
+      return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, p), v2h{(_Float16)1.0f, (_Float16)1.0f}, to, false);
+    else
+      return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2bf, p), v2bf{(__bf16)1.0f, (__bf16)1.0f}, to, false);
+  }
   static __device__ __forceinline__ v2f unpack(uint32_t p) {
     if constexpr (T == PPOCR_F16)
       return __builtin_convertvector(__builtin_bit_cast(v2h, p), v2f);

@@ -110,8 +110,8 @@ __device__ __forceinline__ int tiles_a_part(int tiles, int each, int splits) {
 // runs at 4.7. Each wave keeps one tile's loads on their way while it takes in
 // the one before (0.36 ms when it asked for a tile as it came to it).
 //
-// Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.y, part
-// blockIdx.x of its tiles. PAGED16: pages are multiples of 16 tokens.
+// Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.x, part
+// blockIdx.y of its tiles. PAGED16: pages are multiples of 16 tokens.
 template <int T, int DP, int DIMS, bool PAGED16>
 __global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attention_parts(PagedArgs a) {
   typedef Attend<T, DP, DIMS> A;
@@ -123,15 +123,15 @@ __global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attent
   const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int b = blockIdx.z, per = a.heads / a.c.heads, blocks = (per + 15) / 16;
-  const int kv = blockIdx.y / blocks, h0 = kv * per + blockIdx.y % blocks * 16;
+  const int kv = blockIdx.x / blocks, h0 = kv * per + blockIdx.x % blocks * 16;
   const int rows = min(16, kv * per + per - h0);
   const long capacity = a.c.table_width * a.c.page_size;
   const int length = a.c.lengths[b];
   const bool too_long = length > capacity;
   const Seen s = seen_of(too_long ? 0 : length, a.window, a.sinks, K);
   const int each = tiles_a_part(s.tiles, a.each, a.splits);
-  const int begin = blockIdx.x * each, end = min(begin + each, s.tiles);
-  if (begin >= end && blockIdx.x) return;  // part 0 of an empty text writes its zeros
+  const int begin = blockIdx.y * each, end = min(begin + each, s.tiles);
+  if (begin >= end && blockIdx.y) return;  // part 0 of an empty text writes its zeros
   if (threadIdx.x == 0) lds_bad = too_long;
   __syncthreads();
 
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(64 * kWaves, (DP <= 128 ? 2 : 1)) void paged_attent
     }
     if (lds_bad) sum = o = __uint_as_float(0x7fc00000u);
     if (split) {
-      float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + blockIdx.x) * (a.c.dim + 2);
+      float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + blockIdx.y) * (a.c.dim + 2);
       p[d + 2] = o;
       if (d == 0) p[0] = m, p[1] = sum;
     } else {
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void paged_attention_join(PagedArgs a) {
 template <int T, int DP>
 hipError_t launch_parts(const PagedArgs &a, hipStream_t s) {
   const int per = a.heads / a.c.heads;
-  const dim3 grid(a.splits, a.c.heads * ((per + 15) / 16), a.batch), block(64 * kWaves);
+  const dim3 grid(a.c.heads * ((per + 15) / 16), a.splits, a.batch), block(64 * kWaves);
   const bool paged16 = a.c.page_size % 16 == 0;
   if (a.c.dim == DP && paged16) return launch_kernel(paged_attention_parts<T, DP, DIMS_WHOLE, true>, grid, block, 0, s, a);
   if (a.c.dim == DP) return launch_kernel(paged_attention_parts<T, DP, DIMS_WHOLE, false>, grid, block, 0, s, a);

@@ -405,8 +405,9 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
         for (int i = 0; i < 16; i += 2) {
           const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -base));
           const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale, -base));
-          l += x + y;
-          pf[2 * b + i / 8][i / 2 % 4] = Tile16<T>::pack(x, y);
+          const uint32_t w = Tile16<T>::pack(x, y);
+          l = Tile16<T>::sum(w, l);
+          pf[2 * b + i / 8][i / 2 % 4] = w;
         }
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll

@@ -124,11 +124,13 @@ def attend(q, k, v, seen, scale):
 
 
 def attention_bound(y, size, reach, t, rounded):
-    """Half a step of y; of the weights, where they are rounded to t; and a
-    weight's relative error from its logarithm's, 16 steps of sum |q k| scale,
+    """Half a step of y; of the weights, where they are rounded to t, in the
+    product with v and in their sum (e_i: a weight's relative error, at most
+    half a step; sum p (1 + e) v / sum p (1 + e) = y + sum p e (v - y) but for
+    e^2, and sum p |v - y| <= sum p |v| + |y|); and a weight's relative error from its logarithm's, 16 steps of sum |q k| scale,
     twice (in the sum too), with 8 steps of its exponential."""
     steps = (2 * 16 * reach + 8 + 16) * STEP
-    return half_step(y, t) + size * (steps + (EPS[t] / 2 if rounded else 0))
+    return half_step(y, t) + size * steps + ((size + np.abs(y)) * EPS[t] / 2 if rounded else 0)
 
 
 def window_seen(places, keys, window, sinks):
