@@ -331,8 +331,8 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
  * q, and heads x (rows_q / 32 + batch) below 2^24. q and y: heads x
  * dim a row, k and v: kv_heads x dim, dim up to 256, type F32, BF16 or F16.
  * What lies in keys that a query does not see does not matter to it. In BF16
- * and F16 the softmax's weights are rounded to the type before the product
- * with v, as v itself is; their sum is not. */
+ * and F16 the softmax's weights may be rounded to the type before the product
+ * with v, as v itself is, and are then summed as rounded. */
 int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
                                size_t v_stride, void *y, size_t y_stride, const int32_t *starts_q,
                                const int32_t *starts_k, size_t batch, size_t rows_q, size_t rows_k, size_t heads,

@@ -28,10 +28,10 @@
 // stretches at a time, x as finished operands.
 //
 // 4096 inputs to 28672 outputs (59 to 71 MB): one row of bf16, groups of 128,
-// 17.5 us, 3.5 TB/s; 16 rows of f16, groups of 32 with zero points, 26 us, 2.7
-// TB/s, of which the vector units are busy half; 5 rows of f32 40 us. What is
-// left is the wait at each chunk's start. Fetching a chunk's x ahead into
-// registers spilled (43 us); tiles of 32 and 64 rows of x were slower than
+// 17.5 us, 3.4 TB/s; 16 rows of f16, groups of 32 with zero points, 26 us, 2.7
+// TB/s; 5 rows of f32, groups of 64, 30 us. What is left is the wait for a
+// chunk at its start and the launch. Fetching a chunk's x ahead into registers
+// spilled (60 us for the 26); tiles of 32 and 64 rows of x were slower than
 // blocks of 16 that share the weights through L2 (64 rows of f32: 715 us
 // against 171).
 #include <algorithm>
@@ -133,8 +133,9 @@ __device__ __forceinline__ v4u weights16(uint32_t w, uint32_t mask, uint32_t bas
 
 constexpr int kRing = 3;
 
-// LDS: the waves' rings; then a chunk of x, for each 32 inputs and part, 4 x `rows` 16-byte operand pieces (rows: 1, 2, 4, 8 or 16, not fewer
-// than there are), piece (quarter, row) at quarter * rows + (row ^ turn), turn
+// LDS: the waves' rings; then a chunk of x, for each 32 inputs and part, 4 x
+// `rows` 16-byte operand pieces (rows: 1, 2, 4, 8 or 16, not fewer than there
+// are), piece (quarter, row) at quarter * rows + (row ^ turn), turn
 // = the 8 inputs' number: so that neighbouring pieces of a row, written
 // together, lie in different banks; the weights' scales and 16 + zero points,
 // [output][group][2]; and 8-bit x's scales a group, [group][row].
@@ -394,6 +395,17 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
   }
 }
 
+// A wave a stretch, up to kWaves.
+inline int waves_of(int k) {
+  int waves = kWaves;
+  while (waves > 1 && waves / 2 * kStretch >= k) waves /= 2;
+  return waves;
+}
+
+// Workgroups of kWaves that the card holds at once, by their registers.
+template <int X>
+constexpr int kAtOnce = X == PPOCR_F32 ? 256 : 512;
+
 template <int X, int NT, int GROUP, int SB>
 hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   const int steps = (a.k + kStretch - 1) / kStretch, row_bytes = (a.k + 1) / 2;
@@ -406,11 +418,12 @@ hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   constexpr int SG = kStretch / GROUP;
   const int a_stretch = 4 * XRow<X>::parts * 64 * ch.rows + SG * 16 * NT * 8 + (a.x_group ? SG * 64 : 0);
   constexpr int once = 16 * NT * 8;  // the scales' extra column
-  // Eight waves and two workgroups a CU, each with half its LDS; all of it
-  // where there are not more workgroups than CUs. At least a stretch a wave.
-  int waves = kWaves;
-  const int room = (strips * (long)m_blocks <= 256 ? 152 : 76) * 1024;
-  while (waves > 1 && (waves / 2 >= steps || waves * (a_stretch + kRing * 1024) + once > 152 * 1024)) waves /= 2;
+  // Each of the workgroups that run on a CU at once has its share of its LDS.
+  // At least a stretch a wave.
+  int waves = waves_of(a.k);
+  const int on_cu = std::min((strips * (long)m_blocks + 255) / 256, long(kAtOnce<X> / 256 * (kWaves / waves)));
+  const int room = 152 * 1024 / on_cu;
+  while (waves > 1 && waves * (a_stretch + kRing * 1024) + once > 152 * 1024) waves /= 2;
   ch.stretches = waves;
   while (ch.stretches < steps && waves * kRing * 1024 + 2 * ch.stretches * a_stretch + once <= room) ch.stretches *= 2;
   ch.log_stretches = __builtin_ctz(ch.stretches);
@@ -439,8 +452,13 @@ hipError_t launch_tile(const Q4Args &a, int e4m3, hipStream_t s) {
 hipError_t PPOCR_Q4_LAUNCH(const Q4Args &a, int e4m3, hipStream_t s) {
   constexpr int X = PPOCR_Q4_X;
   const long tiles = (a.n + 15L) / 16 * ((a.m + 15) / 16);
-  if (tiles <= 512) return launch_tile<X, 1>(a, e4m3, s);
-  if (tiles <= 1024) return launch_tile<X, 2>(a, e4m3, s);
+  // As few tiles a workgroup as all run at once with (18385 outputs of 1024
+  // inputs from 5 rows of f32: 288 workgroups 13.9 us, 144 of them 11.0).
+  const long at_once = kAtOnce<X> * (kWaves / waves_of(a.k));
+  if (tiles <= at_once) return launch_tile<X, 1>(a, e4m3, s);
+  if (tiles <= 2 * at_once) return launch_tile<X, 2>(a, e4m3, s);
+  if constexpr (X == PPOCR_F32)
+    if (tiles > 4 * at_once && tiles <= 8 * at_once) return launch_tile<X, 8>(a, e4m3, s);
   return launch_tile<X, 4>(a, e4m3, s);
 }
 

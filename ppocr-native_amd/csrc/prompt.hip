@@ -399,6 +399,7 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
       continue;
     } else {
       v4u pf[4];
+      float part[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int b = 0; b < SB; b++)
 #pragma unroll
@@ -406,9 +407,10 @@ __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_att
           const float x = __builtin_amdgcn_exp2f(fmaf(s[b][i], a.scale, -base));
           const float y = __builtin_amdgcn_exp2f(fmaf(s[b][i + 1], a.scale, -base));
           const uint32_t w = Tile16<T>::pack(x, y);
-          l = Tile16<T>::sum(w, l);
+          part[i / 2 % 4] = Tile16<T>::sum(w, part[i / 2 % 4]);
           pf[2 * b + i / 8][i / 2 % 4] = w;
         }
+      l += (part[0] + part[1]) + (part[2] + part[3]);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int b = 0; b < DB; b++) {
