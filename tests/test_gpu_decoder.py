@@ -472,6 +472,16 @@ def test_prompt_window(t, window, sinks):
 
 
 @pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [15, 64])
+@pytest.mark.parametrize("window", [0, 31, 200])
+def test_prompt_ragged_texts(t, dim, window):
+    # Texts of very different lengths, empty ones among them: every block of every text once, in any order.
+    rng = np.random.default_rng(17)
+    nq = [0, 400, 1, 33, 0, 290, 128, 64, 129, 5, 0]
+    run_prompt(rng, nq, [n + i % 3 for i, n in enumerate(nq)], 4, 2, dim, t, window, 3)
+
+
+@pytest.mark.parametrize("t", R.REAL)
 @pytest.mark.parametrize("window", [149, 150, 151, 2 ** 31 - 2, 2 ** 31 - 1, 2 ** 40])
 def test_prompt_window_of_all(t, window):
     # A window as long as the text, or longer, is none.
