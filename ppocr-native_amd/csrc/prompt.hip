@@ -25,7 +25,7 @@ __device__ __forceinline__ int wave_total(int v, int bits) {
 // walks the starts, 64 texts at a time. Of those, blocks that are far into
 // their text come first, as they see most keys, so that the last to run are
 // short (14 texts of up to 6971 tokens, one head of 256 in f32, 2.6 ms text by
-// text, 2.1 so; 20 of up to 3000, 4 heads of 128 in bf16, 160 and 140 us).
+// text, 2.1 so; 20 of up to 3000, 4 heads of 128 in bf16, 155 and 132 us).
 // Blocks further in than the window see as many keys as one another and come
 // text by text: neighbours share most of them. Starts past the rows there are,
 // and such as decrease, leave texts of no rows.
@@ -259,11 +259,12 @@ __device__ __forceinline__ int not_finite2(uint32_t x) {
 // operand's order instead, f32 ran at 60 TFLOP/s: the address unit takes a
 // cycle a lane.)
 // What bounds it: the matrix cores, which a wave's softmax leaves waiting where
-// the other wave of its SIMD has none of its own to do. One text of 8192 tokens,
-// 32 heads of 128 in bf16: 0.63 ms, 870 TFLOP/s of the seen keys' products, where
-// a library product of 8192 x 8192 x 8192 runs at 1124; a window of 2048 over
-// two such texts 0.33 ms, 790 TFLOP/s. Eight waves a workgroup: 2 to 3 % faster
-// on these, 10 to 16 % slower on heads of 64 and on 1115 tokens of 4 heads.
+// the other wave of its SIMD has none of its own to do. One text of 8192
+// tokens, 32 heads of 128 in bf16: 0.62 ms, 880 TFLOP/s of the seen keys'
+// products, where a library product of 8192 x 8192 x 8192 runs at 1124; a window
+// of 2048 over two such texts 0.32 to 0.36 ms, 720 to 800 TFLOP/s. Eight waves
+// a workgroup: 2 to 3 % faster on these, 10 to 16 % slower on heads of 64 and on
+// 1115 tokens of 4 heads.
 // WHOLE: dim == DP and fills the pieces.
 template <int T, int DP, bool WHOLE>
 __global__ __launch_bounds__(64 * kTileWaves, DP <= 128 ? 2 : 1) void window_attention_tiles(PromptArgs a, int hg) {
