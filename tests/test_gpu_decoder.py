@@ -329,6 +329,16 @@ def test_paged(t, heads, kv_heads, dim, page):
 
 
 @pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [80, 88, 96, 104, 136, 184, 192, 200])
+@pytest.mark.parametrize("page", [16, 24])
+def test_paged_dims(t, dim, page):
+    # Head sizes between the powers of two.
+    rng = np.random.default_rng(dim)
+    run_paged(rng, [700, 1, 95, 0, 33], page, 6, 2, dim, t)
+    run_paged(rng, [700, 1, 95, 0, 33], page, 6, 2, dim, t, 50, 3, layout="heads")
+
+
+@pytest.mark.parametrize("t", R.REAL)
 @pytest.mark.parametrize("page", [16, 48, 1, 5])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (40, 4), (32, 32), (33, 40), (500, 70), (64, 1000), (100000, 3)])
 def test_paged_window(t, page, window, sinks):
