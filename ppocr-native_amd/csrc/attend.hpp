@@ -90,6 +90,11 @@ struct Attend {
   static constexpr int QC = F32 ? DP / 16 : DP / 32;  // 16-byte pieces of a row a lane has
   static constexpr int QN = F32 ? 4 : 8;            // values in one
   static constexpr int E = DP / 16;                 // values of a V row a lane has
+  // Weights (and so their sum) are held 2^UP times as large: F16 ends at 2^-24,
+  // and where one key is far ahead of all others, theirs are what counts if its
+  // value is near 0. The largest is 2^14 then, below F16's 65504, and a weight
+  // is off by 2^-39 of the largest at most.
+  static constexpr float UP = T == PPOCR_F16 ? 14.0f : 0.0f;
   V q[QC][QN];
   v4f o[E];  // O^T: this lane's row, d = E (4 quarter + r) + e
   float m, l;  // running maximum of the products and this lane's share of the sum
@@ -198,7 +203,7 @@ struct Attend {
       }
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now * scale;
+    const float now = fmaxf(m, top), base = now == -INFINITY ? 0.0f : now * scale - UP;
     if (__any(now != m)) {
       const float shrink = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - now) * scale);
       l *= shrink;
@@ -231,8 +236,10 @@ struct Attend {
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[0][r][e], p[0][r], o[e], 0, 0, 0);
     } else {
-      // P as a high and a low part of T: the weights keep f32's precision at
-      // twice the products, which memory hides.
+      // P as a high and a low part of T: the weights keep 16 bits in BF16 and 22
+      // in F16 (down to the parts' last step, 2^-24 of the unit UP makes) where
+      // T alone has 8 and 11, at twice the products, which memory hides. Their
+      // sum is of the f32 weights.
       v4u hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; i++) {

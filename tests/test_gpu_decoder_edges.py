@@ -1,0 +1,120 @@
+"""The decoder layers on the GPU where numbers or shapes are at an edge: weights
+far below the largest, infinities that are seen, sums that leave f32's range,
+codes next to a rounding's border, tiles and heads of every kernel, a first
+call inside a capture."""
+import subprocess
+import sys
+from pathlib import Path
+
+import numpy as np
+import pytest
+
+import decoder_plain as R
+from ppocr_native_amd import decoder as D
+from ppocr_native_amd.devmem import synchronize
+
+pytestmark = pytest.mark.gpu
+STEP = R.STEP
+
+
+# ------------------------------------------- attention: given keys and values
+
+def paged(q, k, v, t, scale, kv_heads=1, page=16, work=1 << 20):
+    """q [heads][dim] of one text, k and v [keys][kv heads][dim], stored -> y [heads][dim] as float64."""
+    heads, dim = q.shape
+    n = k.shape[0]
+    p = R.Pages(np.random.default_rng(1), [n], page, kv_heads, dim, t)
+    for i in range(n):
+        p.put(0, i, k[i], v[i])
+    cache = p.upload()
+    dq, dl, dy = R.on_gpu(q), R.on_gpu(np.array([n], np.int32)), R.on_gpu(np.zeros((heads, dim), R.dtype(t)))
+    dw = R.on_gpu(np.zeros(max(work, 4), np.uint8))
+    print(f"paged {n} keys, {heads}/{kv_heads} heads of {dim}, type {t}, work {work}", flush=True)
+    D.paged_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, 1, heads, scale=scale,
+                      workspace=dw.addr if work else 0, workspace_bytes=work)
+    synchronize()
+    return R.values(R.back(dy, R.dtype(t), (heads, dim)), t)
+
+
+def prompt(q, k, v, t, scale, odd=0, window=0, sinks=0):
+    """q [rows][heads][dim], k and v [rows][1][dim] of one text, stored; rows of k and v `odd` values apart (1: the
+    kernel that takes any address) -> y as float64."""
+    rows, heads, dim = q.shape
+    wide = lambda a: R.on_gpu(np.concatenate([a.reshape(len(a), -1), np.zeros((len(a), odd), a.dtype)], 1))  # noqa: E731
+    dq, dk, dv, dy = R.on_gpu(q), wide(k), wide(v), R.on_gpu(np.zeros(q.shape, R.dtype(t)))
+    ds, dt = R.on_gpu(np.array([0, rows], np.int32)), R.on_gpu(np.array([0, len(k)], np.int32))
+    print(f"prompt {rows} of {len(k)} keys, {heads} heads of {dim}, type {t}, odd {odd}", flush=True)
+    D.window_attention(dq.addr, dk.addr, dv.addr, dy.addr, ds.addr, dt.addr, 1, rows, len(k), heads, 1, dim,
+                       type=t, scale=scale, window=window, sinks=sinks, k_stride=dim + odd, v_stride=dim + odd)
+    synchronize()
+    return R.values(R.back(dy, R.dtype(t), q.shape), t)
+
+
+# --------------------------------------- one key far ahead of all the others
+
+def far_ahead(t, dim, heads, keys):
+    """Keys 1, 2, ... at the same score, key 0 between 13 and 18.3 nats ahead of them (another distance a head), its
+    value 0: what comes out is the others' alone."""
+    rng = np.random.default_rng(dim)
+    q = np.zeros((heads, dim))
+    q[:, 3] = np.linspace(13, 18.3, heads)
+    k = np.zeros((keys, 1, dim))
+    k[0, 0, 3] = 1.0
+    v = rng.uniform(500, 1500, (keys, 1, dim))
+    v[0] = 0
+    return tuple(R.stored(a, t) for a in (q, k, v))
+
+
+# F16's smallest step is 2^-24: a weight that goes into the product as F16 is off by up to 2^-25 of the unit it is
+# held in. The decode attention's unit is 2^-14 of the row's largest weight, the prompt attention's 2^-13 of a
+# reference that the largest is at most 2^2 above (so never more than 2^-13 of the largest): 2^-39 and 2^-38 of the
+# largest, which the sum of weights is not below.
+LEAST_DECODE, LEAST_PROMPT = 2.0 ** -39, 2.0 ** -38
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [64, 128, 80, 30])
+@pytest.mark.parametrize("work", [0, 1 << 20])
+def test_decode_of_small_weights(t, dim, work):
+    q, k, v = far_ahead(t, dim, 8, 2000)
+    got = paged(q, k, v, t, 1.0, work=work)
+    qv, kv, vv = R.values(q, t), R.values(k, t)[:, 0], R.values(v, t)[:, 0]
+    y, size, reach = R.attend(qv, kv, vv, np.ones((8, 2000), bool), 1.0)
+    least = LEAST_DECODE * np.abs(vv).sum(0)[None] if t == D.F16 else 0
+    R.close(got, y, R.attention_bound(y, size, reach, t, False) + least)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [64, 128, 96, 30])
+@pytest.mark.parametrize("odd", [0, 1])
+def test_prompt_of_small_weights(t, dim, odd):
+    # Every query sees key 0 and all before it: the one ahead comes in the first tile.
+    q1, k, v = far_ahead(t, dim, 4, 700)
+    q = np.repeat(q1[None], 700, 0)
+    got = prompt(q, k, v, t, 1.0, odd)
+    seen = R.window_seen(np.arange(700), 700, 0, 0)
+    kv, vv = R.values(k, t)[:, 0], R.values(v, t)[:, 0]
+    sums = np.cumsum(np.abs(vv), 0)
+    for h in range(4):
+        y, size, reach = R.attend(R.values(q[:, h], t), kv, vv, seen, 1.0)
+        least = LEAST_PROMPT * (sums + np.arange(1, 701)[:, None] * np.abs(y)) if t == D.F16 else 0
+        R.close(got[:, h], y, R.attention_bound(y, size, reach, t, t != D.F32) + least)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("odd", [0, 1])
+def test_prompt_of_growing_scores(t, odd):
+    # Scores that rise by a little from key to key: the running maximum follows in steps, in every tile.
+    rng = np.random.default_rng(3)
+    keys, dim = 600, 64
+    q, k = np.zeros((keys, 2, dim)), np.zeros((keys, 1, dim))
+    q[:, 0, 5], q[:, 1, 5] = 1.0, -1.0
+    k[:, 0, 5] = np.arange(keys) * 0.02
+    q, k, v = R.stored(q, t), R.stored(k, t), R.stored(rng.normal(0, 1, (keys, 1, dim)), t)
+    got = prompt(q, k, v, t, 1.0, odd)
+    seen = R.window_seen(np.arange(keys), keys, 0, 0)
+    kv, vv = R.values(k, t)[:, 0], R.values(v, t)[:, 0]
+    for h in range(2):
+        y, size, reach = R.attend(R.values(q[:, h], t), kv, vv, seen, 1.0)
+        least = LEAST_PROMPT * np.cumsum(np.abs(vv) + np.abs(y), 0) if t == D.F16 else 0
+        R.close(got[:, h], y, R.attention_bound(y, size, reach, t, t != D.F32) + least)
