@@ -305,7 +305,9 @@ int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_
  * i < lengths[b]; with `window` > 0 only the last `window` of them and the
  * first `sinks`. A text of length 0 (or less) gives zeros; one whose length
  * passes table_width * page_size, or with a seen token in a page that does
- * not exist, gives NaN. What lies in unseen tokens does not matter.
+ * not exist, gives NaN. What lies in unseen tokens does not matter; an
+ * infinity in the v of a seen one gives that infinity (in F16, NaN where its
+ * weight is below 2^-39 of the largest).
  *
  * `longest` bounds the lengths (0: table_width * page_size); it only guides
  * how far the cache is split, and longer texts are right too. The parts are
@@ -330,7 +332,9 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
  * decreasing, within them (rows past them are not touched), at most 2^24 rows of
  * q, and heads x (rows_q / 32 + batch) below 2^24. q and y: heads x
  * dim a row, k and v: kv_heads x dim, dim up to 256, type F32, BF16 or F16.
- * What lies in keys that a query does not see does not matter to it. In BF16
+ * What lies in keys that a query does not see does not matter to it; an
+ * infinity in the v of one that it sees gives that infinity (in F16, NaN where
+ * its weight is below 2^-38 of the largest). In BF16
  * and F16 the softmax's weights may be rounded to the type before the product
  * with v, as v itself is, and are then summed as rounded. */
 int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,

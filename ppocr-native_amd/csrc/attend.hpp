@@ -65,6 +65,13 @@ struct Tile16 {
     else
       return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a, b}, v2bf));
   }
+  // Both positive, or 0: rounded down.
+  static __device__ __forceinline__ uint32_t pack_down(float a, float b) {
+    if constexpr (T == PPOCR_F16)
+      return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    else
+      return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+  }
   // Adds the two values to a sum.
   static __device__ __forceinline__ float sum(uint32_t p, float to) {
     if constexpr (T == PPOCR_F16)
@@ -92,9 +99,9 @@ struct Attend {
   static constexpr int E = DP / 16;                 // values of a V row a lane has
   // Weights (and so their sum) are held 2^UP times as large: F16 ends at 2^-24,
   // and where one key is far ahead of all others, theirs are what counts if its
-  // value is near 0. The largest is 2^14 then, below F16's 65504, and a weight
+  // value is near 0. The largest is 2^15 then, below F16's 65504, and a weight
   // is off by 2^-39 of the largest at most.
-  static constexpr float UP = T == PPOCR_F16 ? 14.0f : 0.0f;
+  static constexpr float UP = T == PPOCR_F16 ? 15.0f : 0.0f;
   V q[QC][QN];
   v4f o[E];  // O^T: this lane's row, d = E (4 quarter + r) + e
   float m, l;  // running maximum of the products and this lane's share of the sum
@@ -239,14 +246,18 @@ struct Attend {
       // P as a high and a low part of T: the weights keep 16 bits in BF16 and 22
       // in F16 (down to the parts' last step, 2^-24 of the unit UP makes) where
       // T alone has 8 and 11, at twice the products, which memory hides. Their
-      // sum is of the f32 weights.
+      // sum is of the f32 weights. The high part is rounded down and the low one
+      // is not 0 where the weight is not, so that an infinity in V times both is
+      // that infinity.
+      constexpr float least = T == PPOCR_F16 ? 0x1p-24f : 0x1p-126f;
+      auto rest = [&](float x, float high) { return __builtin_amdgcn_fmed3f(x - high, least, x); };
       v4u hi, lo;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         const float x = p[i / 2][2 * (i % 2)], y = p[i / 2][2 * (i % 2) + 1];
-        hi[i] = Tile16<T>::pack(x, y);
+        hi[i] = Tile16<T>::pack_down(x, y);
         const v2f back = Tile16<T>::unpack(hi[i]);
-        lo[i] = Tile16<T>::pack(x - back[0], y - back[1]);
+        lo[i] = Tile16<T>::pack(rest(x, back[0]), rest(y, back[1]));
       }
 #pragma unroll
       for (int e = 0; e < E; e++) {

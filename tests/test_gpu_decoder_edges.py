@@ -118,3 +118,49 @@ def test_prompt_of_growing_scores(t, odd):
         y, size, reach = R.attend(R.values(q[:, h], t), kv, vv, seen, 1.0)
         least = LEAST_PROMPT * np.cumsum(np.abs(vv) + np.abs(y), 0) if t == D.F16 else 0
         R.close(got[:, h], y, R.attention_bound(y, size, reach, t, t != D.F32) + least)
+
+
+# ---------------------------------------------- infinities in values that are seen
+
+def with_infinities(v, t, at):
+    """Infinities in values `at` and behind: columns that come out as inf, -inf, and NaN (both, or a NaN)."""
+    v = np.asarray(R.values(v, t), np.float32)
+    n = len(v)
+    for i, d, x in ((0, 1, np.inf), (0, 2, -np.inf), (3, 2, -np.inf), (5, 7, np.inf), (6, 7, -np.inf), (2, 9, np.nan)):
+        if at + i < n:
+            v[at + i, 0, d] = x
+    return R.stored(v, t)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [64, 128, 80, 30])
+@pytest.mark.parametrize("keys,at,work", [(1, 0, 0), (40, 10, 0), (70, 68, 0), (3000, 1700, 0), (3000, 1700, 1 << 20)])
+def test_decode_of_infinities(t, dim, keys, at, work):
+    rng = np.random.default_rng(keys)
+    q, k = R.stored(rng.normal(0, 2, (4, dim)), t), R.stored(rng.normal(0, 1, (keys, 1, dim)), t)
+    v = with_infinities(R.stored(rng.normal(0, 1, (keys, 1, dim)), t), t, at)
+    got = paged(q, k, v, t, dim ** -0.5, work=work)
+    with np.errstate(invalid="ignore"):
+        y, size, reach = R.attend(R.values(q, t), R.values(k, t)[:, 0], R.values(v, t)[:, 0],
+                                  np.ones((4, keys), bool), dim ** -0.5)
+        assert np.isinf(y[:, 1]).all() and np.isinf(y[:, 2]).all()
+        R.close(got, y, R.attention_bound(y, size, reach, t, False))
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [64, 128, 96, 30])
+@pytest.mark.parametrize("odd", [0, 1])
+@pytest.mark.parametrize("window,sinks,at", [(0, 0, 0), (0, 0, 100), (30, 4, 2), (30, 4, 100), (200, 0, 30)])
+def test_prompt_of_infinities(t, dim, odd, window, sinks, at):
+    rng = np.random.default_rng(at + dim)
+    rows = 290
+    q, k = R.stored(rng.normal(0, 2, (rows, 2, dim)), t), R.stored(rng.normal(0, 1, (rows, 1, dim)), t)
+    v = with_infinities(R.stored(rng.normal(0, 1, (rows, 1, dim)), t), t, at)
+    got = prompt(q, k, v, t, dim ** -0.5, odd, window, sinks)
+    seen = R.window_seen(np.arange(rows), rows, window, sinks)
+    with np.errstate(invalid="ignore"):
+        for h in range(2):
+            y, size, reach = R.attend(R.values(q[:, h], t), R.values(k, t)[:, 0], R.values(v, t)[:, 0], seen,
+                                      dim ** -0.5)
+            assert np.isinf(y).any() and np.isfinite(y).any()
+            R.close(got[:, h], y, R.attention_bound(y, size, reach, t, t != D.F32))
