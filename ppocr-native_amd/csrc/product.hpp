@@ -13,6 +13,9 @@
 //   sum x (q - z) = sum x (16 + q) - (16 + z) sum x,
 // every term exact in bf16 and f16 but for the f32 sums. f32 rows are split
 // into three bf16 parts first (split.hpp), 8-bit rows are exact in bf16.
+// (16 + q) x passes f32's range before q x does, and f32 values past bf16's
+// largest are infinite in the split: an output of f32 or bf16 rows that comes out
+// as an infinity or NaN is computed again, in f64 from the formula as it stands.
 //
 // A workgroup takes up to NT tiles of 16 outputs, its waves every W-th stretch
 // of 128 inputs of them; the waves' sums are added in LDS in their order. The
@@ -144,6 +147,33 @@ struct Chunk {
   int rows;
   int align;  // of the weights' rows: 16, 4 or 1
 };
+
+// Output n of row m by one wave, in f64; NaN where x has an infinity or NaN.
+template <int X, int GROUP>
+__device__ __forceinline__ float q4_alone(const Q4Args &a, int m, int n, int lane) {
+  const num_t<X> *x = (const num_t<X> *)a.x + m * a.x_stride;
+  const uint8_t *q = a.q + (long)n * ((a.k + 1) / 2);
+  const long g0 = (long)n * a.groups;
+  double sum = 0.0;
+#pragma unroll 1
+  for (int k0 = 0; k0 < a.k; k0 += 64) {
+    const int k = k0 + lane;
+    float v = 0.0f;
+    if (k < a.k) v = Num<X>::get(x[k]);
+    if (__any(!(fabsf(v) < INFINITY))) return __uint_as_float(0x7fc00000u);
+    if (k < a.k) {
+      const long g = g0 + k / GROUP;
+      const float s = a.scale_type == PPOCR_F32    ? ((const float *)a.scales)[g]
+                      : a.scale_type == PPOCR_BF16 ? (float)((const __bf16 *)a.scales)[g]
+                                                   : (float)((const _Float16 *)a.scales)[g];
+      const int w = (q[k / 2] >> k % 2 * 4 & 15) - (a.zeros ? a.zeros[g] : 8);
+      sum += double(v) * w * double(s);
+    }
+  }
+#pragma unroll
+  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+  return float(sum);
+}
 
 template <int X, int NT, int GROUP, int SB>
 __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows(Q4Args a, int e4m3, Chunk ch) {
@@ -377,13 +407,14 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
     for (int t = 0; t < AT; t++)
       *(v4f *)&red[wave][t][4 * lane] = acc[t0 + t];
     __syncthreads();
-    for (int i = tid; i < AT * 256; i += threads) {
-      const int c = i % 16, r = i / 16 % 16, n = n0 + 16 * (t0 + i / 256) + c, m = m0 + r;
-      if (m >= a.m || n >= a.n) continue;
+    auto row_of = [&](int i) { return m0 + i / 16 % 16; };
+    auto col_of = [&](int i) { return n0 + 16 * (t0 + i / 256) + i % 16; };
+    auto sum_of = [&](int i) {
       float v = 0.0f;
-      for (int w = 0; w < waves; w++) v += red[w][i / 256][4 * (c + 16 * (r / 4)) + r % 4];
-      if constexpr (X == PPOCR_I8)
-        if (!x_grouped) v *= a.x_scales[m];
+      for (int w = 0; w < waves; w++) v += red[w][i / 256][4 * (i % 16 + 16 * (i / 64 % 4)) + i / 16 % 4];
+      return v;
+    };
+    auto put = [&](int m, int n, float v) {
       const long at = m * a.y_stride + n;
       if (a.y_type == PPOCR_F32)
         ((float *)a.y)[at] = a.bias ? v + ((const float *)a.bias)[n] : v;
@@ -391,7 +422,26 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
         ((__bf16 *)a.y)[at] = (__bf16)(a.bias ? v + (float)((const __bf16 *)a.bias)[n] : v);
       else
         ((_Float16 *)a.y)[at] = (_Float16)(a.bias ? v + (float)((const _Float16 *)a.bias)[n] : v);
+    };
+    bool bad = false;
+    for (int i = tid; i < AT * 256; i += threads) {
+      const int m = row_of(i), n = col_of(i);
+      if (m >= a.m || n >= a.n) continue;
+      float v = sum_of(i);
+      if constexpr (X == PPOCR_I8)
+        if (!x_grouped) v *= a.x_scales[m];
+      bad |= !(fabsf(v) < INFINITY);
+      put(m, n, v);
     }
+    if constexpr (X == PPOCR_F32 || X == PPOCR_BF16)
+      if (__any(bad)) {  // rare
+        for (int i = 64 * wave; i < AT * 256; i += i % 64 == 63 ? threads - 63 : 1) {
+          const int m = row_of(i), n = col_of(i);
+          if (m >= a.m || n >= a.n || fabsf(sum_of(i)) < INFINITY) continue;
+          const float v = q4_alone<X, GROUP>(a, m, n, lane);
+          if (lane == i % 64) put(m, n, v);  // (the lane that wrote it)
+        }
+      }
   }
 }
 

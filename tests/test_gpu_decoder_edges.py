@@ -164,3 +164,56 @@ def test_prompt_of_infinities(t, dim, odd, window, sinks, at):
                                       dim ** -0.5)
             assert np.isinf(y).any() and np.isfinite(y).any()
             R.close(got[:, h], y, R.attention_bound(y, size, reach, t, t != D.F32))
+
+
+# -------------------------------------------------- products of very large numbers
+
+@pytest.mark.parametrize("t", [D.F32, D.BF16, D.F16])
+@pytest.mark.parametrize("m,n,k,group,zeros", [(1, 40, 256, 128, False), (5, 100, 300, 32, True),
+                                               (17, 33, 1030, 64, True), (3, 9001, 640, 128, False)])
+def test_product_of_large_x(t, m, n, k, group, zeros):
+    # Groups of like signs whose sums of x (16 + q) pass f32's largest where those of x (q - z) do not, values that
+    # round past bf16's largest, and beside them ordinary rows, and rows with an infinity or NaN.
+    rng = np.random.default_rng(n)
+    x = rng.normal(0, 1, (m, k))
+    big = 3.0e38 if t == D.BF16 else 65504.0 if t == D.F16 else 3.4e38
+    x[0] = rng.uniform(0.2, 0.9, k) * big
+    if m > 2:
+        x[2, 3], x[2, k - 1] = big, -big
+    if m > 4:
+        x[3, 7], x[4, k // 2] = np.inf, np.nan
+    raw = R.stored(x, t)
+    groups = -(-k // group)
+    q, s = rng.integers(0, 16, (n, k)), R.stored(rng.uniform(0.5, 1.5, (n, groups)) / 2 ** 14, D.F32)
+    z = rng.integers(0, 16, (n, groups)).astype(np.uint8) if zeros else None
+    b = R.stored(rng.normal(0, 1, n), t)
+    dx, dq, ds, db = (R.on_gpu(a) for a in (raw, R.packed(q), s, b))
+    dz = R.on_gpu(z) if zeros else None
+    dy = R.on_gpu(np.zeros((m, n), R.dtype(t)))
+    print(f"product of large x {m}x{k}->{n} type {t}", flush=True)
+    D.q4_product(dx.addr, dq.addr, ds.addr, dy.addr, m, n, k, group=group, zeros=dz.addr if zeros else 0,
+                 bias=db.addr, x_type=t, scale_type=D.F32, y_type=t)
+    synchronize()
+    got = R.values(R.back(dy, R.dtype(t), (m, n)), t)
+    rows = [i for i in range(m) if i not in (3, 4)] if m > 4 else list(range(m))
+    want, size = R.product(R.values(raw, t)[rows], q, s.astype(np.float64), z, group)
+    want = want + R.values(b, t)
+    assert np.abs(want).max() < R.values(R.stored([big], t), t)[0]  # all of it can be told
+    R.close(got[rows], want, R.half_step(want, t) + 16 * STEP * size)
+    if m > 4:
+        assert np.isnan(got[3:5]).all()
+
+
+def test_product_that_overflows():
+    # A sum past f32's largest is an infinity.
+    x, q = np.full((2, 64), 3e38, np.float32), np.full((20, 64), 15)
+    x[1] = 1
+    q[::2] = 0
+    s = np.full((20, 2), 1, np.float32)
+    dx, dq, ds, dy = R.on_gpu(x), R.on_gpu(R.packed(q)), R.on_gpu(s), R.on_gpu(np.zeros((2, 20), np.float32))
+    print("product that overflows", flush=True)
+    D.q4_product(dx.addr, dq.addr, ds.addr, dy.addr, 2, 20, 64, group=32)
+    synchronize()
+    y = R.back(dy, np.float32, (2, 20))
+    assert (y[0, ::2] == -np.inf).all() and (y[0, 1::2] == np.inf).all()
+    assert (y[1, ::2] == -512).all() and (y[1, 1::2] == 448).all()
