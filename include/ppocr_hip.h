@@ -279,6 +279,11 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
                          size_t m, size_t n, size_t k, size_t group, int x_type, int scale_type, int y_type,
                          void *stream, char *err, size_t err_len);
 
+/* How many tiles of 16 outputs a workgroup of that product takes (1, 2, 4 or
+ * 8; 0 for sizes that are refused): which of its kernels runs, for tests and
+ * profiles. */
+size_t ppocr_hip_q4_product_tiles(size_t m, size_t n, size_t k, int x_type);
+
 /* A paged cache of keys and values: `pages` pages of `page_size` tokens of
  * `heads` heads of `dim` values (up to 256) of `type` (F32, BF16, F16).
  * Strides count values from page to page, token to token and head to head;

@@ -171,6 +171,12 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
                                                           : launch_q4_i8(a, x_type == PPOCR_E4M3, st));
 }
 
+size_t ppocr_hip_q4_product_tiles(size_t m, size_t n, size_t k, int x_type) {
+  if (x_type < PPOCR_F32 || x_type > PPOCR_I8 || !m || !n || !k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20)
+    return 0;
+  return size_t(q4_tiles(x_type, int(m), int(n), int(k)));
+}
+
 int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_stride, const ppocr_kv_cache *cache,
                         const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
                         size_t batch, size_t rows, void *stream, char *err, size_t err_len) {

@@ -46,8 +46,7 @@
 namespace ppocr {
 namespace {
 
-constexpr int kWaves = 8;      // most waves of a workgroup
-constexpr int kStretch = 128;  // inputs a wave takes at a time
+constexpr int kWaves = kQ4Waves, kStretch = kQ4Stretch;
 
 // Eight values of x as loaded (DW dwords), and as matrix operands: dword d
 // holds values d (low half) and d + 4, the order the nibbles come in.
@@ -445,17 +444,6 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
   }
 }
 
-// A wave a stretch, up to kWaves.
-inline int waves_of(int k) {
-  int waves = kWaves;
-  while (waves > 1 && waves / 2 * kStretch >= k) waves /= 2;
-  return waves;
-}
-
-// Workgroups of kWaves that the card holds at once, by their registers.
-template <int X>
-constexpr int kAtOnce = X == PPOCR_F32 ? 256 : 512;
-
 template <int X, int NT, int GROUP, int SB>
 hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   const int steps = (a.k + kStretch - 1) / kStretch, row_bytes = (a.k + 1) / 2;
@@ -470,8 +458,8 @@ hipError_t launch_of(const Q4Args &a, int e4m3, hipStream_t s) {
   constexpr int once = 16 * NT * 8;  // the scales' extra column
   // Each of the workgroups that run on a CU at once has its share of its LDS.
   // At least a stretch a wave.
-  int waves = waves_of(a.k);
-  const int on_cu = std::min((strips * (long)m_blocks + 255) / 256, long(kAtOnce<X> / 256 * (kWaves / waves)));
+  int waves = q4_waves(a.k);
+  const int on_cu = std::min((strips * (long)m_blocks + 255) / 256, long(q4_at_once(X) / 256 * (kWaves / waves)));
   const int room = 152 * 1024 / on_cu;
   while (waves > 1 && waves * (a_stretch + kRing * 1024) + once > 152 * 1024) waves /= 2;
   ch.stretches = waves;
@@ -501,15 +489,13 @@ hipError_t launch_tile(const Q4Args &a, int e4m3, hipStream_t s) {
 // One type of x a file (product_*.hip).
 hipError_t PPOCR_Q4_LAUNCH(const Q4Args &a, int e4m3, hipStream_t s) {
   constexpr int X = PPOCR_Q4_X;
-  const long tiles = (a.n + 15L) / 16 * ((a.m + 15) / 16);
-  // As few tiles a workgroup as all run at once with (18385 outputs of 1024
-  // inputs from 5 rows of f32: 288 workgroups 13.9 us, 144 of them 11.0).
-  const long at_once = kAtOnce<X> * (kWaves / waves_of(a.k));
-  if (tiles <= at_once) return launch_tile<X, 1>(a, e4m3, s);
-  if (tiles <= 2 * at_once) return launch_tile<X, 2>(a, e4m3, s);
-  if constexpr (X == PPOCR_F32)
-    if (tiles > 4 * at_once && tiles <= 8 * at_once) return launch_tile<X, 8>(a, e4m3, s);
-  return launch_tile<X, 4>(a, e4m3, s);
+  switch (q4_tiles(X, a.m, a.n, a.k)) {
+    case 1: return launch_tile<X, 1>(a, e4m3, s);
+    case 2: return launch_tile<X, 2>(a, e4m3, s);
+    case 4: return launch_tile<X, 4>(a, e4m3, s);
+  }
+  if constexpr (X == PPOCR_F32) return launch_tile<X, 8>(a, e4m3, s);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace ppocr

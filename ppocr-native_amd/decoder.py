@@ -64,6 +64,9 @@ def _functions() -> dict:
         fn = L.ppocr_hip_paged_attention_workspace
         fn.argtypes, fn.restype = [cache, n, n, n], n
         fns["workspace"] = fn
+        fn = L.ppocr_hip_q4_product_tiles
+        fn.argtypes, fn.restype = [n, n, n, i], n
+        fns["tiles"] = fn
         _fns.update(fns)  # all at once: another thread may be looking
     return _fns
 
@@ -90,6 +93,11 @@ def q4_product(x: int, q: int, scales: int, y: int, m: int, n: int, k: int, *, g
     4 bits a weight, g = i / group."""
     _call("q4_product", x, x_stride, x_scales, x_group, q, scales, zeros, bias, y, y_stride, m, n, k, group, x_type,
           scale_type, y_type, stream)
+
+
+def q4_product_tiles(m: int, n: int, k: int, x_type: int = F32) -> int:
+    """Tiles of 16 outputs that a workgroup of `q4_product` takes: which of its kernels runs."""
+    return (_fns or _functions())["tiles"](m, n, k, x_type)
 
 
 def kv_append(k: int, v: int, cache: KvCache, table: int, table_width: int, lengths: int, batch: int, rows: int, *,

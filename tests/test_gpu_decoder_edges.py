@@ -12,6 +12,7 @@ import pytest
 import decoder_plain as R
 from ppocr_native_amd import decoder as D
 from ppocr_native_amd.devmem import synchronize
+from test_gpu_decoder import run_product
 
 pytestmark = pytest.mark.gpu
 STEP = R.STEP
@@ -217,3 +218,48 @@ def test_product_that_overflows():
     y = R.back(dy, np.float32, (2, 20))
     assert (y[0, ::2] == -np.inf).all() and (y[0, 1::2] == np.inf).all()
     assert (y[1, ::2] == -512).all() and (y[1, 1::2] == 448).all()
+
+
+# ------------------------------------------------------ codes of 8 bits of the norm
+
+@pytest.mark.parametrize("y_type", [D.E4M3, D.I8])
+@pytest.mark.parametrize("rows,c,group", [(64, 16384, 0), (64, 16384, 128), (3, 40000, 0), (500, 2000, 32)])
+def test_norm_codes_are_the_nearest(y_type, rows, c, group):
+    # The same norm in F32 tells y. A scale is max |y| times 1 / 448 (127): two roundings, of half a step each, so at
+    # most 2^-23 (1 + 2^-24) off. A code is that of y / scale, which is rounded to f32 once before: next to a code's
+    # border it may fall to the other side by half a step of f32.
+    rng = np.random.default_rng(c)
+    x, w = rng.normal(0, 1, (rows, c)).astype(np.float32), rng.normal(1, 0.2, c).astype(np.float32)
+    groups, size, top = -(-c // group) if group else 1, group or c, 448.0 if y_type == D.E4M3 else 127.0
+    dx, dw, dy = R.on_gpu(x), R.on_gpu(w), R.on_gpu(np.zeros((rows, c), np.float32))
+    d8, ds = R.on_gpu(np.zeros((rows, c), np.uint8)), R.on_gpu(np.zeros((rows, groups), np.float32))
+    print(f"norm codes {rows}x{c} type {y_type} group {group}", flush=True)
+    D.rms_norm(dx.addr, dw.addr, dy.addr, rows, c)
+    D.rms_norm(dx.addr, dw.addr, d8.addr, rows, c, scales=ds.addr, y_type=y_type, group=group)
+    synchronize()
+    y = R.back(dy, np.float32, (rows, c)).astype(np.float64)
+    s = R.back(ds, np.float32, (rows, groups))
+    most = np.stack([np.abs(y[:, i:i + size]).max(1) for i in range(0, c, size)], 1)
+    assert int((np.abs(s - most / top) > most / top * STEP * (1 + STEP / 2)).sum()) == 0
+    quotient = y / np.repeat(s.astype(np.float64), size, 1)[:, :c]
+    step = np.ones_like(quotient)
+    if y_type == D.E4M3:
+        step = 2.0 ** (np.maximum(np.floor(np.log2(np.maximum(np.abs(quotient), 1e-30))), -6) - 3)
+    got = R.values(R.back(d8, np.uint8, (rows, c)), y_type)
+    assert int((np.abs(got - quotient) > step / 2 + np.abs(quotient) * STEP / 2).sum()) == 0
+
+
+# ------------------------------------------------ the product's kernels of several tiles
+
+# Tiles a workgroup takes: 2 and 4 of each type of x, 8 of f32 (test_decoder_tiles.py holds these sizes to that);
+# last strips that are cut; rows of weights of 16-, 4- and 1-byte alignment; more blocks of rows than one.
+TILES = [(1, 6000, 520, 32), (5, 9003, 640, 64), (16, 17001, 1030, 128), (17, 8215, 530, 32), (40, 6001, 513, 64),
+         (3, 40005, 600, 32), (16, 17000, 1088, 32), (9, 17100, 576, 128), (2, 17500, 520, 64)]
+
+
+@pytest.mark.parametrize("x_type", [D.F32, D.BF16, D.F16, D.E4M3, D.I8])
+@pytest.mark.parametrize("m,n,k,group", TILES)
+def test_product_of_several_tiles(x_type, m, n, k, group):
+    y_type = x_type if x_type in R.REAL else D.BF16
+    run_product(np.random.default_rng(n), m, n, k, group, x_type, D.F32 if group == 64 else D.F16, y_type, group != 64,
+                group == 128, x_group=group if x_type not in R.REAL and m % 2 else 0, gap=3 if group == 32 else 0)
