@@ -12,7 +12,7 @@ import pytest
 import decoder_plain as R
 from ppocr_native_amd import decoder as D
 from ppocr_native_amd.devmem import synchronize
-from test_gpu_decoder import run_product
+from test_gpu_decoder import run_product, run_prompt
 
 pytestmark = pytest.mark.gpu
 STEP = R.STEP
@@ -263,3 +263,47 @@ def test_product_of_several_tiles(x_type, m, n, k, group):
     y_type = x_type if x_type in R.REAL else D.BF16
     run_product(np.random.default_rng(n), m, n, k, group, x_type, D.F32 if group == 64 else D.F16, y_type, group != 64,
                 group == 128, x_group=group if x_type not in R.REAL and m % 2 else 0, gap=3 if group == 32 else 0)
+
+
+# ------------------------------- the prompt attention's heads side by side, and head sizes
+
+HEADS = [(4, 1), (8, 2), (8, 1), (6, 1), (7, 1)]  # four, two or one of a key head's in a workgroup
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads,kv_heads", HEADS)
+@pytest.mark.parametrize("nq,nk", [([1], [1]), ([5, 0, 64, 1, 33], [5, 0, 64, 1, 33]), ([3, 70, 9], [200, 70, 140]),
+                                   ([130, 20], [40, 7]), ([257], [300])])
+def test_prompt_heads(t, heads, kv_heads, nq, nk):
+    for window, sinks in ((0, 0), (20, 4)):
+        run_prompt(np.random.default_rng(heads), nq, nk, heads, kv_heads, 64, t, window, sinks)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim", [40, 104, 128, 136, 160, 192, 256])
+def test_prompt_dims(t, dim):
+    # Head sizes in the kernels for those up to 64, 96, 128, 192 and 256, four query heads to a key head.
+    rng = np.random.default_rng(dim)
+    run_prompt(rng, [150, 0, 33], [150, 4, 60], 4, 1, dim, t, 0, 0)
+    run_prompt(rng, [150, 0, 33], [150, 4, 60], 4, 1, dim, t, 50, 3)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (17, 40), (64, 64), (100, 300), (128, 129), (5000, 2)])
+def test_prompt_heads_window(t, window, sinks):
+    run_prompt(np.random.default_rng(window), [290, 70], [400, 70], 4, 1, 64, t, window, sinks)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("window", [0, 31, 200])
+def test_prompt_heads_ragged_texts(t, window):
+    nq = [0, 400, 1, 33, 0, 290, 128, 64, 31, 5, 0]
+    run_prompt(np.random.default_rng(18), nq, [n + i % 3 for i, n in enumerate(nq)], 4, 1, 64, t, window, 3)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 64), (8, 1, 128), (6, 1, 192), (4, 1, 96)])
+def test_prompt_heads_nan_in_unseen_keys(t, heads, kv_heads, dim):
+    for window, sinks, at in ((0, 0, 150), (40, 3, 1), (9, 0, 260)):
+        run_prompt(np.random.default_rng(at), [290, 40], [290, 40], heads, kv_heads, dim, t, window, sinks,
+                   poison=[(0, at), (1, 20)])
