@@ -307,3 +307,58 @@ def test_prompt_heads_nan_in_unseen_keys(t, heads, kv_heads, dim):
     for window, sinks, at in ((0, 0, 150), (40, 3, 1), (9, 0, 260)):
         run_prompt(np.random.default_rng(at), [290, 40], [290, 40], heads, kv_heads, dim, t, window, sinks,
                    poison=[(0, at), (1, 20)])
+
+
+# ------------------------------------------------------------ a first call inside a capture
+
+FIRST = """
+import ctypes as C
+import conftest
+import numpy as np
+import decoder_plain as R
+import test_gpu_decoder as T
+from ppocr_native_amd import decoder as D
+from ppocr_native_amd.devmem import hip, synchronize
+
+t, rows, heads, dim = D.BF16, 150, 4, 64
+rng = np.random.default_rng(2)
+steps = [T.Step(np.random.default_rng(9), t=t) for _ in range(2)]
+q, k, v = (R.on_gpu(R.stored(rng.normal(0, 1, (rows, h, dim)), t)) for h in (heads, 1, 1))
+y = [R.on_gpu(np.zeros((rows, heads, dim), np.uint16)) for _ in range(2)]
+starts = R.on_gpu(np.array([0, rows], np.int32))
+
+
+def run(i, stream):
+    steps[i].run(stream)
+    D.window_attention(q.addr, k.addr, v.addr, y[i].addr, starts.addr, starts.addr, 1, rows, rows, heads, 1, dim,
+                       scale=0.125, type=t, stream=stream)
+
+
+h = hip()
+stream, graph, ready = T._stream(), C.c_void_p(), C.c_void_p()
+assert h.hipStreamBeginCapture(stream, 0) == 0  # the global mode: nothing unsafe in any thread
+run(0, stream.value)
+assert h.hipStreamEndCapture(stream, C.byref(graph)) == 0
+h.hipGraphInstantiate.argtypes = [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]
+h.hipGraphLaunch.argtypes = [C.c_void_p, C.c_void_p]
+assert h.hipGraphInstantiate(C.byref(ready), graph, None, None, 0) == 0
+for i in range(3):
+    assert h.hipGraphLaunch(ready, stream) == 0
+    synchronize()
+    run(1, 0)
+    synchronize()
+    steps[0].check()
+    for a, b in zip(steps[0].outputs() + [R.back(y[0], np.uint16, (rows, heads, dim))],
+                    steps[1].outputs() + [R.back(y[1], np.uint16, (rows, heads, dim))]):
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    print("replay", i, flush=True)
+print("the same", flush=True)
+"""
+
+
+def test_first_calls_inside_a_capture():
+    # In a process of its own, whose first calls of these layers are captured.
+    print("first calls inside a capture", flush=True)
+    r = subprocess.run([sys.executable, "-c", FIRST], cwd=Path(__file__).parent, capture_output=True, text=True,
+                       timeout=100)
+    assert r.returncode == 0 and r.stdout.endswith("the same\n"), (r.returncode, r.stdout[-500:], r.stderr[-2000:])
