@@ -272,8 +272,8 @@ int ppocr_hip_rms_norm(const void *x, size_t x_stride, const void *residual, siz
  * and scaled in f32. k and x_stride up to 2^24. Made for up to 64 rows: every
  * 16 read the weights again (from the L2 cache, where they fit). An infinity
  * in x gives NaN in its row. Finite x may be of any size: where the matrix
- * products' sums leave f32's range, an output is computed again in f64, one by
- * one. */
+ * products' sums leave f32's range, an output is computed again in f64, which
+ * is slow. */
 int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, size_t x_group, const uint8_t *q,
                          const void *scales, const uint8_t *zeros, const void *bias, void *y, size_t y_stride,
                          size_t m, size_t n, size_t k, size_t group, int x_type, int scale_type, int y_type,

@@ -15,7 +15,8 @@
 // into three bf16 parts first (split.hpp), 8-bit rows are exact in bf16.
 // (16 + q) x passes f32's range before q x does, and f32 values past bf16's
 // largest are infinite in the split: an output of f32 or bf16 rows that comes out
-// as an infinity or NaN is computed again, in f64 from the formula as it stands.
+// as an infinity or NaN is computed again, in f64 from the formula as it stands,
+// where its row of x is finite.
 //
 // A workgroup takes up to NT tiles of 16 outputs, its waves every W-th stretch
 // of 128 inputs of them; the waves' sums are added in LDS in their order. The
@@ -147,30 +148,50 @@ struct Chunk {
   int align;  // of the weights' rows: 16, 4 or 1
 };
 
-// Output n of row m by one wave, in f64; NaN where x has an infinity or NaN.
+// Whether row m of x has no infinity or NaN: asked by a whole wave.
+template <int X>
+__device__ __forceinline__ bool row_is_finite(const Q4Args &a, int m, int lane) {
+  const num_t<X> *x = (const num_t<X> *)a.x + m * a.x_stride;
+#pragma unroll 1
+  for (int k0 = 0; k0 < a.k; k0 += 512) {
+    const int k = k0 + 8 * lane;
+    num_t<X> v[8];
+    load_n(x + k, (long)a.k - k, v);
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 8; i++) bad |= !(fabsf(Num<X>::get(v[i])) < INFINITY);
+    if (__any(bad)) return false;
+  }
+  return true;
+}
+
+// Output n of row m (the same in all lanes; n: of lane % 16) by one wave, in
+// f64, lane / 16's eight inputs of each 32.
 template <int X, int GROUP>
 __device__ __forceinline__ float q4_alone(const Q4Args &a, int m, int n, int lane) {
+  const int row_bytes = (a.k + 1) / 2;
   const num_t<X> *x = (const num_t<X> *)a.x + m * a.x_stride;
-  const uint8_t *q = a.q + (long)n * ((a.k + 1) / 2);
+  const uint8_t *q = a.q + (long)n * row_bytes;
   const long g0 = (long)n * a.groups;
   double sum = 0.0;
 #pragma unroll 1
-  for (int k0 = 0; k0 < a.k; k0 += 64) {
-    const int k = k0 + lane;
-    float v = 0.0f;
-    if (k < a.k) v = Num<X>::get(x[k]);
-    if (__any(!(fabsf(v) < INFINITY))) return __uint_as_float(0x7fc00000u);
-    if (k < a.k) {
-      const long g = g0 + k / GROUP;
-      const float s = a.scale_type == PPOCR_F32    ? ((const float *)a.scales)[g]
-                      : a.scale_type == PPOCR_BF16 ? (float)((const __bf16 *)a.scales)[g]
-                                                   : (float)((const _Float16 *)a.scales)[g];
-      const int w = (q[k / 2] >> k % 2 * 4 & 15) - (a.zeros ? a.zeros[g] : 8);
-      sum += double(v) * w * double(s);
-    }
-  }
+  for (int k = lane / 16 * 8; k < a.k; k += 32) {
+    num_t<X> v[8];
+    uint8_t b[4];
+    load_n(x + k, (long)a.k - k, v);
+    load_n(q + k / 2, (long)row_bytes - k / 2, b);
+    const long g = g0 + k / GROUP;
+    const float s = a.scale_type == PPOCR_F32    ? ((const float *)a.scales)[g]
+                    : a.scale_type == PPOCR_BF16 ? (float)((const __bf16 *)a.scales)[g]
+                                                 : (float)((const _Float16 *)a.scales)[g];
+    const int z = a.zeros ? a.zeros[g] : 8;
+    double part = 0.0;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    for (int i = 0; i < 8; i++) part += double(Num<X>::get(v[i])) * ((b[i / 2] >> i % 2 * 4 & 15) - z);
+    sum += part * double(s);
+  }
+  sum += __shfl_xor(sum, 16);
+  sum += __shfl_xor(sum, 32);
   return float(sum);
 }
 
@@ -433,12 +454,17 @@ __global__ __launch_bounds__(64 * kWaves, (X != PPOCR_F32 ? 4 : 2)) void q4_rows
       put(m, n, v);
     }
     if constexpr (X == PPOCR_F32 || X == PPOCR_BF16)
-      if (__any(bad)) {  // rare
-        for (int i = 64 * wave; i < AT * 256; i += i % 64 == 63 ? threads - 63 : 1) {
-          const int m = row_of(i), n = col_of(i);
-          if (m >= a.m || n >= a.n || fabsf(sum_of(i)) < INFINITY) continue;
-          const float v = q4_alone<X, GROUP>(a, m, n, lane);
-          if (lane == i % 64) put(m, n, v);  // (the lane that wrote it)
+      if (__any(bad)) {  // rare: this wave's rows, 16 outputs at a time
+        for (int i0 = 64 * wave; i0 < AT * 256; i0 += threads) {
+          const int m = row_of(i0 + lane), n = col_of(i0 + lane);
+          const unsigned long long again =
+              __ballot(m < a.m && n < a.n && !(fabsf(sum_of(i0 + lane)) < INFINITY));
+          for (int r = 0; r < 4; r++) {
+            const int row = row_of(i0) + r;
+            if (!(again >> 16 * r & 0xffff) || !row_is_finite<X>(a, row, lane)) continue;  // (NaN stays)
+            const float v = q4_alone<X, GROUP>(a, row, min(n, a.n - 1), lane);
+            if (lane / 16 == r && again >> lane & 1) put(m, n, v);  // (the lane that wrote it)
+          }
         }
       }
   }
