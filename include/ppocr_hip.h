@@ -224,8 +224,9 @@ int ppocr_hip_row_argmax(const float *x, float *y, size_t rows, size_t cols, voi
  * What a program calls that writes or corrects text token by token after the
  * recogniser (no reference counterpart: the engine's networks read a line in
  * one pass). Device pointers and a HIP stream (`stream` NULL = the default
- * stream of the current device; another device's stream is launched on that
- * device, to which the pointers then belong). The calls queue their kernels
+ * stream of the current device, hipStreamPerThread its thread's; another
+ * device's stream is launched on that device, to which the pointers then
+ * belong; hipStreamLegacy is refused). The calls queue their kernels
  * and return: they never allocate, wait or keep anything, so they may be
  * captured in a HIP graph and made from several threads. Each returns 0, or
  * nonzero with the reason in `err`, and then has queued nothing.

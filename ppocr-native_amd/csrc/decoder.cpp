@@ -33,12 +33,19 @@ struct Fail {
   }
 };
 
-// Makes the stream's device current for the launch, if it is another.
+// Makes the stream's device current for the launch, if it is another. Two
+// handles are numbers and no streams: that of the thread's own stream, which is
+// the current device's, and that of the legacy default stream, which ended the
+// process in the runtime and is refused (NULL is that stream).
 struct OnDevice {
   int before = -1;
   hipError_t e = hipSuccess;
   explicit OnDevice(hipStream_t s) {
-    if (!s) return;
+    if (s == hipStreamLegacy) {
+      e = hipErrorInvalidHandle;
+      return;
+    }
+    if (!s || s == hipStreamPerThread) return;
     hipDevice_t of = 0;
     int now = 0;
     if ((e = hipGetDevice(&now)) != hipSuccess || (e = hipStreamGetDevice(s, &of)) != hipSuccess) return;
