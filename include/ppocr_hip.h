@@ -234,7 +234,10 @@ int ppocr_hip_row_argmax(const float *x, float *y, size_t rows, size_t cols, voi
  * Types are the codes below. Strides count values from one row to the next;
  * 0 means rows without a gap. Pointers are aligned to their type's size.
  * Sums, norms, softmax statistics and products are held in 32 bits or more
- * and rounded once, at the end, to the nearest value of the output's type. */
+ * and rounded once, at the end, to the nearest value of the output's type. The
+ * softmax's weights go into their products with v in fewer bits where v has 16:
+ * in two numbers of v's type in the decode attention (about 16 bits in BF16, 22
+ * in F16), in one in the prompt attention; see there. */
 enum {
   PPOCR_F32 = 0,
   PPOCR_BF16 = 1,
@@ -252,9 +255,10 @@ enum {
  * row (`group` 0) or of each `group` (32, 64 or 128; the last may be cut off)
  * share the scale max |y| / 448 or max |y| / 127 in `scales`
  * [rows][groups, or 1], y is the nearest code of y / scale, and a group of
- * zeros has scale 0 and codes 0. A group with an infinity or NaN has the
- * scale NaN (codes 0x7f in E4M3, 0 in I8). Squares are summed in f32: values
- * past 1e19 overflow the sum and give zeros. */
+ * zeros (or whose scale would be below 2^-126) has scale 0 and codes 0. A group
+ * with an infinity or NaN has the scale NaN (codes 0x7f in E4M3, 0 in I8).
+ * Squares are summed in f32: values past 1e19 overflow the sum and give zeros,
+ * and where eps is 0, rows of values below 1e-19 lose theirs. */
 int ppocr_hip_rms_norm(const void *x, size_t x_stride, const void *residual, size_t residual_stride,
                        const void *weight, void *sum, size_t sum_stride, void *y, size_t y_stride, float *scales,
                        size_t rows, size_t c, int type, int y_type, size_t group, float eps, void *stream, char *err,
@@ -312,7 +316,8 @@ int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_
  *   y[b][h] = sum over i of softmax_i(scale * q[b][h] . k[i][h']) v[i][h'],  h' = h / (heads / cache heads),
  * for q and y of `batch` rows of heads x dim in the cache's type, over tokens
  * i < lengths[b]; with `window` > 0 only the last `window` of them and the
- * first `sinks`. A text of length 0 (or less) gives zeros; one whose length
+ * first `sinks`. A text of length 0 (or less) gives zeros, as does one all of
+ * whose products q . k are -infinity; one whose length
  * passes table_width * page_size, or with a seen token in a page that does
  * not exist, gives NaN. What lies in unseen tokens does not matter; an
  * infinity in the v of a seen one gives that infinity (in F16, NaN where its
@@ -336,7 +341,8 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
  * and values rows starts_k[b] .. starts_k[b + 1] - 1 of k and v. With nq
  * queries and nk keys, query i stands at p = nk - nq + i and sees the keys
  * j <= p with j > p - window (`window` 0: all) or j < sinks; y is as above.
- * A query that sees no key gives zeros. Rows outside every text are left as
+ * A query that sees no key (or whose products are all -infinity) gives zeros.
+ * Rows outside every text are left as
  * they were. `rows_q`, `rows_k`: the rows there are; starts are int32, not
  * decreasing, within them (rows past them are not touched), at most 2^24 rows of
  * q, and heads x (rows_q / 32 + batch) below 2^24. q and y: heads x

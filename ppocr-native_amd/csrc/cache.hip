@@ -13,7 +13,7 @@ namespace {
 // workgroups, a token a wave at a time: its place is the same in all lanes,
 // its rows of k and v are copied in 16-byte pieces of a head, two of each on
 // their way. Memory bound: 5400 tokens of 8 heads of 128 in 16 bits (44 MB) in
-// 9.0 us, 4.9 TB/s; at a token a text bound by the launch.
+// 9.2 us, 4.8 TB/s; at a token a text bound by the launch.
 // WHOLE: heads are whole pieces.
 template <typename V>
 __device__ __forceinline__ v4u load16(const V *p) {
@@ -106,11 +106,13 @@ __device__ __forceinline__ int tiles_a_part(int tiles, int each, int splits) {
 }
 
 // Reading the seen keys and values bounds it: 32 texts of up to 16384 tokens, 8
-// key heads of 128 in bf16 (1.08 GB), 227 us, 4.8 TB/s, as fast as a copy. Each
-// wave keeps one tile's loads on their way while it takes in the one before
-// (367 us when it asked for a tile as it came to it), and the key heads of one
-// part of a text run side by side, so that they read whole rows of a page
-// together (264 us with the parts of one head side by side).
+// key heads of 128 in bf16 (1.08 GB), 217 us and 6 for the join, 5.0 TB/s, where
+// a kernel that only reads has 6.7; the address unit is 76 % busy, as a wave's
+// load of K takes 16 bytes of each of 16 rows. Each wave keeps one tile's loads
+// on their way while it takes in the one before (367 us when it asked for a tile
+// as it came to it), and the key heads of one part of a text run side by side, so
+// that they read whole rows of a page together (264 us with the parts of one head
+// side by side).
 //
 // Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.x, part
 // blockIdx.y of its tiles. PAGED16: pages are multiples of 16 tokens.
@@ -330,8 +332,11 @@ hipError_t launch_parts(const PagedArgs &a, hipStream_t s) {
 template <int T>
 hipError_t launch_paged(const PagedArgs &a, hipStream_t s) {
   // Heads of 96 and 192 in a kernel of their own size: 32 texts of up to 8000
-  // tokens, 8 key heads in bf16, 126 to 110 and 476 to 240 us against those of
-  // 128 and 256, whose loads past dim are requests all the same.
+  // tokens, 8 key heads in bf16, 126 to 109 and 476 to 238 us against those of
+  // 128 and 256, whose loads past dim are requests all the same. Other heads
+  // run in the next power of two (80: 120 us, 136: 467, 200: 495 to 501), which
+  // spills at 256, and those that are no multiple of 8 value by value, with two
+  // tiles in registers and up to 600 of them spilled (100: 866 us, 129: 2418).
   const hipError_t e = a.c.dim <= 32    ? launch_parts<T, 32>(a, s)
                        : a.c.dim <= 64  ? launch_parts<T, 64>(a, s)
                        : a.c.dim == 96  ? launch_whole<T, 96>(a, s)
@@ -366,7 +371,9 @@ PagedParts paged_parts(int batch, int heads, int kv_heads, int type, long longes
 }
 
 hipError_t launch_kv_append(const AppendArgs &a, int type, hipStream_t s) {
-  // A token a wave where the texts' shares are even, up to 8192 waves.
+  // A token a wave where the texts' shares are even, up to 8192 waves. (Where they
+  // are not, one text's waves take many in turn: 8192 tokens of one text and one
+  // each of 63 others take 54.6 us, 129 each of 64 take 12.0.)
   const long share = (a.rows + a.batch - 1) / a.batch, most = 2048 / a.batch + 1;
   const long x = std::min((share + 3) / 4, most);
   const dim3 grid(unsigned(std::max(x, 1L)), a.batch);

@@ -25,19 +25,21 @@
 // for a load before it copies the register it came to (a ring of four in
 // registers took 0.9 us a stretch). Four neighbouring lanes load a row's 64
 // bytes: with a row a lane, as the operand has them, the address unit takes a
-// cycle a lane and was 95 % busy.
+// cycle a lane and was 95 % busy (35 % so).
 //
 // x, the scales and the zero points are the same for all of a workgroup's
 // waves, or come in rows too short to load well: they go to LDS a chunk of
 // stretches at a time, x as finished operands.
 //
-// 4096 inputs to 28672 outputs (59 to 71 MB): one row of bf16, groups of 128,
-// 17.5 us, 3.4 TB/s; 16 rows of f16, groups of 32 with zero points, 26 us, 2.7
-// TB/s; 5 rows of f32, groups of 64, 30 us. What is left is the wait for a
-// chunk at its start and the launch. Fetching a chunk's x ahead into registers
-// spilled (60 us for the 26); tiles of 32 and 64 rows of x were slower than
-// blocks of 16 that share the weights through L2 (64 rows of f32: 715 us
-// against 171).
+// 4096 inputs to 28672 outputs (61 to 71 MB): one row of bf16, groups of 128,
+// 17.2 us, 3.5 TB/s; 16 rows of f16, groups of 32 with zero points, 22.5 us (25
+// in a trace), 3.2 TB/s; 5 rows of f32, groups of 64, 29.6 us; a kernel that only
+// reads takes 11 us for 71 MB. What is left is the wait for a chunk at its start,
+// the conversion and the launch. Each further 16 rows load and convert all of it
+// again: 32 and 64 rows of bf16 41 and 66 us, of f32 86 and 149, of 8 bits 68 (64
+// rows). Fetching a chunk's x ahead into registers spilled (60 us for the 22.5);
+// tiles of 32 and 64 rows of x were slower than blocks of 16 that share the
+// weights through L2 (64 rows of f32: 715 us against 171 at that time).
 #include <algorithm>
 
 #include "decoder.hpp"

@@ -25,10 +25,12 @@ __device__ __forceinline__ int wave_total(int v, int bits) {
 // walks the starts, 64 texts at a time. Of those, blocks that are far into
 // their text come first, as they see most keys, so that the last to run are
 // short (14 texts of up to 6971 tokens, one head of 256 in f32, 2.6 ms text by
-// text, 2.1 so; 20 of up to 3000, 4 heads of 128 in bf16, 155 and 132 us).
-// Blocks further in than the window see as many keys as one another and come
-// text by text: neighbours share most of them. Starts past the rows there are,
-// and such as decrease, leave texts of no rows.
+// text, 2.1 so; 20 of up to 3000, 4 heads of 128 in bf16, 155 and 132 us; but two
+// of up to 3000, 12 heads of 96 in f32, 409 and 439). Blocks further in than the
+// window see as many keys as one another and come text by text: neighbours share
+// most of them. Starts past the rows there are, and such as decrease, leave texts
+// of no rows. (The walk is all that short texts by the thousand wait for: 1000 of
+// 8 tokens, 8 heads of 64, 87 us, 8000 of 4 2.3 ms.)
 __device__ __forceinline__ bool find_block(const PromptArgs &a, int index, int size, Block &out) {
   const int lane = threadIdx.x % 64, far = a.window ? a.window / size + 1 : 1 << 30;
   for (int b0 = 0; b0 < a.batch; b0 += 64) {
@@ -136,7 +138,10 @@ __device__ __forceinline__ void attend_alone(const PromptArgs &a, const Block &b
 }
 
 // 16 queries of one head, from the block's query `first` on, by one wave,
-// keys and values straight from memory (the caches): any type and dim.
+// keys and values straight from memory (the caches): any type and dim. Two tiles
+// are in registers, of which heads past 64 spill some, and value by value most:
+// four texts of up to 1500 tokens, 8 heads of 129 in bf16, take 2.8 ms, where 128
+// in tiles take 47 us.
 template <int T, int DP, int DIMS>
 __device__ __forceinline__ void attend_rows(const PromptArgs &a, const Block &bl, int head, int first) {
   typedef Attend<T, DP, DIMS> A;
@@ -271,9 +276,10 @@ __device__ __forceinline__ int not_finite2(uint32_t x) {
 // cycle a lane.)
 // What bounds it: the matrix cores, which a wave's softmax leaves waiting where
 // the other wave of its SIMD has none of its own to do. One text of 8192
-// tokens, 32 heads of 128 in bf16: 0.62 ms, 880 TFLOP/s of the seen keys'
-// products, where a library product of 8192 x 8192 x 8192 runs at 1124; a window
-// of 2048 over two such texts 0.32 to 0.36 ms, 720 to 800 TFLOP/s. Eight waves
+// tokens, 32 heads of 128 in bf16: 0.63 ms, 874 TFLOP/s of the seen keys'
+// products, where a library product of 8192 x 8192 x 8192 runs at 1124 (f32: 4.3
+// ms, 129 of 154); a window of 2048 over two such texts 0.32 to 0.36 ms, 720 to
+// 800 TFLOP/s. Eight waves
 // a workgroup: 2 to 3 % faster on these, 10 to 16 % slower on heads of 64 and on
 // 1115 tokens of 4 heads.
 // WHOLE: dim == DP and fills the pieces.
