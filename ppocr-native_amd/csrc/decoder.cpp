@@ -74,6 +74,12 @@ bool stride_of(size_t given, size_t width, long *out) {
   return (!given || given >= width) && given <= kMostStride;
 }
 
+// Whether the 4-bit product takes these sizes.
+bool q4_sizes(size_t m, size_t n, size_t k) {
+  return k && k <= size_t(1) << 24 && n <= kMost && m <= size_t(1) << 20 &&
+         (n + 15) / 16 * ((m + 15) / 16) <= size_t(1) << 24;
+}
+
 // The cache's own checks; fills `c`.
 int cache_of(const Fail &fail, const char *what, const ppocr_kv_cache *k, const int32_t *table, size_t table_width,
              const int32_t *lengths, CacheArgs &c) {
@@ -153,7 +159,7 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
   if (group != 32 && group != 64 && group != 128)
     return fail("4-bit product: groups of %zu inputs: 32, 64 or 128 are taken", group);
   if (m == 0 || n == 0) return 0;
-  if (!k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20 || (n + 15) / 16 * ((m + 15) / 16) > size_t(1) << 24)
+  if (!q4_sizes(m, n, k))
     return fail("4-bit product: %zu rows of %zu inputs to %zu outputs", m, k, n);
   if (!x || !q || !scales || !y || (x8 && !x_scales))
     return fail("4-bit product: x, q, scales, y and (for 8-bit x) x_scales are needed");
@@ -179,8 +185,7 @@ int ppocr_hip_q4_product(const void *x, size_t x_stride, const float *x_scales, 
 }
 
 size_t ppocr_hip_q4_product_tiles(size_t m, size_t n, size_t k, int x_type) {
-  if (x_type < PPOCR_F32 || x_type > PPOCR_I8 || !m || !n || !k || k > size_t(1) << 24 || n > kMost || m > size_t(1) << 20)
-    return 0;
+  if (x_type < PPOCR_F32 || x_type > PPOCR_I8 || !m || !n || !q4_sizes(m, n, k)) return 0;
   return size_t(q4_tiles(x_type, int(m), int(n), int(k)));
 }
 

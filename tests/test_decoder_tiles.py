@@ -24,6 +24,6 @@ def test_product_sizes_reach_every_number_of_tiles(x_type):
 
 def test_tiles_of_sizes_that_are_refused():
     for m, n, k, t in ((0, 16, 32, D.F32), (1, 0, 32, D.F32), (1, 16, 0, D.F32), (1, 16, 1 << 25, D.F32),
-                       (1, 16, 32, 5), (1, 16, 32, -1), (1 << 21, 16, 32, D.F16)):
+                       (1, 16, 32, 5), (1, 16, 32, -1), (1 << 21, 16, 32, D.F16), (1 << 20, 1 << 20, 32, D.F16)):
         assert D.q4_product_tiles(m, n, k, t) == 0
     assert D.q4_product_tiles(1, 16, 32, D.I8) == 1
