@@ -358,6 +358,84 @@ int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, si
                                size_t kv_heads, size_t dim, int type, float scale, size_t window, size_t sinks,
                                void *stream, char *err, size_t err_len);
 
+/* Append new keys and values with the rotation of keys and queries by their
+ * positions on the way. Rows, starts, places and the cache are as
+ * ppocr_hip_kv_append's; v goes as it is. A row's position is its token's place
+ * in its text, or positions[row] where `positions` (int32, one a row) is not
+ * NULL. Of each head of k, and of q (`heads` heads of the cache's dim a row, a
+ * multiple of the cache's heads; q NULL and heads 0: no queries), the first
+ * `rotary` dims (even, up to dim; 0: none) are turned, pair j by the angle
+ * a = position * freqs[j] (`freqs`: rotary / 2 floats, radians a position):
+ *   x1' = x1 cos a - x2 sin a,  x2' = x2 cos a + x1 sin a
+ * for the dims j and j + rotary / 2 (`pairs` 0) or 2 j and 2 j + 1. The angle
+ * is held in f64, its cosine and sine, the two products and their sum are
+ * rounded to f32, the result to the type. q's rows go to q_out (which may be q,
+ * with its stride, and overlaps nothing else), also where the token has no place
+ * in the cache; rows outside every text, and rows of q_out past `rows`, are left
+ * as they were. starts do not decrease; where they do, only which rows are taken
+ * is not determined. */
+int ppocr_hip_kv_append_rotated(const void *q, size_t q_stride, void *q_out, size_t q_out_stride, size_t heads,
+                                const void *k, size_t k_stride, const void *v, size_t v_stride,
+                                const ppocr_kv_cache *cache, const int32_t *table, size_t table_width,
+                                const int32_t *lengths, const int32_t *starts, const int32_t *positions,
+                                const float *freqs, size_t rotary, int pairs, size_t batch, size_t rows, void *stream,
+                                char *err, size_t err_len);
+
+/* A paged cache of keys and values in 4 bits, with a scale and a minimum (F16)
+ * for each `group` dims of a token's head: 32, 64 or 0 (a whole head). A page
+ * holds `page_size` tokens (a multiple of 16) of `heads` heads of `dim` values
+ * (1 to 256, padded to P = 32, 64, 96, 128, 192 or 256), as a chunk for each
+ * head, ppocr_hip_kv4_page_bytes in all (0 for sizes that are refused); pages
+ * are `page_stride` bytes apart (a multiple of 16; 0: without a gap), `data` is
+ * 16-byte aligned. A chunk is the planes
+ *   K codes [token][quarter q of 4][block c of P / 32][byte j of 4]: dims 32 c + 8 q + 2 j (low bits) and the next,
+ *   K scales [token][groups], K minima [token][groups],
+ *   V codes [token / 4][column i of 16][block c][token % 4]: dims 32 c + 2 i (low bits) and the next,
+ *   V scales, V minima,
+ * with P / group groups, rounded up; a code n stands for n * scale + minimum. */
+typedef struct ppocr_kv4_cache {
+  void *data;
+  size_t pages, page_size, heads, dim, group;
+  size_t page_stride;
+} ppocr_kv4_cache;
+size_t ppocr_hip_kv4_page_bytes(size_t page_size, size_t heads, size_t dim, size_t group);
+
+/* As ppocr_hip_kv_append_rotated, into a cache in 4 bits: q, k and v have
+ * `type`, k is turned (`rotary` 0: as it is) in f32 and not rounded before
+ *   minimum = F16(min x), scale = F16((max x - minimum) * F32(1 / 15)), at least 0,
+ *   n = round((x - minimum) * (1 / scale)) within 0 .. 15 (0 where scale is 0)
+ * over a group's dims. Values past F16's range are held at its ends; a group
+ * with an infinity or NaN has the scale NaN, minimum 0 and codes 0, and what is
+ * read of it is NaN. Four neighbouring places (0 .. 3, 4 .. 7, ...) share words of V:
+ * appends that run at the same time must not write to the same four. */
+int ppocr_hip_kv4_append(const void *q, size_t q_stride, void *q_out, size_t q_out_stride, size_t heads, const void *k,
+                         size_t k_stride, const void *v, size_t v_stride, const ppocr_kv4_cache *cache,
+                         const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
+                         const int32_t *positions, const float *freqs, size_t rotary, int pairs, size_t batch,
+                         size_t rows, int type, void *stream, char *err, size_t err_len);
+
+/* What a cache in 4 bits holds, as rows of `type`: text b's rows starts[b] ..
+ * starts[b + 1] - 1 of k and v (`rows` of heads x dim; starts NULL: one a text)
+ * get the last tokens below lengths[b], for ppocr_hip_window_attention over a
+ * prompt's past. Rows whose place is negative, or outside every text, are left
+ * as they were; those past the table's row or in a page that does not exist
+ * get NaN. */
+int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const ppocr_kv4_cache *cache,
+                       const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
+                       size_t batch, size_t rows, int type, void *stream, char *err, size_t err_len);
+
+/* ppocr_hip_paged_attention over a cache in 4 bits, q and y of `type`. Codes,
+ * scales and minima enter the sums as they are; the softmax's weights times V's
+ * scales go into their products in two F16 parts (22 bits), f32 queries too, 16-bit
+ * queries whole. A text with a token of scale NaN that it sees gives NaN (in K:
+ * its whole head, in V: the group's dims), a query with an infinity or NaN gives
+ * NaN. Everything else, and the workspace, is as there. */
+size_t ppocr_hip_kv4_attention_workspace(const ppocr_kv4_cache *cache, size_t batch, size_t heads, size_t longest);
+int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cache *cache, const int32_t *table,
+                            size_t table_width, const int32_t *lengths, void *y, size_t y_stride, size_t batch,
+                            size_t heads, int type, float scale, size_t window, size_t sinks, size_t longest,
+                            void *workspace, size_t workspace_bytes, void *stream, char *err, size_t err_len);
+
 /* --- Host stages either side of the model ---------------------------------
  * CPU code in the same library: the recogniser's text from its [T][2]
  * output, and the detector's text boxes from its probability map. Each

@@ -1,7 +1,8 @@
 """The layers of a text decoder on device memory, over the C ABI
 (ppocr_hip_rms_norm, ppocr_hip_q4_product, ppocr_hip_kv_append,
-ppocr_hip_paged_attention, ppocr_hip_window_attention): what a program calls
-that writes or corrects text token by token after the recogniser.
+ppocr_hip_paged_attention, ppocr_hip_window_attention, the append with the
+rotation of positions, the cache in 4 bits ppocr_hip_kv4_*): what a program
+calls that writes or corrects text token by token after the recogniser.
 
 Arguments are device addresses (integers; 0 = none), sizes, strides in values
 (0 = rows without a gap) and a HIP stream (0 = the default stream); see
@@ -46,17 +47,35 @@ class KvCache(C.Structure):
         super().__init__(k, v, pages, page_size, heads, dim, page_stride, token_stride, head_stride, type)
 
 
+class Kv4Cache(C.Structure):
+    """A paged cache in 4 bits (`ppocr_kv4_cache`): the address of its pages,
+    `pages` of them of `page_size` tokens of `heads` heads of `dim` values, a
+    scale and a minimum each `group` (32, 64; 0: a head), pages `page_stride`
+    bytes apart (0: `kv4_page_bytes`)."""
+
+    _fields_ = [("data", C.c_void_p), ("pages", C.c_size_t), ("page_size", C.c_size_t), ("heads", C.c_size_t),
+                ("dim", C.c_size_t), ("group", C.c_size_t), ("page_stride", C.c_size_t)]
+
+    def __init__(self, data: int, pages: int, page_size: int, heads: int, dim: int, group: int = 64,
+                 page_stride: int = 0):
+        super().__init__(data, pages, page_size, heads, dim, group, page_stride)
+
+
 def _functions() -> dict:
     if not _fns:
         L, fns = lib(), {}
         p, n, i, f = C.c_void_p, C.c_size_t, C.c_int, C.c_float
-        cache, end = C.POINTER(KvCache), [p, C.c_char_p, n]
+        cache, cache4, end = C.POINTER(KvCache), C.POINTER(Kv4Cache), [p, C.c_char_p, n]
         for name, args in {
             "rms_norm": [p, n, p, n, p, p, n, p, n, p, n, n, i, i, n, f] + end,
             "q4_product": [p, n, p, n, p, p, p, p, p, n, n, n, n, n, i, i, i] + end,
             "kv_append": [p, n, p, n, cache, p, n, p, p, n, n] + end,
             "paged_attention": [p, n, cache, p, n, p, p, n, n, n, f, n, n, n, p, n] + end,
             "window_attention": [p, n, p, n, p, n, p, n, p, p, n, n, n, n, n, n, i, f, n, n] + end,
+            "kv_append_rotated": [p, n, p, n, n, p, n, p, n, cache, p, n, p, p, p, p, n, i, n, n] + end,
+            "kv4_append": [p, n, p, n, n, p, n, p, n, cache4, p, n, p, p, p, p, n, i, n, n, i] + end,
+            "kv4_read": [p, n, p, n, cache4, p, n, p, p, n, n, i] + end,
+            "kv4_attention": [p, n, cache4, p, n, p, p, n, n, n, i, f, n, n, n, p, n] + end,
         }.items():
             fn = getattr(L, "ppocr_hip_" + name)
             fn.argtypes, fn.restype = args, i
@@ -64,6 +83,12 @@ def _functions() -> dict:
         fn = L.ppocr_hip_paged_attention_workspace
         fn.argtypes, fn.restype = [cache, n, n, n], n
         fns["workspace"] = fn
+        fn = L.ppocr_hip_kv4_attention_workspace
+        fn.argtypes, fn.restype = [cache4, n, n, n], n
+        fns["kv4_workspace"] = fn
+        fn = L.ppocr_hip_kv4_page_bytes
+        fn.argtypes, fn.restype = [n, n, n, n], n
+        fns["kv4_page_bytes"] = fn
         fn = L.ppocr_hip_q4_product_tiles
         fn.argtypes, fn.restype = [n, n, n, i], n
         fns["tiles"] = fn
@@ -128,3 +153,48 @@ def window_attention(q: int, k: int, v: int, y: int, starts_q: int, starts_k: in
     """Causal attention of prompts with a sliding window and sinks."""
     _call("window_attention", q, q_stride, k, k_stride, v, v_stride, y, y_stride, starts_q, starts_k, batch, rows_q,
           rows_k, heads, kv_heads, dim, type, scale, window, sinks, stream)
+
+
+def kv_append_rotated(k: int, v: int, cache: KvCache, table: int, table_width: int, lengths: int, batch: int, rows: int,
+                      *, freqs: int = 0, rotary: int = 0, pairs: bool = False, positions: int = 0, q: int = 0,
+                      q_out: int = 0, heads: int = 0, starts: int = 0, q_stride: int = 0, q_out_stride: int = 0,
+                      k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+    """`kv_append` of keys turned by their positions (first `rotary` dims of a
+    head, halves apart or in neighbouring `pairs`, angle position * freqs[j]);
+    q's rows, turned alike, go to `q_out` (or stay in q, where they are one)."""
+    _call("kv_append_rotated", q, q_stride, q_out, q_out_stride, heads, k, k_stride, v, v_stride, cache, table,
+          table_width, lengths, starts, positions, freqs, rotary, pairs, batch, rows, stream)
+
+
+def kv4_page_bytes(page_size: int, heads: int, dim: int, group: int = 64) -> int:
+    """Bytes of a page of a cache in 4 bits (0 for sizes that are refused)."""
+    return (_fns or _functions())["kv4_page_bytes"](page_size, heads, dim, group)
+
+
+def kv4_append(k: int, v: int, cache: Kv4Cache, table: int, table_width: int, lengths: int, batch: int, rows: int, *,
+               type: int = F32, freqs: int = 0, rotary: int = 0, pairs: bool = False, positions: int = 0, q: int = 0,
+               q_out: int = 0, heads: int = 0, starts: int = 0, q_stride: int = 0, q_out_stride: int = 0,
+               k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+    """`kv_append_rotated` into a cache in 4 bits, from rows of `type`."""
+    _call("kv4_append", q, q_stride, q_out, q_out_stride, heads, k, k_stride, v, v_stride, cache, table, table_width,
+          lengths, starts, positions, freqs, rotary, pairs, batch, rows, type, stream)
+
+
+def kv4_read(k: int, v: int, cache: Kv4Cache, table: int, table_width: int, lengths: int, batch: int, rows: int, *,
+             starts: int = 0, type: int = F32, k_stride: int = 0, v_stride: int = 0, stream: int = 0) -> None:
+    """The last tokens below each text's length, out of a cache in 4 bits, into `rows` rows of k and v."""
+    _call("kv4_read", k, k_stride, v, v_stride, cache, table, table_width, lengths, starts, batch, rows, type, stream)
+
+
+def kv4_attention_workspace(cache: Kv4Cache, batch: int, heads: int, longest: int = 0) -> int:
+    """Bytes of workspace with which `kv4_attention` splits as far as it would."""
+    return (_fns or _functions())["kv4_workspace"](cache, batch, heads, longest)
+
+
+def kv4_attention(q: int, cache: Kv4Cache, table: int, table_width: int, lengths: int, y: int, batch: int, heads: int,
+                  *, scale: float, type: int = F32, window: int = 0, sinks: int = 0, longest: int = 0,
+                  workspace: int = 0, workspace_bytes: int = 0, q_stride: int = 0, y_stride: int = 0,
+                  stream: int = 0) -> None:
+    """`paged_attention` over a cache in 4 bits, of queries of `type`."""
+    _call("kv4_attention", q, q_stride, cache, table, table_width, lengths, y, y_stride, batch, heads, type, scale,
+          window, sinks, longest, workspace, workspace_bytes, stream)
