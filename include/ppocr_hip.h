@@ -436,6 +436,59 @@ int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cach
                             size_t heads, int type, float scale, size_t window, size_t sinks, size_t longest,
                             void *workspace, size_t workspace_bytes, void *stream, char *err, size_t err_len);
 
+/* Beam search: the `keep` best continuations (up to 128) of each of `batch`
+ * texts' `beams` beams (up to 128) by `vocab` tokens (up to 2^24). With logits
+ * x of `type` (rows of beams, `stride` values apart; 0: vocab),
+ *   score(i, v) = scores[b][i] + log_softmax(x[b][i])[v],
+ * computed and ordered in 64 bits (sums of exponentials in 32), ties to the
+ * lower i, then the lower v; [batch][keep] scores, the best first, their beams'
+ * numbers `parents` and their `tokens`. A beam whose `ended` byte is not 0
+ * (`ended` NULL: none) goes on with the token `end` alone, its score as it is.
+ * `out_ended` (or NULL) says of each choice whether its beam had ended or its
+ * token is `end` (-1: none is). A score of -infinity or NaN, a row of -infinity
+ * alone or with an infinity or NaN has no continuation, nor has a logit of
+ * -infinity; where fewer than `keep` are left, score -infinity, token -1, ended 0
+ * and the parent min(place, beams - 1) follow. Outputs overlap no input.
+ * `workspace`: as many bytes as ppocr_hip_beam_select_workspace says (0 for
+ * sizes that are refused), 16-byte aligned, written and read within the call:
+ * calls that may overlap each need their own. */
+size_t ppocr_hip_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t keep);
+int ppocr_hip_beam_select(const void *logits, size_t stride, const float *scores, const uint8_t *ended,
+                          float *out_scores, int32_t *parents, int32_t *tokens, uint8_t *out_ended, int32_t end,
+                          size_t batch, size_t beams, size_t vocab, size_t keep, int type, void *workspace,
+                          size_t workspace_bytes, void *stream, char *err, size_t err_len);
+
+/* A state of each beam, `bytes` a row, rows as many bytes apart as the strides
+ * say (0: `bytes`): to[row] = from[the row's parent]; `to` overlaps nothing. */
+typedef struct ppocr_beam_state {
+  const void *from;
+  void *to;
+  size_t bytes, from_stride, to_stride;
+} ppocr_beam_state;
+
+/* Beam search: each beam goes on from its parent's state, in one pass over the
+ * layers' caches (`caches` or `caches4`, up to 4096, all with the same page
+ * table and page size) and up to 16 dense states (token histories, recurrent
+ * states). Row b * beams + i has the parent b * beams + parents[b][i] (itself,
+ * where that is no beam of its text). Of a page table [batch * beams][width] and
+ * `lengths` [batch * beams], equal among a text's beams:
+ * pages that are full are shared: the row takes its parent's entries; the page
+ * being written (lengths % page_size tokens of it) is copied to the row's spare
+ * page, spare[row], unless the row is its own parent; the row keeps its own
+ * entries after that. Then spare_out[row] is the page that the row gave up for
+ * it, else spare[row]. So tables and spares of two sets, in turn, need no
+ * allocator: each beam begins with pages of its own for all it may write, a
+ * spare one, and appends only to the page being written. table_out and
+ * spare_out overlap nothing. A copy has the page's tokens in use (in 4 bits up
+ * to the next multiple of four); if the parent's page does not exist, its
+ * number is taken over and nothing copied. More caches than 28 (9 in 4 bits)
+ * take more than one launch. */
+int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const ppocr_kv4_cache *caches4,
+                           size_t n_caches4, const ppocr_beam_state *states, size_t n_states, const int32_t *parents,
+                           const int32_t *table, int32_t *table_out, size_t table_width, const int32_t *lengths,
+                           const int32_t *spare, int32_t *spare_out, size_t batch, size_t beams, void *stream,
+                           char *err, size_t err_len);
+
 /* --- Host stages either side of the model ---------------------------------
  * CPU code in the same library: the recogniser's text from its [T][2]
  * output, and the detector's text boxes from its probability map. Each

@@ -1,0 +1,473 @@
+// Beam search: the choice of the best continuations over beams and vocabulary
+// (ppocr_hip_beam_select) and the reordering of caches and states after it
+// (ppocr_hip_beam_reorder).
+//
+//   score(i, v) = scores_i + (x_iv - max_i) - log(sum over v of exp(x_iv - max_i))
+//
+// Within a beam the order of scores is that of the logits, so one pass over
+// them gives each part of a row its largest value, its sum of exponentials and
+// its `keep` best; a workgroup a text then has the beams' logarithms and
+// chooses among the parts' best, in f64, so that scores of different beams that
+// differ at all are told apart. Numbers to be ordered carry their position in
+// their low bits, the lower one the larger: no two are equal, and the result
+// does not depend on the order in which workgroups or lanes come to them.
+#include <algorithm>
+
+#include "writer.hpp"
+
+namespace ppocr {
+namespace {
+
+// Floats and doubles as numbers that are ordered as they are.
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t u = __float_as_uint(v);
+  return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+  return __uint_as_float(u ^ (u >> 31 ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ uint64_t ordered(double v) {
+  const uint64_t u = (uint64_t)__double_as_longlong(v);
+  return u ^ (u >> 63 ? ~uint64_t(0) : uint64_t(1) << 63);
+}
+__device__ __forceinline__ double unordered(uint64_t u) {
+  return __longlong_as_double((long long)(u ^ (u >> 63 ? uint64_t(1) << 63 : ~uint64_t(0))));
+}
+
+__device__ __forceinline__ uint64_t shuffled(uint64_t v, int o) {
+  return (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), o) << 32 | (uint32_t)__shfl_xor((int)v, o);
+}
+
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504088896340736f); }
+
+// ---------------------------------------------------------------- a row's parts
+
+constexpr int kThreads = 256, kList = 512;
+
+// The `keep` largest of a workgroup's numbers: those past a bound that at least
+// `keep` are not below, which is the least of `keep` (or more) groups' largest,
+// gathered in LDS and ranked there. Of shuffled numbers that leaves a few times
+// `keep`; where more than LDS holds (sorted ones), the bound is halved in on.
+// R: rounds of 8 values a thread.
+template <int T, int R>
+__global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
+  typedef num_t<T> V;
+  __shared__ uint64_t list[kList];
+  __shared__ uint64_t lds_least[4], lds_most[4];
+  __shared__ float lds_f[4];
+  __shared__ int lds_n[4], lds_count;
+  const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+  // Beams that have no score to go on from, or have ended, need no logits.
+  if (!(a.scores[row] > -INFINITY) || (a.ended && a.ended[row])) return;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int begin = part * a.chunk, end = min(begin + a.chunk, a.vocab);
+  const V *p = (const V *)a.logits + row * a.stride;
+
+  V raw[R][8];
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int at = begin + (r * kThreads + (int)threadIdx.x) * 8;
+    if (at < end) load_n(p + at, end - at, raw[r]);
+  }
+  float x[R][8], top = -INFINITY;
+  uint32_t best = 0;
+  int best_at = 0;
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int at = begin + (r * kThreads + (int)threadIdx.x) * 8 + j;
+      x[r][j] = at < end ? Num<T>::get(raw[r][j]) + 0.0f : -INFINITY;  // (-0 is 0)
+      top = fmaxf(top, x[r][j]);
+      const uint32_t o = ordered(x[r][j]);
+      if (o > best) best = o, best_at = at;
+    }
+  const auto key_of = [&](int r, int j) {
+    return (uint64_t)ordered(x[r][j]) << 32 | ~(uint32_t)(begin + (r * kThreads + (int)threadIdx.x) * 8 + j);
+  };
+  // The largest, and the bound: the largest of each group of lanes, the least of those.
+  int groups = 4;
+  while (groups < a.keep) groups *= 2;
+  const int lanes = kThreads / groups;
+  uint64_t least = (uint64_t)best << 32 | ~(uint32_t)best_at, most = least;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const uint64_t other = shuffled(least, o);
+    least = (o < lanes) == (other > least) ? other : least;
+    const uint64_t more = shuffled(most, o);
+    most = more > most ? more : most;
+    top = fmaxf(top, __shfl_xor(top, o));
+  }
+  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most, lds_f[wave] = top;
+  if (threadIdx.x == 0) lds_count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    least = min(least, lds_least[w]), most = max(most, lds_most[w]);
+    top = fmaxf(top, lds_f[w]);
+  }
+  // Nothing of -infinity is chosen.
+  const uint64_t floor_ = (uint64_t)ordered(-INFINITY) << 32 | 0xffffffffu;
+  uint64_t bound = max(least, floor_ + 1);
+  const auto gather = [&] {
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const uint64_t k = key_of(r, j);
+        if (k >= bound) {
+          const int at = atomicAdd(&lds_count, 1);
+          if (at < kList) list[at] = k;
+        }
+      }
+  };
+  gather();
+
+  // The sum of exponentials.
+  const float from = top == -INFINITY ? 0.0f : top;
+  float sum = 0.0f;
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) sum += exp_of(x[r][j] - from);
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+  __syncthreads();  // the list is whole, lds_f read
+  if (lane == 0) lds_f[wave] = sum;
+
+  if (lds_count > kList) {  // (the same in all threads)
+    // count(low) > kList, count(high) < keep; numbers differ, so some bound
+    // between leaves between `keep` and kList of them.
+    uint64_t low = bound, high = most + 1;
+    while (true) {
+      const uint64_t mid = low + (high - low) / 2;
+      int n = 0;
+#pragma unroll
+      for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) n += __popcll(__ballot(key_of(r, j) >= mid));
+      __syncthreads();
+      if (lane == 0) lds_n[wave] = n;
+      __syncthreads();
+      n = lds_n[0] + lds_n[1] + lds_n[2] + lds_n[3];
+      bound = mid;
+      if (n > kList) {
+        low = mid;
+      } else if (n < a.keep && high - low > 1) {
+        high = mid;
+      } else {
+        break;
+      }
+      if (high - low <= 1) break;  // (never, as numbers differ; NaNs' do too)
+    }
+    if (threadIdx.x == 0) lds_count = 0;
+    __syncthreads();
+    gather();
+    __syncthreads();
+  }
+  const int n = min(lds_count, kList);
+  uint64_t *out = a.keys + (long)blockIdx.x * a.keep;
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += list[j] > mine;
+    if (rank < a.keep) out[rank] = mine;
+  }
+  for (int i = n + threadIdx.x; i < a.keep; i += kThreads) out[i] = 0;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    a.stats[2L * blockIdx.x] = top;
+    a.stats[2L * blockIdx.x + 1] = (lds_f[0] + lds_f[1]) + (lds_f[2] + lds_f[3]);
+  }
+}
+
+// ------------------------------------------------------- a text's choice
+
+constexpr int kChoices = 2048;
+
+// A candidate: its score, ordered, and its position among beams x vocabulary,
+// the lower one the larger. 0, 0: none.
+struct Choice {
+  uint64_t score, at;
+  __device__ __forceinline__ bool operator>(const Choice &o) const {
+    return score > o.score || (score == o.score && at > o.at);
+  }
+};
+
+// A workgroup a text. `groups`: at least `keep`, of at most 64 neighbouring threads.
+__global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int groups, Divide by_each) {
+  __shared__ Choice list[kChoices];
+  __shared__ double lds_base[kMostBeams], lds_top[kMostBeams], lds_log[kMostBeams];
+  __shared__ Choice lds_least[16], lds_most[16];
+  __shared__ int lds_live[kMostBeams], lds_n[16], lds_count;  // live: 0 no candidates, 1 its tokens, 2 ended
+  const int b = blockIdx.x, threads = blockDim.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = threads / 64;
+  const int each = a.parts * a.keep;
+  for (int i = wave; i < a.beams; i += waves) {
+    const long row = (long)b * a.beams + i;
+    const float base = a.scores[row];
+    int live = !(base > -INFINITY) ? 0 : a.ended && a.ended[row] ? 2 : 1;
+    float top = -INFINITY;
+    double sum = 0;
+    if (live == 1) {
+      for (int k = lane; k < a.parts; k += 64) top = fmaxf(top, a.stats[2 * (row * a.parts + k)]);
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+      for (int k = lane; k < a.parts; k += 64) {
+        const float t = a.stats[2 * (row * a.parts + k)], s = a.stats[2 * (row * a.parts + k) + 1];
+        sum += t == -INFINITY ? (double)s : (double)s * exp((double)t - (double)top);
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) sum += __longlong_as_double((long long)shuffled((uint64_t)__double_as_longlong(sum), o));
+      // (Not so for a row of -infinity, or with an infinity or a NaN.)
+      if (!(sum > 0) || !(top < INFINITY)) live = 0;
+    }
+    if (lane == 0) {
+      lds_base[i] = (double)base, lds_top[i] = (double)top, lds_log[i] = live == 1 ? log(sum) : 0;
+      lds_live[i] = live;
+    }
+  }
+  if (threadIdx.x == 0) lds_count = 0;
+  __syncthreads();
+  const int all = a.beams * each;  // (at most 2^25)
+  auto choice = [&](int c) -> Choice {
+    if (c >= all) {
+      const int i = c - all;
+      return lds_live[i] == 2 ? Choice{ordered(lds_base[i] + 0.0), ~((uint64_t)i * a.vocab + a.end)} : Choice{0, 0};
+    }
+    const int i = by_each(c);
+    if (lds_live[i] != 1) return Choice{0, 0};
+    const uint64_t key = a.keys[(long)b * all + c];
+    if (key == 0) return Choice{0, 0};
+    const double x = (double)unordered((uint32_t)(key >> 32));
+    const double score = lds_base[i] + ((x - lds_top[i]) - lds_log[i]);
+    if (!(score > -INFINITY)) return Choice{0, 0};
+    return Choice{ordered(score + 0.0), ~((uint64_t)i * a.vocab + (uint32_t)~(uint32_t)key)};
+  };
+  const int count = all + a.beams;
+  Choice least{0, 0};
+  for (int c = threadIdx.x; c < count; c += threads) {
+    const Choice k = choice(c);
+    if (k > least) least = k;
+  }
+  Choice most = least;
+  const int lanes = threads / groups;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const Choice other{shuffled(least.score, o), shuffled(least.at, o)};
+    if (o < lanes ? other > least : least > other) least = other;
+    const Choice more{shuffled(most.score, o), shuffled(most.at, o)};
+    if (more > most) most = more;
+  }
+  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most;
+  __syncthreads();
+  for (int w = 0; w < waves; w++) {
+    if (least > lds_least[w]) least = lds_least[w];
+    if (lds_most[w] > most) most = lds_most[w];
+  }
+  if (least.score == 0) least = Choice{0, 1};  // none is not chosen
+  auto gather = [&] {
+    for (int c = threadIdx.x; c < count; c += threads) {
+      const Choice k = choice(c);
+      if (!(least > k)) {
+        const int at = atomicAdd(&lds_count, 1);
+        if (at < kChoices) list[at] = k;
+      }
+    }
+  };
+  gather();
+  __syncthreads();
+  if (lds_count > kChoices) {  // (the same in all threads)
+    auto count_from = [&](const Choice &bound) {
+      int n = 0;
+      for (int c = threadIdx.x; c < count; c += threads) n += !(bound > choice(c));
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) n += __shfl_xor(n, o);
+      __syncthreads();
+      if (lane == 0) lds_n[wave] = n;
+      __syncthreads();
+      n = 0;
+      for (int w = 0; w < waves; w++) n += lds_n[w];
+      return n;
+    };
+    // First by scores alone, then, where too many share one, by positions.
+    uint64_t low = least.score, high = most.score + 1;
+    bool done = false;
+    while (high - low > 1) {
+      const uint64_t mid = low + (high - low) / 2;
+      const int n = count_from(Choice{mid, 0});
+      if (n > kChoices) {
+        low = mid;
+      } else if (n < a.keep) {
+        high = mid;
+      } else {
+        least = Choice{mid, 0}, done = true;
+        break;
+      }
+    }
+    if (!done) {
+      const uint64_t score = low;
+      uint64_t below = 0, above = ~uint64_t(0);
+      while (above - below > 1) {
+        const uint64_t mid = below + (above - below) / 2;
+        const int n = count_from(Choice{score, mid});
+        if (n > kChoices) {
+          below = mid;
+        } else if (n < a.keep) {
+          above = mid;
+        } else {
+          below = mid;
+          break;
+        }
+      }
+      least = Choice{score, below};
+    }
+    if (threadIdx.x == 0) lds_count = 0;
+    __syncthreads();
+    gather();
+    __syncthreads();
+  }
+  const int n = min(lds_count, kChoices);
+  const long out = (long)b * a.keep;
+  for (int i = threadIdx.x; i < n; i += threads) {
+    const Choice mine = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; j++) rank += list[j] > mine;
+    if (rank >= a.keep) continue;
+    const uint64_t at = ~mine.at;
+    const int parent = (int)(at / a.vocab), token = (int)(at - (uint64_t)parent * a.vocab);
+    a.out_scores[out + rank] = (float)unordered(mine.score);
+    a.parents[out + rank] = parent;
+    a.tokens[out + rank] = token;
+    if (a.out_ended) a.out_ended[out + rank] = token == a.end || lds_live[parent] == 2;
+  }
+  for (int i = n + threadIdx.x; i < a.keep; i += threads) {
+    a.out_scores[out + i] = -INFINITY;
+    a.parents[out + i] = min(i, a.beams - 1);
+    a.tokens[out + i] = -1;
+    if (a.out_ended) a.out_ended[out + i] = 0;
+  }
+}
+
+template <int T>
+hipError_t launch_parts_of(const SelectArgs &a, hipStream_t s) {
+  const dim3 grid(unsigned((long)a.batch * a.beams * a.parts)), block(kThreads);
+  if (a.chunk <= kThreads * 8) return launch_kernel(beam_parts<T, 1>, grid, block, 0, s, a);
+  if (a.chunk <= kThreads * 16) return launch_kernel(beam_parts<T, 2>, grid, block, 0, s, a);
+  return launch_kernel(beam_parts<T, 4>, grid, block, 0, s, a);
+}
+
+// -------------------------------------------------------------- the reordering
+
+__device__ __forceinline__ v4u piece_at(const char *p, long i) {
+  v4u v;
+  __builtin_memcpy(&v, p + 16 * i, 16);
+  return v;
+}
+__device__ __forceinline__ void put_piece(char *p, long i, v4u v) { __builtin_memcpy(p + 16 * i, &v, 16); }
+
+// Copies `bytes` from one place to another, a thread's share: from piece of 16
+// `first` on every `step`-th.
+__device__ __forceinline__ void copy_pieces(char *to, const char *from, long bytes, long first, long step) {
+  const long whole = bytes / 16;
+  long i = first;
+  for (; i + 3 * step < whole; i += 4 * step) {
+    const v4u a = piece_at(from, i), b = piece_at(from, i + step), c = piece_at(from, i + 2 * step),
+              d = piece_at(from, i + 3 * step);
+    put_piece(to, i, a);
+    put_piece(to, i + step, b);
+    put_piece(to, i + 2 * step, c);
+    put_piece(to, i + 3 * step, d);
+  }
+  for (; i < whole; i += step) put_piece(to, i, piece_at(from, i));
+  for (long k = 16 * whole + first; k < bytes; k += step) to[k] = from[k];
+}
+
+// Row (a text's beam) blockIdx.y; workgroup 0 of it has its table, the next ones
+// the states, the others a split of a plane's tokens each. Memory bound, or by
+// the launch.
+__global__ __launch_bounds__(256) void beam_reorder_rows(ReorderArgs a) {
+  const int row = blockIdx.y, text = a.by_beams(row);
+  const int parent = a.parents[row];
+  const int from = parent < 0 || parent >= a.beams ? row : text * a.beams + parent;
+  int job = blockIdx.x;
+  const int of_states = a.n_states * a.state_splits;
+  if (a.tables && job > 0 && job <= of_states) {
+    const int state = (job - 1) / a.state_splits, split = job - 1 - state * a.state_splits;
+    const BeamState &s = a.states[state];
+    copy_pieces(s.to + row * s.to_stride, s.from + from * s.from_stride, s.bytes, split * 256 + threadIdx.x,
+                a.state_splits * 256);
+    return;
+  }
+  if (!a.table) return;
+  const int length = max(a.lengths[from], 0), full = a.by_page(length), part = length - full * a.by_page.d;
+  const int *mine = a.table + row * a.table_width, *other = a.table + from * a.table_width;
+  // The page being written is copied where the row has another parent.
+  const bool moved = from != row;
+  int source = -1, into = -1;
+  if (moved && part > 0 && full < a.table_width) source = other[full], into = a.spare[row];
+  const bool there = source >= 0 && source < a.pages, copied = there && into >= 0 && into < a.pages;
+  if (a.tables) {
+    if (job == 0) {
+      for (long i = threadIdx.x; i < a.table_width; i += 256)
+        a.table_out[row * a.table_width + i] = !moved || i > full || (i == full && part == 0) ? mine[i]
+                                               : i < full                                     ? other[i]
+                                               : there                                        ? into
+                                                                                              : source;
+      if (threadIdx.x == 0) a.spare_out[row] = there ? mine[full] : a.spare[row];
+      return;
+    }
+    job -= 1 + of_states;
+  }
+  if (!copied) return;
+  const int plane = job / a.splits, split = job - plane * a.splits;
+  const Plane &p = a.planes[plane];
+  const char *src = p.base + source * p.page_stride;
+  char *dst = p.base + into * p.page_stride;
+  const int tokens = a.whole4 ? min((part + 3) / 4 * 4, a.by_page.d) : part;
+  if (p.token_stride == p.bytes) {
+    for (int h = 0; h < p.heads; h++)
+      copy_pieces(dst + h * p.head_stride, src + h * p.head_stride, (long)tokens * p.bytes, split * 256 + threadIdx.x,
+                  a.splits * 256);
+  } else {
+    // A row of a head a wave at a time.
+    const int lane = threadIdx.x % 64;
+    for (int i = split * 4 + threadIdx.x / 64; i < tokens * p.heads; i += a.splits * 4) {
+      const int token = i / p.heads, h = i - token * p.heads;
+      const long at = token * p.token_stride + h * p.head_stride;
+      copy_pieces(dst + at, src + at, p.bytes, lane, 64);
+    }
+  }
+}
+
+}  // namespace
+
+SelectParts select_parts(long rows, int vocab) {
+  // Parts of 2048 to 8192 values (8 to 32 a thread), as large as still gives the
+  // card 2048 workgroups; all about as long.
+  const long least = (vocab + 8191L) / 8192, most = (vocab + 2047L) / 2048;
+  const long parts = std::min(std::max((2048 + rows - 1) / rows, least), most);
+  const int chunk = int(((vocab + parts - 1) / parts + 7) / 8 * 8);
+  return {(vocab + chunk - 1) / chunk, chunk};
+}
+
+hipError_t launch_beam_select(const SelectArgs &a, int type, hipStream_t s) {
+  const hipError_t e = type == PPOCR_F32    ? launch_parts_of<PPOCR_F32>(a, s)
+                       : type == PPOCR_BF16 ? launch_parts_of<PPOCR_BF16>(a, s)
+                       : type == PPOCR_F16  ? launch_parts_of<PPOCR_F16>(a, s)
+                                            : hipErrorInvalidValue;
+  if (e != hipSuccess) return e;
+  // Four candidates or more a thread, and a group of threads at least for each kept.
+  int threads = 64, groups = 1;
+  while (groups < a.keep) groups *= 2;
+  while (threads < 1024 && (threads < groups || 4L * threads * 2 <= (long)a.beams * a.parts * a.keep)) threads *= 2;
+  groups = std::max(groups, threads / 64);
+  return launch_kernel(beam_choice, dim3(a.batch), dim3(threads), 0, s, a, groups,
+                       Divide(a.parts * a.keep));
+}
+
+hipError_t launch_beam_reorder(const ReorderArgs &a, hipStream_t s) {
+  const dim3 grid((a.tables ? 1 + a.n_states * a.state_splits : 0) + a.n_planes * a.splits, a.rows), block(256);
+  return launch_kernel(beam_reorder_rows, grid, block, 0, s, a);
+}
+
+}  // namespace ppocr

@@ -79,6 +79,14 @@ int turn_of(const Fail &fail, const char *what, const void *q, size_t q_stride, 
   return 0;
 }
 
+bool select_sizes(size_t batch, size_t beams, size_t vocab, size_t keep) {
+  if (!batch || batch > 65535 || !beams || beams > kMostBeams || !vocab || vocab > size_t(1) << 24 || !keep ||
+      keep > kMostKeep)
+    return false;
+  const long rows = long(batch * beams);
+  return rows * select_parts(rows, int(vocab)).parts < 1 << 24;
+}
+
 }  // namespace
 
 extern "C" {
@@ -200,6 +208,147 @@ int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cach
   if (on.e != hipSuccess) return fail.hip(what, on.e);
   return fail.hip(what, type == PPOCR_F32 ? launch_kv4_attention_32(a, hipStream_t(stream))
                                           : launch_kv4_attention_16(a, hipStream_t(stream)));
+}
+
+size_t ppocr_hip_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t keep) {
+  if (!select_sizes(batch, beams, vocab, keep)) return 0;
+  const long rows = long(batch * beams);
+  return size_t(rows) * select_parts(rows, int(vocab)).parts * (keep + 1) * 8;
+}
+
+int ppocr_hip_beam_select(const void *logits, size_t stride, const float *scores, const uint8_t *ended,
+                          float *out_scores, int32_t *parents, int32_t *tokens, uint8_t *out_ended, int32_t end,
+                          size_t batch, size_t beams, size_t vocab, size_t keep, int type, void *workspace,
+                          size_t workspace_bytes, void *stream, char *err, size_t err_len) {
+  const Fail fail{err, err_len};
+  const char *what = "beam selection";
+  if (!is_real(type)) return fail("%s: type %d", what, type);
+  if (batch == 0) return 0;
+  if (!select_sizes(batch, beams, vocab, keep))
+    return fail("%s: %zu of %zu beams of %zu texts and %zu tokens (up to %d beams, %d kept, 2^24 tokens and 2^24 parts "
+                "of rows are taken)", what, keep, beams, batch, vocab, kMostBeams, kMostKeep);
+  if (!logits || !scores || !out_scores || !parents || !tokens)
+    return fail("%s: logits, scores, out_scores, parents and tokens are needed", what);
+  if (!aligned(logits, size_of(type)) || !aligned(scores, 4) || !aligned(out_scores, 4) || !aligned(parents, 4) ||
+      !aligned(tokens, 4) || !aligned(workspace, 16))
+    return fail("%s: a pointer is not aligned", what);
+  if (end < -1 || (end >= 0 && size_t(end) >= vocab) || (ended && end < 0))
+    return fail("%s: end token %d of %zu%s", what, int(end), vocab, ended ? ", and beams that have ended need one" : "");
+  SelectArgs a{};
+  if (!stride_of(stride, vocab, &a.stride)) return fail("%s: stride %zu for %zu tokens", what, stride, vocab);
+  const size_t need = ppocr_hip_beam_select_workspace(batch, beams, vocab, keep);
+  if (!workspace || workspace_bytes < need)
+    return fail("%s: a workspace of %zu bytes is needed, not %zu", what, need, workspace ? workspace_bytes : 0);
+  a.logits = logits, a.scores = scores, a.ended = ended, a.out_scores = out_scores;
+  a.parents = parents, a.tokens = tokens, a.out_ended = out_ended, a.end = int(end);
+  a.batch = int(batch), a.beams = int(beams), a.vocab = int(vocab), a.keep = int(keep);
+  const SelectParts parts = select_parts(long(batch * beams), a.vocab);
+  a.parts = parts.parts, a.chunk = parts.chunk;
+  a.keys = static_cast<uint64_t *>(workspace);
+  a.stats = reinterpret_cast<float *>(a.keys + batch * beams * size_t(a.parts) * keep);
+  const OnDevice on{hipStream_t(stream)};
+  if (on.e != hipSuccess) return fail.hip(what, on.e);
+  return fail.hip(what, launch_beam_select(a, type, hipStream_t(stream)));
+}
+
+int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const ppocr_kv4_cache *caches4,
+                           size_t n_caches4, const ppocr_beam_state *states, size_t n_states, const int32_t *parents,
+                           const int32_t *table, int32_t *table_out, size_t table_width, const int32_t *lengths,
+                           const int32_t *spare, int32_t *spare_out, size_t batch, size_t beams, void *stream,
+                           char *err, size_t err_len) {
+  const Fail fail{err, err_len};
+  const char *what = "beam reordering";
+  if ((n_caches && !caches) || (n_caches4 && !caches4) || (n_states && !states))
+    return fail("%s: a list is missing", what);
+  if (n_caches && n_caches4) return fail("%s: caches of one kind are taken, not %zu and %zu", what, n_caches, n_caches4);
+  if (n_states > kMostStates || n_caches > 4096 || n_caches4 > 4096)
+    return fail("%s: %zu states, %zu caches: %d and 4096 are taken", what, n_states, n_caches + n_caches4, kMostStates);
+  if (batch == 0) return 0;
+  if (!beams || beams > kMost || batch > 65535 || batch * beams > 65535)
+    return fail("%s: %zu texts of %zu beams: up to 65535 beams in all are taken", what, batch, beams);
+  if (!parents || !aligned(parents, 4)) return fail("%s: parents are needed, aligned to their type", what);
+  ReorderArgs a{};
+  a.rows = int(batch * beams), a.beams = int(beams), a.by_beams = Divide(a.beams), a.parents = parents;
+  const bool paged = n_caches || n_caches4;
+  size_t page_size = 0;
+  // Each cache's planes, twice: counted and checked, then launched.
+  Plane planes[6];
+  auto planes_of = [&](size_t i, int &n) -> int {
+    n = 0;
+    if (n_caches4) {
+      Kv4Args c{};
+      if (const int rc = kv4_of(fail, what, caches4 + i, table, table_width, lengths, c)) return rc;
+      const int at[6] = {0, c.at_ks, c.at_km, c.at_v, c.at_vs, c.at_vm};
+      for (int k = 0; k < 6; k++) {
+        const int bytes = k % 3 ? 2 * c.groups : 16 * c.nc;
+        planes[n++] = Plane{c.data + at[k], c.page_stride, bytes, c.chunk, c.heads, bytes};
+      }
+      a.pages = i && a.pages < c.pages ? a.pages : c.pages;
+      if (i && page_size != size_t(c.page_size)) return fail("%s: caches of pages of %zu and %d tokens", what, page_size, c.page_size);
+      page_size = size_t(c.page_size);
+    } else {
+      CacheArgs c{};
+      if (const int rc = cache_of(fail, what, caches + i, table, table_width, lengths, c)) return rc;
+      const long size = long(size_of(caches[i].type));
+      const bool rows = c.head_stride == c.dim && c.token_stride == long(c.heads) * c.dim;
+      for (void *p : {c.k, c.v})
+        planes[n++] = rows ? Plane{static_cast<char *>(p), c.page_stride * size, c.token_stride * size, 0, 1,
+                                   int(c.token_stride * size)}
+                           : Plane{static_cast<char *>(p), c.page_stride * size, c.token_stride * size,
+                                   c.head_stride * size, c.heads, int(c.dim * size)};
+      a.pages = i && a.pages < c.pages ? a.pages : c.pages;
+      if (i && page_size != size_t(c.page_size)) return fail("%s: caches of pages of %zu and %d tokens", what, page_size, c.page_size);
+      page_size = size_t(c.page_size);
+    }
+    return 0;
+  };
+  const size_t count = n_caches + n_caches4;
+  for (size_t i = 0; i < count; i++) {
+    int n;
+    if (const int rc = planes_of(i, n)) return rc;
+  }
+  if (paged) {
+    if (!table_out || !spare || !spare_out || table_out == table || spare_out == spare)
+      return fail("%s: table_out, spare and spare_out are needed, apart from table and spare", what);
+    if (!aligned(table_out, 4) || !aligned(spare, 4) || !aligned(spare_out, 4))
+      return fail("%s: a pointer is not aligned to its type", what);
+    a.table = table, a.table_out = table_out, a.table_width = long(table_width);
+    a.lengths = lengths, a.spare = spare, a.spare_out = spare_out;
+    a.by_page = Divide(int(page_size)), a.whole4 = n_caches4 != 0;
+  }
+  for (size_t i = 0; i < n_states; i++) {
+    const ppocr_beam_state &s = states[i];
+    if (!s.from || !s.to || s.from == s.to) return fail("%s: state %zu needs from and to, apart", what, i);
+    const size_t from_stride = s.from_stride ? s.from_stride : s.bytes, to_stride = s.to_stride ? s.to_stride : s.bytes;
+    if (s.bytes > kMostStride || from_stride < s.bytes || to_stride < s.bytes || from_stride > kMostStride ||
+        to_stride > kMostStride)
+      return fail("%s: state %zu of %zu bytes with strides %zu, %zu", what, i, s.bytes, s.from_stride, s.to_stride);
+    a.states[i] = BeamState{static_cast<const char *>(s.from), static_cast<char *>(s.to), long(s.bytes),
+                            long(from_stride), long(to_stride)};
+  }
+  a.n_states = int(n_states);
+  size_t most = 0;
+  for (size_t i = 0; i < n_states; i++) most = states[i].bytes > most ? states[i].bytes : most;
+  a.state_splits = most < 65536 ? 1 : most < 1 << 20 ? int(most >> 15) : 32;
+  if (!paged && !n_states) return 0;
+  const OnDevice on{hipStream_t(stream)};
+  if (on.e != hipSuccess) return fail.hip(what, on.e);
+  // As many planes a launch as its arguments hold; the tables and states in the first.
+  const int a_cache = n_caches4 ? 6 : 2;
+  size_t i = 0;
+  do {
+    a.tables = i == 0, a.n_planes = 0;
+    for (; i < count && a.n_planes + a_cache <= kMostPlanes; i++) {
+      int n;
+      if (const int rc = planes_of(i, n)) return rc;
+      for (int k = 0; k < n; k++) a.planes[a.n_planes++] = planes[k];
+    }
+    // A plane's tokens in parts while there are few rows and planes.
+    const long work = long(a.n_planes) * a.rows;
+    a.splits = work >= 1024 || !work ? 1 : work >= 512 ? 2 : work >= 256 ? 4 : 8;
+    if (const int rc = fail.hip(what, launch_beam_reorder(a, hipStream_t(stream)))) return rc;
+  } while (i < count);
+  return 0;
 }
 
 }  // extern "C"

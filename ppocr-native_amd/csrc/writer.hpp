@@ -80,4 +80,53 @@ hipError_t launch_kv4_attention_16(const Attend4Args &a, hipStream_t s);
 hipError_t launch_kv4_attention_32(const Attend4Args &a, hipStream_t s);
 hipError_t launch_kv4_join(const Attend4Args &a, hipStream_t s);
 
+// Beam search: the choice over beams and vocabulary.
+constexpr int kMostBeams = 128, kMostKeep = 128;
+struct SelectArgs {
+  const void *logits;
+  long stride;
+  const float *scores;
+  const uint8_t *ended;  // NULL: none
+  float *out_scores;
+  int *parents, *tokens;
+  uint8_t *out_ended;  // NULL: not wanted
+  int end;             // -1: none
+  int batch, beams, vocab, keep;
+  int parts, chunk;  // of a row: chunk values a part
+  uint64_t *keys;    // [row][part][keep]: a part's best, the best first, 0 past the last
+  float *stats;      // [row][part]: largest, sum of exponentials
+};
+struct SelectParts {
+  int parts, chunk;
+};
+SelectParts select_parts(long rows, int vocab);
+hipError_t launch_beam_select(const SelectArgs &a, int type, hipStream_t s);
+
+// Beam search: the reordering of caches and states. A plane is part of a cache
+// whose tokens have `bytes` each a head.
+struct Plane {
+  char *base;
+  long page_stride, token_stride, head_stride;  // bytes
+  int heads, bytes;
+};
+struct BeamState {
+  const char *from;
+  char *to;
+  long bytes, from_stride, to_stride;
+};
+constexpr int kMostPlanes = 56, kMostStates = 16;
+struct ReorderArgs {
+  Plane planes[kMostPlanes];
+  BeamState states[kMostStates];
+  int n_planes, n_states, splits, state_splits;  // splits: workgroups a plane (a state) and row
+  int tables;                      // whether this launch has the tables
+  int whole4;                      // tokens are copied by fours
+  const int *parents, *table, *lengths, *spare;
+  int *table_out, *spare_out;
+  long table_width;
+  int rows, beams, pages;
+  Divide by_page, by_beams;
+};
+hipError_t launch_beam_reorder(const ReorderArgs &a, hipStream_t s);
+
 }  // namespace ppocr

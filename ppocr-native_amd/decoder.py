@@ -1,8 +1,9 @@
 """The layers of a text decoder on device memory, over the C ABI
 (ppocr_hip_rms_norm, ppocr_hip_q4_product, ppocr_hip_kv_append,
 ppocr_hip_paged_attention, ppocr_hip_window_attention, the append with the
-rotation of positions, the cache in 4 bits ppocr_hip_kv4_*): what a program
-calls that writes or corrects text token by token after the recogniser.
+rotation of positions, the cache in 4 bits ppocr_hip_kv4_*, beam search
+ppocr_hip_beam_*): what a program calls that writes or corrects text token by
+token after the recogniser.
 
 Arguments are device addresses (integers; 0 = none), sizes, strides in values
 (0 = rows without a gap) and a HIP stream (0 = the default stream); see
@@ -61,6 +62,17 @@ class Kv4Cache(C.Structure):
         super().__init__(data, pages, page_size, heads, dim, group, page_stride)
 
 
+class BeamState(C.Structure):
+    """A dense state of each beam (`ppocr_beam_state`): rows of `bytes`, at
+    addresses `from_` and `to`, strides in bytes (0: `bytes`)."""
+
+    _fields_ = [("from_", C.c_void_p), ("to", C.c_void_p), ("bytes", C.c_size_t), ("from_stride", C.c_size_t),
+                ("to_stride", C.c_size_t)]
+
+    def __init__(self, from_: int, to: int, bytes: int, from_stride: int = 0, to_stride: int = 0):
+        super().__init__(from_, to, bytes, from_stride, to_stride)
+
+
 def _functions() -> dict:
     if not _fns:
         L, fns = lib(), {}
@@ -75,6 +87,8 @@ def _functions() -> dict:
             "kv_append_rotated": [p, n, p, n, n, p, n, p, n, cache, p, n, p, p, p, p, n, i, n, n] + end,
             "kv4_append": [p, n, p, n, n, p, n, p, n, cache4, p, n, p, p, p, p, n, i, n, n, i] + end,
             "kv4_read": [p, n, p, n, cache4, p, n, p, p, n, n, i] + end,
+            "beam_select": [p, n, p, p, p, p, p, p, C.c_int32, n, n, n, n, i, p, n] + end,
+            "beam_reorder": [p, n, p, n, p, n, p, p, p, n, p, p, p, n, n] + end,
             "kv4_attention": [p, n, cache4, p, n, p, p, n, n, n, i, f, n, n, n, p, n] + end,
         }.items():
             fn = getattr(L, "ppocr_hip_" + name)
@@ -89,6 +103,9 @@ def _functions() -> dict:
         fn = L.ppocr_hip_kv4_page_bytes
         fn.argtypes, fn.restype = [n, n, n, n], n
         fns["kv4_page_bytes"] = fn
+        fn = L.ppocr_hip_beam_select_workspace
+        fn.argtypes, fn.restype = [n, n, n, n], n
+        fns["select_workspace"] = fn
         fn = L.ppocr_hip_q4_product_tiles
         fn.argtypes, fn.restype = [n, n, n, i], n
         fns["tiles"] = fn
@@ -198,3 +215,33 @@ def kv4_attention(q: int, cache: Kv4Cache, table: int, table_width: int, lengths
     """`paged_attention` over a cache in 4 bits, of queries of `type`."""
     _call("kv4_attention", q, q_stride, cache, table, table_width, lengths, y, y_stride, batch, heads, type, scale,
           window, sinks, longest, workspace, workspace_bytes, stream)
+
+
+def beam_select_workspace(batch: int, beams: int, vocab: int, keep: int) -> int:
+    """Bytes of workspace that `beam_select` needs (0 for sizes that are refused)."""
+    return (_fns or _functions())["select_workspace"](batch, beams, vocab, keep)
+
+
+def beam_select(logits: int, scores: int, out_scores: int, parents: int, tokens: int, batch: int, beams: int,
+                vocab: int, keep: int, *, workspace: int, workspace_bytes: int, type: int = F32, ended: int = 0,
+                out_ended: int = 0, end: int = -1, stride: int = 0, stream: int = 0) -> None:
+    """The `keep` best continuations of each text's beams by one of `vocab`
+    tokens, scores[i] + log_softmax(logits[i])[v], the best first."""
+    _call("beam_select", logits, stride, scores, ended, out_scores, parents, tokens, out_ended, end, batch, beams, vocab,
+          keep, type, workspace, workspace_bytes, stream)
+
+
+def _array(of, items):
+    return items if isinstance(items, C.Array) else (of * len(items))(*items)
+
+
+def beam_reorder(caches, parents: int, table: int, table_out: int, table_width: int, lengths: int, spare: int,
+                 spare_out: int, batch: int, beams: int, *, states=(), stream: int = 0) -> None:
+    """Each beam goes on from its parent's state: `caches` (KvCache or Kv4Cache,
+    a sequence or a ctypes array of them) with their page table, and dense
+    `states` (BeamState)."""
+    n = len(caches)
+    four = n and isinstance(caches[0], Kv4Cache)
+    held, dense = _array(Kv4Cache if four else KvCache, caches) if n else None, _array(BeamState, states) if len(states) else None
+    _call("beam_reorder", None if four else held, 0 if four else n, held if four else None, n if four else 0, dense,
+          len(states), parents, table, table_out, table_width, lengths, spare, spare_out, batch, beams, stream)

@@ -99,3 +99,83 @@ def test_workspace4():
     assert n > 0 and n % (32 * 130 * 4) == 0
     assert D.kv4_attention_workspace(c, 4096, 32, 16384) == 0  # enough texts
     assert D.kv4_attention_workspace(c, 1, 33, 16384) == 0 and D.kv4_attention_workspace(None, 1, 1, 1) == 0
+
+
+# ------------------------------------------------------------------ beam search
+
+def select(**k):
+    a = dict(logits=A, scores=A, out_scores=A, parents=A, tokens=A, batch=2, beams=4, vocab=1000, keep=4, type=D.F16,
+             workspace=A, workspace_bytes=1 << 20)
+    a.update(k)
+    D.beam_select(**a)
+
+
+def reorder(caches=(cache(),), states=(), **k):
+    a = dict(parents=A, table=A, table_out=A + 64, table_width=4, lengths=A, spare=A, spare_out=A + 64, batch=2, beams=3)
+    a.update(k)
+    D.beam_reorder(list(caches), states=list(states), **a)
+
+
+@pytest.mark.parametrize("call,args,reason", [
+    (select, dict(type=D.E4M3), "type 3"),
+    (select, dict(beams=0), "of 0 beams"),
+    (select, dict(beams=129), "of 129 beams"),
+    (select, dict(keep=0), "0 of 4 beams"),
+    (select, dict(keep=129), "129 of 4"),
+    (select, dict(vocab=0), "0 tokens"),
+    (select, dict(vocab=(1 << 24) + 1), "tokens"),
+    (select, dict(batch=70000), "70000 texts"),
+    (select, dict(batch=60000, beams=128, vocab=1 << 20), "parts"),
+    (select, dict(logits=0), "needed"),
+    (select, dict(scores=0), "needed"),
+    (select, dict(parents=0), "needed"),
+    (select, dict(logits=A + 1), "aligned"),
+    (select, dict(tokens=A + 2), "aligned"),
+    (select, dict(workspace=A + 8), "aligned"),
+    (select, dict(stride=999), "stride 999"),
+    (select, dict(end=1000), "end token 1000 of 1000"),
+    (select, dict(end=-2), "end token -2"),
+    (select, dict(ended=A), "have ended need one"),
+    (select, dict(workspace=0), "workspace of"),
+    (select, dict(workspace_bytes=100), "not 100"),
+    (reorder, dict(beams=0), "0 beams"),
+    (reorder, dict(batch=30000), "30000 texts"),
+    (reorder, dict(parents=0), "parents"),
+    (reorder, dict(parents=A + 2), "parents"),
+    (reorder, dict(table=0), "page table"),
+    (reorder, dict(table_out=0), "needed"),
+    (reorder, dict(table_out=A), "apart"),
+    (reorder, dict(spare=0), "needed"),
+    (reorder, dict(spare_out=A), "apart"),
+    (reorder, dict(spare_out=A + 66), "aligned"),
+    (reorder, dict(lengths=0), "lengths"),
+    (reorder, dict(caches=[cache(), cache(page_size=32)]), "pages of 16 and 32"),
+    (reorder, dict(caches=[cache(dim=300)]), "300"),
+    (reorder, dict(caches=[cache4(dim=300)]), "300"),
+    (reorder, dict(caches=[cache4(), cache4(page_size=32)]), "pages of 16 and 32"),
+    (reorder, dict(states=[D.BeamState(0, A, 4)]), "state 0"),
+    (reorder, dict(states=[D.BeamState(A, A, 4)]), "apart"),
+    (reorder, dict(states=[D.BeamState(A, A + 64, 8), D.BeamState(A, A + 64, 8, 4)]), "state 1 of 8 bytes"),
+    (reorder, dict(states=[D.BeamState(A, A + 64, 8)] * 17), "17 states"),
+])
+def test_beams_refused(call, args, reason):
+    with pytest.raises(GpuError, match=reason):
+        call(**args)
+
+
+def test_beams_nothing_to_do():
+    select(batch=0)
+    reorder(batch=0)
+    reorder(caches=[])
+    with pytest.raises(GpuError, match="handle"):
+        select(stream=1)
+    with pytest.raises(GpuError, match="handle"):
+        reorder(stream=1)
+
+
+def test_select_workspace():
+    # For each part of a row, its best and two floats; parts of 2048 to 8192 tokens.
+    assert D.beam_select_workspace(1, 4, 1000, 4) == 4 * 5 * 8
+    n = D.beam_select_workspace(32, 8, 131072, 8)
+    assert n % (256 * 9 * 8) == 0 and 16 <= n // (256 * 9 * 8) <= 64
+    assert D.beam_select_workspace(1, 129, 100, 4) == 0 and D.beam_select_workspace(1, 1, 100, 0) == 0
