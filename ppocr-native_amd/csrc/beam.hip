@@ -42,20 +42,29 @@ __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f
 
 // ---------------------------------------------------------------- a row's parts
 
-constexpr int kThreads = 256, kList = 512;
+constexpr int kThreads = 256, kList = 1024;
+
+// Lanes of a group, of `used` threads that have values: as many as leave `keep`
+// groups, up to a wave.
+__host__ __device__ inline int lanes_of(int used, int keep) {
+  int lanes = 64;
+  while (lanes > 1 && used / lanes < keep) lanes /= 2;
+  return lanes;
+}
 
 // The `keep` largest of a workgroup's numbers: those past a bound that at least
 // `keep` are not below, which is the least of `keep` (or more) groups' largest,
 // gathered in LDS and ranked there. Of shuffled numbers that leaves a few times
-// `keep`; where more than LDS holds (sorted ones), the bound is halved in on.
+// `keep`; where more than LDS holds (sorted ones, or equal ones), the bound is
+// halved in on. What costs is the logits' own arithmetic, ten operations each,
+// four of them the exponential's: 256 rows of 131072 in bf16, 30 % of them ended.
 // R: rounds of 8 values a thread.
 template <int T, int R>
 __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
   typedef num_t<T> V;
   __shared__ uint64_t list[kList];
-  __shared__ uint64_t lds_least[4], lds_most[4];
-  __shared__ float lds_f[4];
-  __shared__ int lds_n[4], lds_count;
+  __shared__ float lds_least[4], lds_top[4], lds_sum[4];
+  __shared__ int lds_groups[4], lds_n[4], lds_count;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   // Beams that have no score to go on from, or have ended, need no logits.
   if (!(a.scores[row] > -INFINITY) || (a.ended && a.ended[row])) return;
@@ -70,58 +79,57 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
     if (at < end) load_n(p + at, end - at, raw[r]);
   }
   float x[R][8], top = -INFINITY;
-  uint32_t best = 0;
-  int best_at = 0;
+#pragma unroll
+  for (int r = 0; r < R; r++) {
+    const int have = end - (begin + (r * kThreads + (int)threadIdx.x) * 8);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      x[r][j] = j < have ? Num<T>::get(raw[r][j]) : -INFINITY;
+      top = fmaxf(top, x[r][j]);
+    }
+  }
+  const auto key_of = [&](int r, int j) {  // (-0 is 0)
+    return (uint64_t)ordered(x[r][j] + 0.0f) << 32 | ~(uint32_t)(begin + (r * kThreads + (int)threadIdx.x) * 8 + j);
+  };
+  // The largest, and the bound: the largest of each group of lanes that has any, the least of those.
+  const int lanes = lanes_of((min(end - begin, kThreads * 8) + 7) / 8, a.keep);
+  float most = top;
+  for (int o = 1; o < lanes; o *= 2) most = fmaxf(most, __shfl_xor(most, o));
+  const uint64_t any = __ballot(most > -INFINITY && lane % lanes == 0);
+  float least = most > -INFINITY ? most : INFINITY;
+  top = most;
+  for (int o = lanes; o < 64; o *= 2) {
+    least = fminf(least, __shfl_xor(least, o));
+    top = fmaxf(top, __shfl_xor(top, o));
+  }
+  if (lane == 0) lds_least[wave] = least, lds_top[wave] = top, lds_groups[wave] = __popcll(any);
+  if (threadIdx.x == 0) lds_count = 0;
+  __syncthreads();
+  int groups = 0;
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    least = fminf(least, lds_least[w]);
+    top = fmaxf(top, lds_top[w]);
+    groups += lds_groups[w];
+  }
+  // (Nothing of -infinity is chosen.)
+  const float bound = groups >= a.keep && least < INFINITY ? least : -3.402823466e38f;
+  // Which of a thread's values are past it, a bit each; their values are read once more, where there are any.
+  const auto push = [&](uint64_t key) {
+    const int at = atomicAdd(&lds_count, 1);
+    if (at < kList) list[at] = key;
+  };
+  uint32_t past = 0;
 #pragma unroll
   for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const int at = begin + (r * kThreads + (int)threadIdx.x) * 8 + j;
-      x[r][j] = at < end ? Num<T>::get(raw[r][j]) + 0.0f : -INFINITY;  // (-0 is 0)
-      top = fmaxf(top, x[r][j]);
-      const uint32_t o = ordered(x[r][j]);
-      if (o > best) best = o, best_at = at;
-    }
-  const auto key_of = [&](int r, int j) {
-    return (uint64_t)ordered(x[r][j]) << 32 | ~(uint32_t)(begin + (r * kThreads + (int)threadIdx.x) * 8 + j);
-  };
-  // The largest, and the bound: the largest of each group of lanes, the least of those.
-  int groups = 4;
-  while (groups < a.keep) groups *= 2;
-  const int lanes = kThreads / groups;
-  uint64_t least = (uint64_t)best << 32 | ~(uint32_t)best_at, most = least;
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    const uint64_t other = shuffled(least, o);
-    least = (o < lanes) == (other > least) ? other : least;
-    const uint64_t more = shuffled(most, o);
-    most = more > most ? more : most;
-    top = fmaxf(top, __shfl_xor(top, o));
+    for (int j = 0; j < 8; j++) past = past + past + (x[r][j] >= bound ? 1u : 0u);
+  while (past) {
+    const int bit = __builtin_ctz(past), k = 8 * R - 1 - bit;
+    past &= past - 1;
+    const int at = begin + (k / 8 * kThreads + (int)threadIdx.x) * 8 + k % 8;
+    push((uint64_t)ordered(Num<T>::get(p[at]) + 0.0f) << 32 | ~(uint32_t)at);
   }
-  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most, lds_f[wave] = top;
-  if (threadIdx.x == 0) lds_count = 0;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < 4; w++) {
-    least = min(least, lds_least[w]), most = max(most, lds_most[w]);
-    top = fmaxf(top, lds_f[w]);
-  }
-  // Nothing of -infinity is chosen.
-  const uint64_t floor_ = (uint64_t)ordered(-INFINITY) << 32 | 0xffffffffu;
-  uint64_t bound = max(least, floor_ + 1);
-  const auto gather = [&] {
-#pragma unroll
-    for (int r = 0; r < R; r++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const uint64_t k = key_of(r, j);
-        if (k >= bound) {
-          const int at = atomicAdd(&lds_count, 1);
-          if (at < kList) list[at] = k;
-        }
-      }
-  };
-  gather();
 
   // The sum of exponentials.
   const float from = top == -INFINITY ? 0.0f : top;
@@ -132,14 +140,13 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
     for (int j = 0; j < 8; j++) sum += exp_of(x[r][j] - from);
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
-  __syncthreads();  // the list is whole, lds_f read
-  if (lane == 0) lds_f[wave] = sum;
-
+  if (lane == 0) lds_sum[wave] = sum;
+  __syncthreads();
   if (lds_count > kList) {  // (the same in all threads)
     // count(low) > kList, count(high) < keep; numbers differ, so some bound
     // between leaves between `keep` and kList of them.
-    uint64_t low = bound, high = most + 1;
-    while (true) {
+    uint64_t low = (uint64_t)ordered(bound) << 32, high = ((uint64_t)ordered(top + 0.0f) + 1) << 32;
+    while (high - low > 1) {
       const uint64_t mid = low + (high - low) / 2;
       int n = 0;
 #pragma unroll
@@ -150,19 +157,22 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
       if (lane == 0) lds_n[wave] = n;
       __syncthreads();
       n = lds_n[0] + lds_n[1] + lds_n[2] + lds_n[3];
-      bound = mid;
       if (n > kList) {
         low = mid;
-      } else if (n < a.keep && high - low > 1) {
+      } else if (n < a.keep) {
         high = mid;
       } else {
+        low = mid;
         break;
       }
-      if (high - low <= 1) break;  // (never, as numbers differ; NaNs' do too)
     }
     if (threadIdx.x == 0) lds_count = 0;
     __syncthreads();
-    gather();
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+        if (key_of(r, j) >= low) push(key_of(r, j));
     __syncthreads();
   }
   const int n = min(lds_count, kList);
@@ -174,10 +184,9 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
     if (rank < a.keep) out[rank] = mine;
   }
   for (int i = n + threadIdx.x; i < a.keep; i += kThreads) out[i] = 0;
-  __syncthreads();
   if (threadIdx.x == 0) {
     a.stats[2L * blockIdx.x] = top;
-    a.stats[2L * blockIdx.x + 1] = (lds_f[0] + lds_f[1]) + (lds_f[2] + lds_f[3]);
+    a.stats[2L * blockIdx.x + 1] = (lds_sum[0] + lds_sum[1]) + (lds_sum[2] + lds_sum[3]);
   }
 }
 
@@ -194,14 +203,26 @@ struct Choice {
   }
 };
 
-// A workgroup a text. `groups`: at least `keep`, of at most 64 neighbouring threads.
-__global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int groups, Divide by_each) {
+// A workgroup a text, a candidate or more a thread; `lanes` of a group, as above.
+// A chain of waits: the parts' statistics, their logarithm, the candidates (asked
+// for before it), the bound, the list.
+__global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Divide by_beams) {
   __shared__ Choice list[kChoices];
   __shared__ double lds_base[kMostBeams], lds_top[kMostBeams], lds_log[kMostBeams];
   __shared__ Choice lds_least[16], lds_most[16];
-  __shared__ int lds_live[kMostBeams], lds_n[16], lds_count;  // live: 0 no candidates, 1 its tokens, 2 ended
+  __shared__ int lds_live[kMostBeams], lds_n[16], lds_groups[16], lds_count;  // live: 0 no candidates, 1 its tokens, 2 ended
   const int b = blockIdx.x, threads = blockDim.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = threads / 64;
-  const int each = a.parts * a.keep;
+  const int each = a.parts * a.keep, all = a.beams * each, count = all + a.beams;  // (at most 2^25)
+  const uint64_t *keys = a.keys + (long)b * all;
+  // Neighbouring threads have candidates of different beams, so that a group has some of the best beam's.
+  auto key_at = [&](int c) {
+    const int i = by_beams(min(c, all - 1));
+    return keys[(min(c, all - 1) - i * a.beams) * each + i];
+  };
+  constexpr int kAhead = 4;
+  uint64_t ahead[kAhead];  // of beams without candidates: whatever lies there
+#pragma unroll
+  for (int k = 0; k < kAhead; k++) ahead[k] = key_at((int)threadIdx.x + k * threads);
   for (int i = wave; i < a.beams; i += waves) {
     const long row = (long)b * a.beams + i;
     const float base = a.scores[row];
@@ -214,7 +235,7 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int groups, Di
       for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
       for (int k = lane; k < a.parts; k += 64) {
         const float t = a.stats[2 * (row * a.parts + k)], s = a.stats[2 * (row * a.parts + k) + 1];
-        sum += t == -INFINITY ? (double)s : (double)s * exp((double)t - (double)top);
+        sum += t == -INFINITY ? (double)s : (double)s * (double)exp_of(t - top);
       }
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) sum += __longlong_as_double((long long)shuffled((uint64_t)__double_as_longlong(sum), o));
@@ -228,58 +249,68 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int groups, Di
   }
   if (threadIdx.x == 0) lds_count = 0;
   __syncthreads();
-  const int all = a.beams * each;  // (at most 2^25)
-  auto choice = [&](int c) -> Choice {
+  auto choice = [&](int c, uint64_t key) -> Choice {
     if (c >= all) {
       const int i = c - all;
       return lds_live[i] == 2 ? Choice{ordered(lds_base[i] + 0.0), ~((uint64_t)i * a.vocab + a.end)} : Choice{0, 0};
     }
-    const int i = by_each(c);
+    const int i = c - by_beams(c) * a.beams;
     if (lds_live[i] != 1) return Choice{0, 0};
-    const uint64_t key = a.keys[(long)b * all + c];
     if (key == 0) return Choice{0, 0};
     const double x = (double)unordered((uint32_t)(key >> 32));
     const double score = lds_base[i] + ((x - lds_top[i]) - lds_log[i]);
     if (!(score > -INFINITY)) return Choice{0, 0};
     return Choice{ordered(score + 0.0), ~((uint64_t)i * a.vocab + (uint32_t)~(uint32_t)key)};
   };
-  const int count = all + a.beams;
-  Choice least{0, 0};
-  for (int c = threadIdx.x; c < count; c += threads) {
-    const Choice k = choice(c);
-    if (k > least) least = k;
-  }
-  Choice most = least;
-  const int lanes = threads / groups;
+  // Each thread's candidates: the first from what was asked for ahead.
+  auto each_choice = [&](auto &&take) {
 #pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
+    for (int k = 0; k < kAhead; k++) {
+      const int c = (int)threadIdx.x + k * threads;
+      if (c < count) take(choice(c, ahead[k]));
+    }
+    for (int c = (int)threadIdx.x + kAhead * threads; c < count; c += threads) take(choice(c, key_at(c)));
+  };
+  Choice best{0, 0};
+  each_choice([&](const Choice &k) {
+    if (k > best) best = k;
+  });
+  for (int o = 1; o < lanes; o *= 2) {
+    const Choice other{shuffled(best.score, o), shuffled(best.at, o)};
+    if (other > best) best = other;
+  }
+  const uint64_t any = __ballot(best.score != 0 && lane % lanes == 0);
+  constexpr Choice kPast{~uint64_t(0), ~uint64_t(0)};
+  Choice least = best.score ? best : kPast, most = best;
+  for (int o = lanes; o < 64; o *= 2) {
     const Choice other{shuffled(least.score, o), shuffled(least.at, o)};
-    if (o < lanes ? other > least : least > other) least = other;
+    if (least > other) least = other;
     const Choice more{shuffled(most.score, o), shuffled(most.at, o)};
     if (more > most) most = more;
   }
-  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most;
+  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most, lds_groups[wave] = __popcll(any);
   __syncthreads();
+  int groups = 0;
   for (int w = 0; w < waves; w++) {
     if (least > lds_least[w]) least = lds_least[w];
     if (lds_most[w] > most) most = lds_most[w];
+    groups += lds_groups[w];
   }
-  if (least.score == 0) least = Choice{0, 1};  // none is not chosen
+  if (groups < a.keep) least = Choice{0, 1};  // all there are (none, 0, is not chosen)
   auto gather = [&] {
-    for (int c = threadIdx.x; c < count; c += threads) {
-      const Choice k = choice(c);
+    each_choice([&](const Choice &k) {
       if (!(least > k)) {
         const int at = atomicAdd(&lds_count, 1);
         if (at < kChoices) list[at] = k;
       }
-    }
+    });
   };
   gather();
   __syncthreads();
   if (lds_count > kChoices) {  // (the same in all threads)
     auto count_from = [&](const Choice &bound) {
       int n = 0;
-      for (int c = threadIdx.x; c < count; c += threads) n += !(bound > choice(c));
+      each_choice([&](const Choice &k) { n += !(bound > k); });
 #pragma unroll
       for (int o = 1; o < 64; o *= 2) n += __shfl_xor(n, o);
       __syncthreads();
@@ -456,13 +487,10 @@ hipError_t launch_beam_select(const SelectArgs &a, int type, hipStream_t s) {
                        : type == PPOCR_F16  ? launch_parts_of<PPOCR_F16>(a, s)
                                             : hipErrorInvalidValue;
   if (e != hipSuccess) return e;
-  // Four candidates or more a thread, and a group of threads at least for each kept.
-  int threads = 64, groups = 1;
-  while (groups < a.keep) groups *= 2;
-  while (threads < 1024 && (threads < groups || 4L * threads * 2 <= (long)a.beams * a.parts * a.keep)) threads *= 2;
-  groups = std::max(groups, threads / 64);
-  return launch_kernel(beam_choice, dim3(a.batch), dim3(threads), 0, s, a, groups,
-                       Divide(a.parts * a.keep));
+  const long all = (long)a.beams * a.parts * a.keep;
+  const int threads = int(std::min((all + 63) / 64 * 64, 1024L));
+  return launch_kernel(beam_choice, dim3(a.batch), dim3(threads), 0, s, a,
+                       lanes_of(int(std::min(all, long(threads))), a.keep), Divide(a.beams));
 }
 
 hipError_t launch_beam_reorder(const ReorderArgs &a, hipStream_t s) {
