@@ -58,8 +58,8 @@ __host__ __device__ inline int lanes_of(int used, int keep) {
 // `keep`; where more than LDS holds (sorted ones, or equal ones), the bound is
 // halved in on. What costs is the logits' own arithmetic, ten operations each,
 // four of them the exponential's: 256 rows of 131072 in bf16, 30 % of them ended.
-// R: rounds of 8 values a thread.
-template <int T, int R>
+// R: rounds of 8 values a thread. FEW: rows of fewer than 8 values.
+template <int T, int R, bool FEW>
 __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
   typedef num_t<T> V;
   __shared__ uint64_t list[kList];
@@ -67,29 +67,46 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
   __shared__ int lds_groups[4], lds_n[4], lds_count;
   const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
   // Beams that have no score to go on from, or have ended, need no logits.
-  if (!(a.scores[row] > -INFINITY) || (a.ended && a.ended[row])) return;
+  const float score = a.scores[row];
+  int over = 0;
+  if (a.ended) over = a.ended[row];
+  if (!(score > -INFINITY) || over) return;
   const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int begin = part * a.chunk, end = min(begin + a.chunk, a.vocab);
   const V *p = (const V *)a.logits + row * a.stride;
 
+  // Round r's piece: values at_of(r) .. at_of(r) + 7; the last one begins where the row still has eight, and its
+  // first values are the piece's before it. (Nothing is read behind a branch, which would be waited for.)
   V raw[R][8];
+  const int last = max(a.vocab - 8, 0);
+  const auto at_of = [&](int r) { return min(begin + (r * kThreads + (int)threadIdx.x) * 8, last); };
 #pragma unroll
   for (int r = 0; r < R; r++) {
-    const int at = begin + (r * kThreads + (int)threadIdx.x) * 8;
-    if (at < end) load_n(p + at, end - at, raw[r]);
+    if constexpr (FEW) {
+      for (int j = 0; j < 8; j++) raw[r][j] = p[min(at_of(r) + j, a.vocab - 1)];
+    } else {
+      __builtin_memcpy(raw[r], p + at_of(r), sizeof raw[r]);
+    }
   }
   float x[R][8], top = -INFINITY;
 #pragma unroll
-  for (int r = 0; r < R; r++) {
-    const int have = end - (begin + (r * kThreads + (int)threadIdx.x) * 8);
+  for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      x[r][j] = j < have ? Num<T>::get(raw[r][j]) : -INFINITY;
-      top = fmaxf(top, x[r][j]);
+    for (int j = 0; j < 8; j++) x[r][j] = Num<T>::get(raw[r][j]);
+  if (end - begin != R * kThreads * 8) {  // a row's last part
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int first = begin + (r * kThreads + (int)threadIdx.x) * 8 - at_of(r), have = end - at_of(r);
+#pragma unroll
+      for (int j = 0; j < 8; j++) x[r][j] = j >= first && j < have ? x[r][j] : -INFINITY;
     }
   }
+#pragma unroll
+  for (int r = 0; r < R; r++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) top = fmaxf(top, x[r][j]);
   const auto key_of = [&](int r, int j) {  // (-0 is 0)
-    return (uint64_t)ordered(x[r][j] + 0.0f) << 32 | ~(uint32_t)(begin + (r * kThreads + (int)threadIdx.x) * 8 + j);
+    return (uint64_t)ordered(x[r][j] + 0.0f) << 32 | ~(uint32_t)(at_of(r) + j);
   };
   // The largest, and the bound: the largest of each group of lanes that has any, the least of those.
   const int lanes = lanes_of((min(end - begin, kThreads * 8) + 7) / 8, a.keep);
@@ -127,7 +144,7 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
   while (past) {
     const int bit = __builtin_ctz(past), k = 8 * R - 1 - bit;
     past &= past - 1;
-    const int at = begin + (k / 8 * kThreads + (int)threadIdx.x) * 8 + k % 8;
+    const int at = at_of(k / 8) + k % 8;
     push((uint64_t)ordered(Num<T>::get(p[at]) + 0.0f) << 32 | ~(uint32_t)at);
   }
 
@@ -382,9 +399,10 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
 template <int T>
 hipError_t launch_parts_of(const SelectArgs &a, hipStream_t s) {
   const dim3 grid(unsigned((long)a.batch * a.beams * a.parts)), block(kThreads);
-  if (a.chunk <= kThreads * 8) return launch_kernel(beam_parts<T, 1>, grid, block, 0, s, a);
-  if (a.chunk <= kThreads * 16) return launch_kernel(beam_parts<T, 2>, grid, block, 0, s, a);
-  return launch_kernel(beam_parts<T, 4>, grid, block, 0, s, a);
+  if (a.vocab < 8) return launch_kernel(beam_parts<T, 1, true>, grid, block, 0, s, a);
+  if (a.chunk == kThreads * 8) return launch_kernel(beam_parts<T, 1, false>, grid, block, 0, s, a);
+  if (a.chunk == kThreads * 16) return launch_kernel(beam_parts<T, 2, false>, grid, block, 0, s, a);
+  return launch_kernel(beam_parts<T, 4, false>, grid, block, 0, s, a);
 }
 
 // -------------------------------------------------------------- the reordering
@@ -473,11 +491,10 @@ __global__ __launch_bounds__(256) void beam_reorder_rows(ReorderArgs a) {
 }  // namespace
 
 SelectParts select_parts(long rows, int vocab) {
-  // Parts of 2048 to 8192 values (8 to 32 a thread), as large as still gives the
-  // card 2048 workgroups; all about as long.
-  const long least = (vocab + 8191L) / 8192, most = (vocab + 2047L) / 2048;
-  const long parts = std::min(std::max((2048 + rows - 1) / rows, least), most);
-  const int chunk = int(((vocab + parts - 1) / parts + 7) / 8 * 8);
+  // Parts of 8192 values (32 a thread), or of 4096 or 2048 where that leaves the
+  // card fewer than 2048 workgroups.
+  int chunk = 8192;
+  while (chunk > 2048 && rows * ((vocab + chunk - 1) / chunk) < 2048) chunk /= 2;
   return {(vocab + chunk - 1) / chunk, chunk};
 }
 
