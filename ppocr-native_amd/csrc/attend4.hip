@@ -1,6 +1,7 @@
-// Attention over a cache in 4 bits, of bf16 and f16 queries; the join of a
-// split cache's parts, and how many there are.
-#include "attend4.hpp"
+// Attention over a cache in 4 bits: the choice of a kernel, the parts of a split
+// cache and their join.
+#include "seen.hpp"
+#include "writer.hpp"
 
 namespace ppocr {
 namespace {
@@ -11,11 +12,11 @@ constexpr int kMostParts4 = 128;
 // parts i and i + 64's factors, wave w adds parts w, w + 4, ... of them.
 // J: 64s of dim, rounded up to a power of two.
 template <int J>
-__global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a) {
+__global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a, int keys) {
   __shared__ float lds_o[4][256], lds_f[kMostParts4];
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const int length = a.c.lengths[b];
-  const Seen s = seen_of(length > a.c.table_width * a.c.page_size ? 0 : length, a.window, a.sinks, kKeys4);
+  const Seen s = seen_of(length > a.c.table_width * a.c.page_size ? 0 : length, a.window, a.sinks, keys);
   const int each = tiles_a_part(s.tiles, a.each, a.splits);
   const int parts = max(1, (s.tiles + each - 1) / each), dim = a.c.dim, row = dim + 2, far = lane + 64;
   const float *p = a.part + ((long)b * a.heads + head) * a.splits * row;
@@ -56,17 +57,34 @@ __global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a) {
 }  // namespace
 
 PagedParts kv4_parts(int batch, int heads, int kv_heads, long longest) {
-  // As the plain cache's parts of 32 keys a tile.
-  return paged_parts(batch, heads, kv_heads, PPOCR_BF16, longest);
+  // As long as were 2048 workgroups of it if all texts were the longest: two to
+  // four times what the card holds at once (1024: 92 instead of 76 us for 32 texts
+  // of every length up to 16384; 4096: 78); but of 512 tokens at least, or 128
+  // where that leaves too few for the card. A text of 512 is done without a join.
+  const int per = heads / kv_heads, keys = 16 * halves4(copies4(per)), least = 512 / keys, few = 128 / keys;
+  const long groups = (long)batch * kv_heads * ((per + 15) / 16), tiles = (longest + keys - 1) / keys + 2;
+  long each = (tiles * groups + 2047) / 2048;
+  if (each < least) {
+    const long fill = (tiles * groups + 511) / 512;
+    each = tiles <= least + 1 ? least + 1 : fill < few ? few : fill < least ? fill : least;
+  }
+  if (each < (tiles + kMostParts4 - 1) / kMostParts4) each = (tiles + kMostParts4 - 1) / kMostParts4;
+  const long splits = (tiles + each - 1) / each;
+  return {int(splits < 1 ? 1 : splits), int(each)};
 }
 
-hipError_t launch_kv4_join(const Attend4Args &a, hipStream_t s) {
+hipError_t launch_kv4_attention(const Attend4Args &a, hipStream_t s) {
+  const int copies = copies4(a.heads / a.c.heads);
+  const bool two = a.type == PPOCR_F32;
+  const hipError_t e = copies == 4   ? (two ? launch_attention4<true, 4>(a, s) : launch_attention4<false, 4>(a, s))
+                       : copies == 2 ? (two ? launch_attention4<true, 2>(a, s) : launch_attention4<false, 2>(a, s))
+                                     : (two ? launch_attention4<true, 1>(a, s) : launch_attention4<false, 1>(a, s));
+  if (e != hipSuccess || a.splits == 1) return e;
   const dim3 grid(a.heads, a.batch), block(256);
-  if (a.c.dim <= 64) return launch_kernel(kv4_attention_join<1>, grid, block, 0, s, a);
-  if (a.c.dim <= 128) return launch_kernel(kv4_attention_join<2>, grid, block, 0, s, a);
-  return launch_kernel(kv4_attention_join<4>, grid, block, 0, s, a);
+  const int keys = 16 * halves4(copies);
+  if (a.c.dim <= 64) return launch_kernel(kv4_attention_join<1>, grid, block, 0, s, a, keys);
+  if (a.c.dim <= 128) return launch_kernel(kv4_attention_join<2>, grid, block, 0, s, a, keys);
+  return launch_kernel(kv4_attention_join<4>, grid, block, 0, s, a, keys);
 }
-
-hipError_t launch_kv4_attention_16(const Attend4Args &a, hipStream_t s) { return launch_attention4<false>(a, s); }
 
 }  // namespace ppocr

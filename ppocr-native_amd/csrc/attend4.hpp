@@ -10,52 +10,69 @@
 //
 // Four bits are an f16 as they are: bits 0 .. 3 of a 16-bit half are n 2^-24,
 // bits 4 .. 7 are n 2^-20, both below the smallest normal number. So eight codes
-// of a word cost four masks and one shift, and four packed products with 2^15
-// to make them normal numbers, n 2^-9 and n 2^-5: the matrix cores take the
-// others too, but line products up by exponents that leave out the zeros in
-// front, and cut them 2^-20 of the largest from the top (4 % faster, and 16-bit
-// results hardly show it; f32 ones were off by 2^-13). The 2^4 between the two
-// goes into q (K) or into the result (V). K's words have eight dims of a token;
-// V's have two dims of four tokens, so that the same masks give pairs of keys,
-// which is what the product over keys wants.
+// of a word cost four masks and one shift. The matrix cores take such numbers,
+// but line products up by exponents that leave out the zeros in front, and cut
+// each product 2^-20 or so below the largest: 16-bit queries' logits are off by
+// some 2^-16 of their terms, an eighth of an f16's half step at most. For f32
+// queries four packed products with 2^15 make them normal numbers, n 2^-9 and
+// n 2^-5. The 2^4 between the two goes into q (K) or into the result (V). K's
+// words have eight dims of a token; V's have two dims of four tokens, so that
+// the same masks give pairs of keys, which is what the product over keys wants.
+//
+// The sixteen columns of a product are a key head's query heads, or where those
+// are eight or four at most, two or four of each: then a column has every second
+// or fourth 16 keys, and its own largest and sum, and a lane half or a quarter of
+// the softmax's work (32 texts to 16384 tokens, four query heads a key head, 8 key
+// heads of 128 in bf16 and groups of 64: 97 us with one column a row).
 #pragma once
+#include <type_traits>
+
 #include "seen.hpp"
 #include "writer.hpp"
 
 namespace ppocr {
 
-constexpr int kWaves4 = 4, kKeys4 = 32;
+constexpr int kWaves4 = 4;
 
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-// The codes that a mask leaves, as normal numbers.
+// The codes that a mask leaves, as they are or as normal numbers.
+template <bool NORMAL>
 __device__ __forceinline__ uint32_t codes16(uint32_t w, uint32_t mask) {
   const uint32_t n = w & mask;
+  if constexpr (!NORMAL) return n;
   return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, n) * v2h{(_Float16)0x1p15f, (_Float16)0x1p15f});
 }
 __device__ __forceinline__ uint32_t pair16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
 }
-__device__ __forceinline__ void put_at(void *p, long i, int type, float v) {
-  if (type == PPOCR_F32)
-    ((float *)p)[i] = v;
-  else if (type == PPOCR_BF16)
-    ((__bf16 *)p)[i] = (__bf16)v;
-  else
-    ((_Float16 *)p)[i] = (_Float16)v;
+// N dwords, in the widest pieces there are.
+template <int N>
+struct Words {
+  typedef std::conditional_t<N % 4 == 0, v4u, std::conditional_t<N % 2 == 0, v2u, uint32_t>> Piece;
+  Piece w[4 * N / sizeof(Piece)];
+};
+template <int N>
+__device__ __forceinline__ Words<N> words_at(const char *p) {
+  Words<N> w;
+  __builtin_memcpy(&w, p, sizeof w);
+  return w;
 }
 
-// The state of 16 rows (query heads of a key head), a wave's worth: a lane has
-// row lane % 16, quarter lane / 16 of the keys. NC: 32s of a padded head; GC:
-// those of a group; TWO: q in two f16 parts (22 bits) instead of one (11 bits,
-// all that 16-bit queries have).
-template <int NC, int GC, bool TWO>
+// The state of 16 columns, a wave's worth: a lane has column lane % 16, row lane %
+// (16 / CP) of the query heads, and of each 16 keys the four of quarter lane / 16.
+// NC: 32s of a padded head; GC: those of a group; TWO: q in two f16 parts (22
+// bits) instead of one (11 bits, all that 16-bit queries have); CP: columns a row.
+template <int NC, int GC, bool TWO, int CP>
 struct Rows4 {
   static constexpr int G = (NC + GC - 1) / GC, DP = 32 * NC, E = 2 * NC;
+  static constexpr int H = halves4(CP), L = H / CP;  // 16s of keys a tile, and a lane
+  static constexpr int UNIT = TWO ? 9 : 24;  // codes are multiplied as n 2^-UNIT
+  static constexpr int FEW = H * G / 2;      // dwords of a tile's scales and minima a lane brings
   v4u q[TWO ? 2 : 1][NC];  // times 2^e of the row, odd dims 2^-4 of that
-  float qs[G];             // sums of q over a group, times 2^(e - 9)
-  v4f o[E];                // lane's row, dim 32 c + 2 (4 quarter + r) + b in o[2 c + b][r]
+  float qs[G];             // sums of q over a group, times 2^(e - UNIT)
+  v4f o[E];                // lane's column, dim 32 c + 2 (4 quarter + r) + b in o[2 c + b][r]
   float om[G];             // this lane's share of sum P m
   // Weights are 2^(S scale - base); base is the largest S scale less `up`, and
   // 2^up times any scale of V is at most 2^15, so that products of the two
@@ -63,11 +80,11 @@ struct Rows4 {
   // above it.
   float m, l, base, scale, most, up;
 
-  // Eight neighbouring dims of a row from d, as they are stored; past dim the
-  // last one (all loads are on their way before the first is used).
-  template <class V>
+  // Eight neighbouring dims of a row from d, as they are stored; past dim some
+  // others of the row. EIGHTS: heads are of a multiple of 8 dims.
+  template <bool EIGHTS, class V>
   static __device__ __forceinline__ void load8(const V *p, int d, int dim, V (&v)[8]) {
-    if (dim % 8 == 0) {
+    if constexpr (EIGHTS) {
       __builtin_memcpy(v, p + min(d, dim - 8), sizeof v);
     } else {
 #pragma unroll
@@ -75,59 +92,92 @@ struct Rows4 {
     }
   }
 
+  template <bool EIGHTS>
   __device__ __forceinline__ void start(const void *q_, long at, int type, int dim, int quarter, float by, bool turn) {
-    float x[NC][8];
-    uint32_t top = 0;
-    if constexpr (TWO) {
+    typedef std::conditional_t<TWO, uint32_t, uint16_t> Raw;
+    constexpr Raw kSign = TWO ? 0x80000000u : 0x8000u;
+    Raw raw[NC][8];
 #pragma unroll
-      for (int c = 0; c < NC; c++) load8((const float *)q_ + at, 32 * c + 8 * quarter, dim, x[c]);
-    } else {
-      uint16_t raw[NC][8];
-#pragma unroll
-      for (int c = 0; c < NC; c++) load8((const uint16_t *)q_ + at, 32 * c + 8 * quarter, dim, raw[c]);
+    for (int c = 0; c < NC; c++) load8<EIGHTS>((const Raw *)q_ + at, 32 * c + 8 * quarter, dim, raw[c]);
+    if (dim != DP) {
 #pragma unroll
       for (int c = 0; c < NC; c++)
 #pragma unroll
         for (int j = 0; j < 8; j++)
-          x[c][j] = type == PPOCR_BF16 ? __uint_as_float((uint32_t)raw[c][j] << 16)
-                                       : (float)__builtin_bit_cast(_Float16, raw[c][j]);
+          if (32 * c + 8 * quarter + j >= dim) raw[c][j] = 0;
     }
+    // The largest, as bits without the sign.
+    uint32_t top = 0;
+    if constexpr (TWO) {
 #pragma unroll
-    for (int c = 0; c < NC; c++)
+      for (int c = 0; c < NC; c++)
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        if (32 * c + 8 * quarter + j >= dim) x[c][j] = 0.0f;
-        top = max(top, __float_as_uint(x[c][j]) & 0x7fffffffu);
-      }
+        for (int j = 0; j < 8; j++) top = max(top, raw[c][j] & 0x7fffffffu);
+    } else {
+      typedef uint16_t v2s __attribute__((ext_vector_type(2)));
+      v2s two{0, 0};
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          two = __builtin_elementwise_max(two, v2s{raw[c][j], raw[c][j + 1]} & (v2s)(0x7fff));
+      top = max((uint32_t)two[0], (uint32_t)two[1]);
+    }
     top = max(top, (uint32_t)__shfl_xor((int)top, 16));
     top = max(top, (uint32_t)__shfl_xor((int)top, 32));
+    if constexpr (!TWO)
+      top = type == PPOCR_BF16 ? top << 16 : __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)top));
     // q's largest is 2^13 or more, below 2^14 (less only where all are below f32's normal numbers).
     const int e = 13 - ((int)(top >> 23) - 127);
     // 2^100 keeps sums times it finite: at such a scale one key has all the weight. 2^-126 stands for 0, which a
     // hidden key's -infinity could not be multiplied with.
-    scale = fmaxf(fminf(__builtin_ldexpf(by, 9 - e) * 1.44269504088896340736f, 0x1p100f), 0x1p-126f);
+    scale = fmaxf(fminf(__builtin_ldexpf(by, UNIT - e) * 1.44269504088896340736f, 0x1p100f), 0x1p-126f);
     if (top >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u);  // an infinity or NaN in q: NaN
+    if (turn) {
 #pragma unroll
-    for (int g = 0; g < G; g++) qs[g] = 0.0f, om[g] = 0.0f;
+      for (int c = 0; c < NC; c++)
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
+        for (int j = 0; j < 8; j++) raw[c][j] ^= kSign;
+    }
+    // (16-bit numbers fit f16's 11 bits: rounding to 0 changes none that is not below its steps.)
+    auto fill = [&](auto value) {
+#pragma unroll
+      for (int c = 0; c < NC; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float x = __builtin_ldexpf(value(raw[c][i]), i & 1 ? e - 4 : e), y = __builtin_ldexpf(value(raw[c][i + 4]), i & 1 ? e - 4 : e);
+          if constexpr (TWO) {
+            const v2h high = __builtin_convertvector(v2f{x, y}, v2h);
+            q[0][c][i] = __builtin_bit_cast(uint32_t, high);
+            q[TWO][c][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{x - (float)high[0], y - (float)high[1]}, v2h));
+          } else {
+            q[0][c][i] = pair16(x, y);
+          }
+        }
+    };
+    if constexpr (TWO)
+      fill([](uint32_t u) { return __uint_as_float(u); });
+    else if (type == PPOCR_BF16)
+      fill([](uint16_t u) { return __uint_as_float((uint32_t)u << 16); });
+    else
+      fill([](uint16_t u) { return (float)__builtin_bit_cast(_Float16, u); });
+    const v2h one{(_Float16)0x1p-9f, (_Float16)0x1p-9f}, few_{(_Float16)0x1p-5f, (_Float16)0x1p-5f};
+#pragma unroll
+    for (int g = 0; g < G; g++) {
       float sum = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        x[c][j] = __builtin_ldexpf(turn ? -x[c][j] : x[c][j], e);
-        sum += x[c][j];
-      }
+      for (int c = g * GC; c < NC && c < (g + 1) * GC; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+          for (int part = 0; part <= TWO; part++) {
+            const uint32_t two = q[part][c][i];
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, two), i & 1 ? few_ : one, sum, false);
+          }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
-      qs[c / GC] += sum * 0x1p-9f;
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float odd = i & 1 ? 0x1p-4f : 1.0f, a = x[c][i] * odd, b = x[c][i + 4] * odd;
-        const v2h high = __builtin_convertvector(v2f{a, b}, v2h);
-        q[0][c][i] = __builtin_bit_cast(uint32_t, high);
-        if constexpr (TWO)
-          q[1][c][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{a - (float)high[0], b - (float)high[1]}, v2h));
-      }
+      qs[g] = TWO ? sum : sum * 0x1p-15f;
+      om[g] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = v4f{0, 0, 0, 0};
@@ -136,52 +186,19 @@ struct Rows4 {
     up = 15.0f;
   }
 
-  // Half a tile's codes of 16 keys, of which this lane has row lane % 16 of K and
-  // the four keys 4 quarter .. 4 quarter + 3 of V and of all scales and minima.
-  struct Half {
-    uint32_t n[NC];
-    _Float16 s[4 * G], m[4 * G];
+  // A tile's codes: 16s of keys, of which this lane has row lane % 16 of K and the
+  // four keys 4 quarter .. 4 quarter + 3 of V. (Its scales and minima, 128 H G
+  // bytes, go through LDS: as loads of a lane's own they would be 4 H times as many.)
+  uint32_t k[H][NC], v[H][NC];
+
+  // Of 16 keys' 4 quarter .. + 3, for each group: plane 0 K's scales, 1 its minima, 2 and 3 V's.
+  struct Few {
+    _Float16 of[4 * G];
   };
-  Half k[2], v[2];
-
-  // `p`: the page's chunk, `slot`: the half's first token in the page.
-  static __device__ __forceinline__ void load(Half &t, const char *p, int codes, int scales, int minima, int slot,
-                                              int at, int quarter) {
-    const int few = 2 * G * (slot + 4 * quarter);
-    __builtin_memcpy(t.n, p + codes + slot * 16 * NC + at * 4 * NC, 4 * NC);
-    __builtin_memcpy(t.s, p + scales + few, 8 * G);
-    __builtin_memcpy(t.m, p + minima + few, 8 * G);
-  }
-  __device__ __forceinline__ void load_k(int half, const char *p, int slot, const Kv4Args &c, int lane) {
-    load(k[half], p, 0, c.at_ks, c.at_km, slot, lane % 16 * 4 + lane / 16, lane / 16);
-  }
-  __device__ __forceinline__ void load_v(int half, const char *p, int slot, const Kv4Args &c, int lane) {
-    load(v[half], p, c.at_v, c.at_vs, c.at_vm, slot, lane, lane / 16);
-  }
-
-  // The products of K's half with q.
-  __device__ __forceinline__ v4f products(const Half &t) const {
-    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    v4f sum[G], s{0, 0, 0, 0};
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-      sum[g] = v4f{0, 0, 0, 0};
-#pragma unroll
-      for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
-        const uint32_t w = t.n[c], u = w >> 8;
-        const v4u a{codes16(w, kLow), codes16(w, kHigh), codes16(u, kLow), codes16(u, kHigh)};
-        sum[g] = mfma16(a, q[0][c], sum[g]);
-        if constexpr (TWO) sum[g] = mfma16(a, q[1][c], sum[g]);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++)
-#pragma unroll
-      for (int g = 0; g < G; g++) {
-        s[r] = fmaf((float)t.m[r * G + g], qs[g], s[r]);
-        s[r] = fmaf((float)t.s[r * G + g], sum[g][r], s[r]);
-      }
-    return s;
+  static __device__ __forceinline__ Few few_of(const char *lds, int half, int plane, int quarter) {
+    Few f;
+    __builtin_memcpy(f.of, __builtin_assume_aligned(lds + ((half * 4 + plane) * 4 + quarter) * 8 * G, G % 2 ? 8 : 16), 8 * G);
+    return f;
   }
 
   // Raises the largest product and V's largest scale to a tile's.
@@ -204,36 +221,72 @@ struct Rows4 {
     base = next;
   }
 
-  // Takes in the tile in k and v. seen(key of the tile): whether the rows see it
-  // (asked where `masked`); next_k() and next_v() ask for the next tile's as soon
-  // as this one's are used.
+  // Takes in the tile in k and v, its scales and minima at `lds`. seen(key of the
+  // tile): whether the rows see it (asked where `masked`); next_k() and next_v()
+  // ask for the next tile's as soon as this one's are used.
   template <class Seen, class NextK, class NextV>
-  __device__ __forceinline__ void use(Seen seen, bool masked, int quarter, NextK next_k, NextV next_v) {
+  __device__ __forceinline__ void use(const char *lds, Seen seen, bool masked, int lane, NextK next_k, NextV next_v) {
     constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
-    v4f s[2] = {products(k[0]), products(k[1])};
-    next_k();
-    if (masked) {
+    const int quarter = lane / 16, copy = lane % 16 / (16 / CP);
+    // The products of K with q: of a lane's own 16s of keys.
+    v4f s[L][G];
 #pragma unroll
-      for (int h = 0; h < 2; h++)
+    for (int h = 0; h < H; h++)
+#pragma unroll
+      for (int g = 0; g < G; g++) {
+        v4f sum{0, 0, 0, 0};
+#pragma unroll
+        for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
+          const uint32_t w = k[h][c], u = w >> 8;
+          const v4u a{codes16<TWO>(w, kLow), codes16<TWO>(w, kHigh), codes16<TWO>(u, kLow), codes16<TWO>(u, kHigh)};
+          sum = mfma16(a, q[0][c], sum);
+          if constexpr (TWO) sum = mfma16(a, q[1][c], sum);
+        }
+        if (h / L == 0) {
+          s[h % L][g] = sum;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; r++) s[h % L][g][r] = copy == h / L ? sum[r] : s[h % L][g][r];
+        }
+      }
+    next_k();
+    Few vs[L], vm[L];
+    float z[L][4];
+#pragma unroll
+    for (int j = 0; j < L; j++) {
+      const int half = copy * L + j;
+      const Few ks = few_of(lds, half, 0, quarter), km = few_of(lds, half, 1, quarter);
+      vs[j] = few_of(lds, half, 2, quarter), vm[j] = few_of(lds, half, 3, quarter);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        z[j][r] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+          z[j][r] = fmaf((float)km.of[r * G + g], qs[g], z[j][r]);
+          z[j][r] = fmaf((float)ks.of[r * G + g], s[j][g][r], z[j][r]);
+        }
+      }
+      if (masked) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const bool on = seen(16 * h + 4 * quarter + r);
-          s[h][r] = on ? s[h][r] : -INFINITY;
+          const bool on = seen(16 * half + 4 * quarter + r);
+          z[j][r] = on ? z[j][r] : -INFINITY;
 #pragma unroll
           for (int g = 0; g < G; g++) {
-            v[h].s[r * G + g] = on ? v[h].s[r * G + g] : (_Float16)0.0f;
-            v[h].m[r * G + g] = on ? v[h].m[r * G + g] : (_Float16)0.0f;
+            vs[j].of[r * G + g] = on ? vs[j].of[r * G + g] : (_Float16)0.0f;
+            vm[j].of[r * G + g] = on ? vm[j].of[r * G + g] : (_Float16)0.0f;
           }
         }
+      }
     }
     float top = -INFINITY;
     v2h wide{0, 0};
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
+    for (int j = 0; j < L; j++) {
 #pragma unroll
-      for (int r = 0; r < 4; r++) top = fmaxf(top, s[h][r]);
+      for (int r = 0; r < 4; r++) top = fmaxf(top, z[j][r]);
 #pragma unroll
-      for (int i = 0; i < 4 * G; i += 2) wide = __builtin_elementwise_max(wide, v2h{v[h].s[i], v[h].s[i + 1]});
+      for (int i = 0; i < 4 * G; i += 2) wide = __builtin_elementwise_max(wide, v2h{vs[j].of[i], vs[j].of[i + 1]});
     }
     const float large = (float)__builtin_elementwise_max(wide[0], wide[1]);
     top = fmaxf(top, __shfl_xor(top, 16));
@@ -241,45 +294,57 @@ struct Rows4 {
     const float now = fmaxf(m, top);
     if (__any(now != m || large > most)) raise(now, large);
     const float from = base == -INFINITY ? 0.0f : base;
-    float p[2][4];
+    float p[L][4];
 #pragma unroll
-    for (int h = 0; h < 2; h++)
+    for (int j = 0; j < L; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        p[h][r] = __builtin_amdgcn_exp2f(fmaf(s[h][r], scale, -from));
-        l += p[h][r];
+        p[j][r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], scale, -from));
+        l += p[j][r];
 #pragma unroll
-        for (int g = 0; g < G; g++) om[g] = fmaf(p[h][r], (float)v[h].m[r * G + g], om[g]);
+        for (int g = 0; g < G; g++) om[g] = fmaf(p[j][r], (float)vm[j].of[r * G + g], om[g]);
       }
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      // Weights times scales in two f16 parts: 22 bits.
-      v4u high, low;
+      // Weights times scales in two f16 parts: 22 bits. Keys r and r + 2 of a quarter side by side, as the masks
+      // leave V's; a column has its own 16s of keys and zeros for the others.
+      uint32_t high[L][2], low[L][2];
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int h = i / 2, r = i % 2;  // keys r and r + 2 of the quarter, as the masks leave V's
-        const float x = fmaf(p[h][r], (float)v[h].s[r * G + g], 0.0f);
-        const float y = fmaf(p[h][r + 2], (float)v[h].s[(r + 2) * G + g], 0.0f);
-        const uint32_t both = pair16(x, y);
-        const v2h back = __builtin_bit_cast(v2h, both);
-        high[i] = both;
-        low[i] = pair16(fmaf((float)back[0], -1.0f, x), fmaf((float)back[1], -1.0f, y));
-      }
+      for (int j = 0; j < L; j++)
 #pragma unroll
-      for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
-        const uint32_t w0 = v[0].n[c], w1 = v[1].n[c], u0 = w0 >> 8, u1 = w1 >> 8;
-        const v4u even{codes16(w0, kLow), codes16(u0, kLow), codes16(w1, kLow), codes16(u1, kLow)};
-        const v4u odd{codes16(w0, kHigh), codes16(u0, kHigh), codes16(w1, kHigh), codes16(u1, kHigh)};
-        o[2 * c] = mfma16(even, low, o[2 * c]);
-        o[2 * c + 1] = mfma16(odd, low, o[2 * c + 1]);
-        o[2 * c] = mfma16(even, high, o[2 * c]);
-        o[2 * c + 1] = mfma16(odd, high, o[2 * c + 1]);
+        for (int r = 0; r < 2; r++) {
+          const float x = fmaf(p[j][r], (float)vs[j].of[r * G + g], 0.0f);
+          const float y = fmaf(p[j][r + 2], (float)vs[j].of[(r + 2) * G + g], 0.0f);
+          const uint32_t both = pair16(x, y);
+          const v2h back = __builtin_bit_cast(v2h, both);
+          high[j][r] = both;
+          low[j][r] = pair16(fmaf((float)back[0], -1.0f, x), fmaf((float)back[1], -1.0f, y));
+        }
+#pragma unroll
+      for (int h = 0; h < H; h += 2) {
+        v4u a, b;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const int of = (h + i / 2) / L, j = (h + i / 2) % L;
+          a[i] = CP == 1 || copy == of ? high[j][i % 2] : 0u;
+          b[i] = CP == 1 || copy == of ? low[j][i % 2] : 0u;
+        }
+#pragma unroll
+        for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
+          const uint32_t w0 = v[h][c], w1 = v[h + 1][c], u0 = w0 >> 8, u1 = w1 >> 8;
+          const v4u even{codes16<TWO>(w0, kLow), codes16<TWO>(u0, kLow), codes16<TWO>(w1, kLow), codes16<TWO>(u1, kLow)};
+          const v4u odd{codes16<TWO>(w0, kHigh), codes16<TWO>(u0, kHigh), codes16<TWO>(w1, kHigh), codes16<TWO>(u1, kHigh)};
+          o[2 * c] = mfma16(even, b, o[2 * c]);
+          o[2 * c + 1] = mfma16(odd, b, o[2 * c + 1]);
+          o[2 * c] = mfma16(even, a, o[2 * c]);
+          o[2 * c + 1] = mfma16(odd, a, o[2 * c + 1]);
+        }
       }
     }
     next_v();
   }
 
-  // The row's whole sum, and its sums of P m, in all four quarters.
+  // The column's whole sum, and its sums of P m, in all four quarters.
   __device__ __forceinline__ float total() {
 #pragma unroll
     for (int g = 0; g < G; g++) {
@@ -291,23 +356,25 @@ struct Rows4 {
   }
 };
 
-// Waves that a SIMD's 512 registers a lane hold without spilling: results, q and
-// codes, scales and minima, and about 45 others.
-template <int NC, int GC, bool TWO>
+// Waves that a SIMD's 512 registers a lane hold without spilling: results, q,
+// codes, the tile's products, scales and minima, and some 55 others.
+template <int NC, int GC, bool TWO, int CP>
 constexpr int waves_a_simd4() {
-  constexpr int n = NC * (8 + (TWO ? 8 : 4) + 4) + 16 * ((NC + GC - 1) / GC) + 45;
-  return n <= 128 ? 4 : n <= 168 ? 3 : n <= 250 ? 2 : 1;
+  typedef Rows4<NC, GC, TWO, CP> A;
+  constexpr int n = NC * (8 + (TWO ? 8 : 4) + 2 * A::H) + A::FEW + A::G * (4 * A::L + 8 * A::L) + 55;
+  return n <= 130 ? 4 : n <= 170 ? 3 : n <= 300 ? 2 : 1;
 }
 
 // Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.x, part
-// blockIdx.y of its tiles of 32 tokens, a tile a wave at a time: a tile's halves
-// lie in one page each, whose number all lanes look up alike.
-template <int NC, int GC, bool TWO>
-__global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO>())) void kv4_attention_parts(Attend4Args a) {
-  typedef Rows4<NC, GC, TWO> A;
-  constexpr int DP = A::DP;
+// blockIdx.y of its tiles, a tile a wave at a time. EIGHTS: heads are of a
+// multiple of 8 dims.
+template <int NC, int GC, bool TWO, int CP, bool EIGHTS>
+__global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) void kv4_attention_parts(Attend4Args a) {
+  typedef Rows4<NC, GC, TWO, CP> A;
+  constexpr int DP = A::DP, H = A::H, KEYS = 16 * H, R = 16 / CP, kTable = 64 / H;
   __shared__ float lds_o[kWaves4][16][DP + 4];
   __shared__ float lds_b[kWaves4][16], lds_l[kWaves4][16];
+  __shared__ __attribute__((aligned(16))) char lds_few[kWaves4][256 * A::FEW];
   __shared__ int lds_bad;
   const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -316,7 +383,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO>())) void 
   const int rows = min(16, kv * per + per - h0);
   const int length = a.c.lengths[b];
   const bool too_long = length > a.c.table_width * a.c.page_size;
-  const Seen s = seen_of(too_long ? 0 : length, a.window, a.sinks, kKeys4);
+  const Seen s = seen_of(too_long ? 0 : length, a.window, a.sinks, KEYS);
   const int each = tiles_a_part(s.tiles, a.each, a.splits);
   const int begin = blockIdx.y * each, end = min(begin + each, s.tiles);
   if (begin >= end && blockIdx.y) return;  // part 0 of an empty text writes its zeros
@@ -324,63 +391,75 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO>())) void 
   __syncthreads();
 
   A at;
-  at.start(a.q, b * a.q_stride + (long)(h0 + min(col, rows - 1)) * a.c.dim, a.type, a.c.dim, quarter, a.scale, a.turn);
+  at.template start<EIGHTS>(a.q, b * a.q_stride + (long)(h0 + min(col % R, rows - 1)) * a.c.dim, a.type, a.c.dim, quarter,
+                            a.scale, a.turn);
   const int *table = a.c.table + b * a.c.table_width;
   const char *data = a.c.data + (long)kv * a.c.chunk;
   bool bad = false;
-  auto tile_key = [&](int t) { return t < s.sink_tiles ? t * kKeys4 : s.first + (t - s.sink_tiles) * kKeys4; };
-  // Where the 16 tokens from k lie, some of which are seen if `wanted`. (A page
-  // that does not exist is read as page 0, and the text's result is NaN.)
-  struct Place {
-    const char *page;
-    int slot;
-  };
-  auto find = [&](int k, bool wanted) -> Place {
-    int page = -1, slot = 0;
-    if (wanted) {
-      const int n = a.c.by_page(k);
-      page = table[n];
-      slot = k - n * a.c.page_size;
-      bad |= page < 0 || page >= a.c.pages;
+  auto tile_key = [&](int t) { return t < s.sink_tiles ? t * KEYS : s.first + (t - s.sink_tiles) * KEYS; };
+  const int whole0 = s.sink_tiles + (s.first < s.low ? 1 : 0), whole1 = s.sink_tiles + (s.length - s.first) / KEYS;
+  const uint32_t k_at = (col * 4 + quarter) * 4 * NC, v_at = a.c.at_v + lane * 4 * NC;
+  // This lane's share of a tile's scales and minima: of 16 keys, a plane, a piece.
+  const int half = lane / kTable, plane = lane / (16 / H) % 4;
+  const uint32_t few_at = (plane == 0 ? a.c.at_ks : plane == 1 ? a.c.at_km : plane == 2 ? a.c.at_vs : a.c.at_vm) +
+                          lane % (16 / H) * 4 * A::FEW;
+  char *few = lds_few[wave];
+  // A wave takes each fourth tile. Of its next ones, each lane finds where 16
+  // keys lie: the page's offset and the first token's slot in it. (A page that
+  // does not exist is read as page 0, and the text's result is NaN.)
+  for (int t0 = begin + wave; t0 < end; t0 += kTable * kWaves4) {
+    long my_page = 0;
+    int my_slot = 0;
+    {
+      const int t = t0 + lane / H * kWaves4, k = tile_key(min(t, end - 1)) + lane % H * 16;
+      // Of 16 neighbours some is seen if one is below the length and above the window's start, or below the sinks' end.
+      if (t < end && k < s.length && (k + 15 >= s.low || k < s.sinks)) {
+        const int n = a.c.by_page(k), page = table[n];
+        if (page >= 0 && page < a.c.pages)
+          my_page = page * a.c.page_stride, my_slot = k - n * a.c.page_size;
+        else
+          bad = true;
+      }
     }
-    const bool there = page >= 0 && page < a.c.pages;
-    return {data + (there ? page * a.c.page_stride : 0), there ? slot : 0};
-  };
-  struct Places {
-    Place half[2];
-  };
-  // Of 16 neighbours some is seen if one is below the length and above the window's start, or below the sinks' end.
-  auto find_tile = [&](int t) -> Places {
-    const int k = tile_key(min(t, end - 1));
-    return {find(k, k < s.length && (k + 15 >= s.low || k < s.sinks)),
-            find(k + 16, k + 16 < s.length && (k + 31 >= s.low || k + 16 < s.sinks))};
-  };
-  const int whole0 = s.sink_tiles + (s.first < s.low ? 1 : 0), whole1 = s.sink_tiles + (s.length - s.first) / kKeys4;
-  int t = begin + wave;
-  if (t < end) {
-    Places at_now = find_tile(t);
+    auto page_of = [&](int i) {
+      return data + (long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(my_page >> 32), i) << 32 |
+                           (uint32_t)__builtin_amdgcn_readlane((int)my_page, i));
+    };
+    auto slot_of = [&](int i) { return __builtin_amdgcn_readlane(my_slot, i); };
+    auto load_codes = [&](uint32_t (&n)[H][NC], int i, uint32_t at_) {
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      at.load_k(h, at_now.half[h].page, at_now.half[h].slot, a.c, lane);
-      at.load_v(h, at_now.half[h].page, at_now.half[h].slot, a.c, lane);
-    }
-    for (; t < end; t += kWaves4) {
-      // (Past the last tile the last one again.)
-      const Places next = find_tile(t + kWaves4);
-      const int k = tile_key(t);
-      at.use([&](int i) { return k + i < s.length && (k + i >= s.low || k + i < s.sinks); }, t < whole0 || t >= whole1,
-             quarter,
+      for (int h = 0; h < H; h++)
+        __builtin_memcpy(n[h], page_of(H * i + h) + slot_of(H * i + h) * 16 * NC + at_, 4 * NC);
+    };
+    // A lane's share of a tile's scales and minima.
+    auto load_few = [&](int i) {
+      const int from = H * i + half;
+      const long o = (long)((uint64_t)(uint32_t)__shfl((int)(my_page >> 32), from) << 32 | (uint32_t)__shfl((int)my_page, from));
+      return words_at<A::FEW>(data + o + (uint32_t)(__shfl(my_slot, from) * 2 * A::G) + few_at);
+    };
+    auto put_few = [&](const Words<A::FEW> &w) {
+      __builtin_amdgcn_wave_barrier();  // (a wave's LDS operations are done in order)
+      *(Words<A::FEW> *)(few + lane * 4 * A::FEW) = w;
+      __builtin_amdgcn_wave_barrier();
+    };
+    const int n = min((end - t0 + kWaves4 - 1) / kWaves4, kTable);
+    Words<A::FEW> share = load_few(0);
+    load_codes(at.k, 0, k_at);
+    load_codes(at.v, 0, v_at);
+    put_few(share);
+    for (int i = 0; i < n; i++) {
+      const int next = min(i + 1, n - 1);  // (the last one again, rather than loads behind a branch, which would be waited for)
+      share = load_few(next);
+      const int t = t0 + i * kWaves4, k = tile_key(t);
+      at.use(few, [&](int j) { return k + j < s.length && (k + j >= s.low || k + j < s.sinks); }, t < whole0 || t >= whole1,
+             lane, [&] { load_codes(at.k, next, k_at); },
              [&] {
-#pragma unroll
-               for (int h = 0; h < 2; h++) at.load_k(h, next.half[h].page, next.half[h].slot, a.c, lane);
-             },
-             [&] {
-#pragma unroll
-               for (int h = 0; h < 2; h++) at.load_v(h, next.half[h].page, next.half[h].slot, a.c, lane);
+               put_few(share);
+               load_codes(at.v, next, v_at);
              });
     }
   }
-  // The waves' parts, joined.
+  // The waves' columns, joined.
   if (bad) lds_bad = 1;
   const float l = at.total();
   if (quarter == 0) lds_b[wave][col] = at.base, lds_l[wave][col] = l;
@@ -391,64 +470,78 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO>())) void 
 #pragma unroll
       for (int r = 0; r < 4; r++)
         lds_o[wave][col][32 * c + 2 * (4 * quarter + r) + odd] =
-            fmaf(at.o[2 * c + odd][r], odd ? 0x1p5f : 0x1p9f, at.om[c / GC]);
+            fmaf(at.o[2 * c + odd][r], TWO ? (odd ? 0x1p5f : 0x1p9f) : (odd ? 0x1p20f : 0x1p24f), at.om[c / GC]);
   __syncthreads();
+  // A column's factor, and a row's sum: a wave's columns in 16 neighbouring lanes.
+  {
+    const int row = col % R;
+    float bw = lane < 16 * kWaves4 ? lds_b[lane / 16][col] : -INFINITY, base_ = bw;
+    auto all = [&](float v, auto join) {
+#pragma unroll
+      for (int o = R; o < 64; o *= 2) v = join(v, __shfl_xor(v, o));
+      return v;
+    };
+    base_ = all(base_, [](float x, float y) { return fmaxf(x, y); });
+    // (A base is -infinity where the column had no key; NaN where q is not finite.)
+    const float f = bw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bw - base_);
+    const float sum = all(f * lds_l[lane / 16][col], [](float x, float y) { return x + y; });
+    __syncthreads();
+    if (wave == 0) {
+      lds_b[lane / 16][col] = f;
+      if (lane < R) lds_l[0][row] = lds_bad ? __uint_as_float(0x7fc00000u) : sum, lds_l[1][row] = base_;
+    }
+    __syncthreads();
+  }
   const bool split = a.splits > 1;
   for (int i = threadIdx.x; i < rows * DP; i += 64 * kWaves4) {
     const int row = i / DP, d = i % DP;
     if (d >= a.c.dim) continue;
-    float base = -INFINITY, sum = 0.0f, o = 0.0f;
+    const float sum = lds_l[0][row];
+    float o = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves4; w++) base = fmaxf(base, lds_b[w][row]);
-#pragma unroll
-    for (int w = 0; w < kWaves4; w++) {
-      // (A base is -infinity where the wave had no key; NaN where q is not finite.)
-      const float f = lds_b[w][row] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lds_b[w][row] - base);
-      sum += f * lds_l[w][row];
-      o += f * lds_o[w][row][d];
-    }
-    if (lds_bad) sum = o = __uint_as_float(0x7fc00000u);
+    for (int w = 0; w < kWaves4 * CP; w++)
+      o = fmaf(lds_b[w / CP][w % CP * R + row], lds_o[w / CP][w % CP * R + row][d], o);
     if (split) {
       float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + blockIdx.y) * (a.c.dim + 2);
       p[d + 2] = o;
-      if (d == 0) p[0] = base, p[1] = sum;
+      if (d == 0) p[0] = lds_l[1][row], p[1] = sum;
     } else {
       put_at(a.y, b * a.y_stride + (long)(h0 + row) * a.c.dim + d, a.type, sum == 0.0f ? 0.0f : o / sum);
     }
   }
 }
 
-template <int NC, int GC, bool TWO>
+template <int NC, int GC, bool TWO, int CP>
 hipError_t launch_parts4(const Attend4Args &a, hipStream_t s) {
   const int per = a.heads / a.c.heads;
   const dim3 grid(a.c.heads * ((per + 15) / 16), a.splits, a.batch), block(64 * kWaves4);
-  return launch_kernel(kv4_attention_parts<NC, GC, TWO>, grid, block, 0, s, a);
+  if (a.c.dim % 8 == 0) return launch_kernel(kv4_attention_parts<NC, GC, TWO, CP, true>, grid, block, 0, s, a);
+  return launch_kernel(kv4_attention_parts<NC, GC, TWO, CP, false>, grid, block, 0, s, a);
 }
 
 // Groups of a whole head, of 32 and of 64 (where a head has more than one).
-template <int NC, bool TWO>
+template <int NC, bool TWO, int CP>
 hipError_t launch_groups4(const Attend4Args &a, hipStream_t s) {
   if constexpr (NC > 1) {
-    if (a.c.group == 32) return launch_parts4<NC, 1, TWO>(a, s);
+    if (a.c.group == 32) return launch_parts4<NC, 1, TWO, CP>(a, s);
   }
   if constexpr (NC > 2) {
-    if (a.c.group == 64) return launch_parts4<NC, 2, TWO>(a, s);
+    if (a.c.group == 64) return launch_parts4<NC, 2, TWO, CP>(a, s);
   }
-  return launch_parts4<NC, NC, TWO>(a, s);
+  return launch_parts4<NC, NC, TWO, CP>(a, s);
 }
 
-template <bool TWO>
+template <bool TWO, int CP>
 hipError_t launch_attention4(const Attend4Args &a, hipStream_t s) {
-  hipError_t e = hipErrorInvalidValue;
   switch (a.c.nc) {
-    case 1: e = launch_groups4<1, TWO>(a, s); break;
-    case 2: e = launch_groups4<2, TWO>(a, s); break;
-    case 3: e = launch_groups4<3, TWO>(a, s); break;
-    case 4: e = launch_groups4<4, TWO>(a, s); break;
-    case 6: e = launch_groups4<6, TWO>(a, s); break;
-    case 8: e = launch_groups4<8, TWO>(a, s); break;
+    case 1: return launch_groups4<1, TWO, CP>(a, s);
+    case 2: return launch_groups4<2, TWO, CP>(a, s);
+    case 3: return launch_groups4<3, TWO, CP>(a, s);
+    case 4: return launch_groups4<4, TWO, CP>(a, s);
+    case 6: return launch_groups4<6, TWO, CP>(a, s);
+    case 8: return launch_groups4<8, TWO, CP>(a, s);
   }
-  return e != hipSuccess || a.splits == 1 ? e : launch_kv4_join(a, s);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace ppocr

@@ -1,0 +1,6 @@
+// Attention over a cache in 4 bits: f32 queries, two columns a query head.
+#include "attend4.hpp"
+
+namespace ppocr {
+template hipError_t launch_attention4<true, 2>(const Attend4Args &, hipStream_t);
+}  // namespace ppocr

@@ -206,8 +206,7 @@ int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cach
   a.part = static_cast<float *>(workspace);
   const OnDevice on{hipStream_t(stream)};
   if (on.e != hipSuccess) return fail.hip(what, on.e);
-  return fail.hip(what, type == PPOCR_F32 ? launch_kv4_attention_32(a, hipStream_t(stream))
-                                          : launch_kv4_attention_16(a, hipStream_t(stream)));
+  return fail.hip(what, launch_kv4_attention(a, hipStream_t(stream)));
 }
 
 size_t ppocr_hip_beam_select_workspace(size_t batch, size_t beams, size_t vocab, size_t keep) {
