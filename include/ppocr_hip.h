@@ -406,8 +406,7 @@ size_t ppocr_hip_kv4_page_bytes(size_t page_size, size_t heads, size_t dim, size
  *   n = round((x - minimum) * (1 / scale)) within 0 .. 15 (0 where scale is 0)
  * over a group's dims. Values past F16's range are held at its ends; a group
  * with an infinity or NaN has the scale NaN, minimum 0 and codes 0, and what is
- * read of it is NaN. Four neighbouring places (0 .. 3, 4 .. 7, ...) share words of V:
- * appends that run at the same time must not write to the same four. */
+ * read of it is NaN. Places of a text next to those that are written keep every bit. */
 int ppocr_hip_kv4_append(const void *q, size_t q_stride, void *q_out, size_t q_out_stride, size_t heads, const void *k,
                          size_t k_stride, const void *v, size_t v_stride, const ppocr_kv4_cache *cache,
                          const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
