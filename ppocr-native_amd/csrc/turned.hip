@@ -7,67 +7,91 @@
 namespace ppocr {
 namespace {
 
-// A new token a workgroup: its row's loads need no more than its number, so
-// they are on their way while the waves find its text, place and angles.
-// Memory bound; at a token a text bound by that chain of waits.
-template <int T, int N>
+constexpr long kNoText = -(1L << 40);  // below every token's number
+
+// TOKENS rows a workgroup: their loads need no more than the rows' numbers, so
+// they are on their way while waves find the texts, places and angles; a thread
+// has the same unit of each row. Memory bound; at a token a text bound by that
+// chain of waits.
+template <int T, int N, int TOKENS>
 __global__ __launch_bounds__(512) void kv_append_turned(TurnedAppendArgs g) {
   typedef num_t<T> V;
-  __shared__ v2f cs[128];
+  __shared__ v2f cs[TOKENS][128];
+  __shared__ long place[TOKENS][2];  // of a row: the token's number in its text, or -1; where it goes, or -1
   const AppendArgs &a = g.a;
   const TurnArgs &t = g.t;
   const int heads = t.heads, kv = a.c.heads, items = (heads + 2 * kv) * g.units, half = t.rotary / 2;
-  for (long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    int b = (int)row;
-    if (a.starts) b = last_not_past(a.batch + 1, row, [&](int i) { return (long)a.starts[i]; });
+  const long row0 = ((long)blockIdx.y * gridDim.x + blockIdx.x) * TOKENS;
+
+  // Item i: a unit of q's heads, then of k's, then of v's.
+  V p[TOKENS][N], r[TOKENS][N];
+  Unit o;
+  int h;
+  auto load = [&](int i) {
+    h = g.by_unit(i);
+    o = unit_of<N>(i - h * g.units, a.c.dim, t.rotary, t.pairs);
+    const int in = h < heads ? h : h < heads + kv ? h - heads : h - heads - kv;
+    const V *from = h < heads ? (const V *)t.q : h < heads + kv ? (const V *)a.k : (const V *)a.v;
+    const long stride = h < heads ? t.q_stride : h < heads + kv ? a.k_stride : a.v_stride;
+    const int d2 = o.d2 < a.c.dim ? o.d2 : o.d1;
+#pragma unroll
+    for (int j = 0; j < TOKENS; j++) {
+      const V *at = from + min(row0 + j, a.rows - 1) * stride + (long)in * a.c.dim;
+      __builtin_memcpy(p[j], at + o.d1, sizeof p[j]);
+      __builtin_memcpy(r[j], at + d2, sizeof r[j]);
+    }
+  };
+  load(min((int)threadIdx.x, items - 1));
+
+  // A wave's rows: where they go.
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
+  for (int j = wave; j < TOKENS; j += waves) {
+    const long row = row0 + j;
+    long at = -1, to = -1;
+    int b = row < a.rows ? (int)row : -1;
+    if (a.starts && b >= 0) b = last_not_past(a.batch + 1, row, [&](int i) { return (long)a.starts[i]; });
     b = __builtin_amdgcn_readfirstlane(b);
-
-    // Item i: a unit of q's heads, then of k's, then of v's.
-    V p[N], r[N];
-    Unit o;
-    int h;
-    auto load = [&](int i) {
-      h = g.by_unit(i);
-      o = unit_of<N>(i - h * g.units, a.c.dim, t.rotary, t.pairs);
-      const V *from = h < heads        ? (const V *)t.q + row * t.q_stride + (long)h * a.c.dim
-                      : h < heads + kv ? (const V *)a.k + row * a.k_stride + (long)(h - heads) * a.c.dim
-                                       : (const V *)a.v + row * a.v_stride + (long)(h - heads - kv) * a.c.dim;
-      __builtin_memcpy(p, from + o.d1, sizeof p);
-      __builtin_memcpy(r, from + (o.d2 < a.c.dim ? o.d2 : o.d1), sizeof r);
-    };
-    int i = threadIdx.x;
-    if (i < items) load(i);
-
-    if (b < 0 || b >= a.batch) continue;
-    long first = b, last = b + 1L;
-    if (a.starts) first = a.starts[b], last = a.starts[b + 1];
-    if (row < first || row >= last) continue;
-    const int end = a.c.lengths[b];
-    const long at = end - (last - row);  // (below end, an int)
-    long to = -1;
-    if (at >= 0) {
-      const int slot = a.c.by_page((int)at);
-      if (slot < a.c.table_width) {
-        const int page = a.c.table[b * a.c.table_width + slot];
-        if (page >= 0 && page < a.c.pages)
-          to = page * a.c.page_stride + (at - (long)slot * a.c.page_size) * a.c.token_stride;
+    if (b >= 0 && b < a.batch) {
+      long first = b, last = b + 1L;
+      if (a.starts) first = a.starts[b], last = a.starts[b + 1];
+      const int end = a.c.lengths[b];
+      if (row >= first && row < last) {
+        at = end - (last - row);  // (below end, an int)
+        const int slot = at >= 0 ? a.c.by_page((int)at) : a.c.table_width;
+        if (slot < a.c.table_width) {
+          const int page = a.c.table[b * a.c.table_width + slot];
+          if (page >= 0 && page < a.c.pages)
+            to = page * a.c.page_stride + (at - (long)slot * a.c.page_size) * a.c.token_stride;
+        }
+      } else {
+        b = -1;
       }
     }
-    const double position = t.positions ? (double)t.positions[row] : (double)at;
-    if (threadIdx.x < half) cs[threadIdx.x] = cosine_sine(position * (double)t.freqs[threadIdx.x]);
-    __syncthreads();
-    for (; i < items; i += blockDim.x) {
-      if (i != threadIdx.x) load(i);
-      if (h < heads + kv && o.turned) turn_unit<T, N>(p, r, cs, o, t.rotary, t.pairs);
-      V *into = h < heads        ? (V *)t.q_out + row * t.q_out_stride + (long)h * a.c.dim
-                : h < heads + kv ? (V *)a.c.k + to + (h - heads) * a.c.head_stride
-                                 : (V *)a.c.v + to + (h - heads - kv) * a.c.head_stride;
-      if (h < heads || to >= 0) {
-        __builtin_memcpy(into + o.d1, p, sizeof p);
-        if (o.d2 < a.c.dim) __builtin_memcpy(into + o.d2, r, sizeof r);
+    if (b < 0 || b >= a.batch) at = kNoText;
+    if (threadIdx.x % 64 == 0) place[j][0] = at, place[j][1] = to;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < TOKENS * half; i += blockDim.x) {
+    const int j = TOKENS == 1 ? 0 : g.by_half(i), n = i - j * half;
+    const double at = t.positions ? (double)t.positions[min(row0 + j, a.rows - 1)] : (double)place[j][0];
+    cs[j][n] = cosine_sine(at * (double)t.freqs[n]);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < items; i += blockDim.x) {
+    if (i != threadIdx.x) load(i);
+    const bool query = h < heads, turned = h < heads + kv && o.turned;
+    V *into = query ? (V *)t.q_out + row0 * t.q_out_stride + (long)h * a.c.dim
+              : h < heads + kv ? (V *)a.c.k + (h - heads) * a.c.head_stride
+                               : (V *)a.c.v + (h - heads - kv) * a.c.head_stride;
+#pragma unroll
+    for (int j = 0; j < TOKENS; j++) {
+      if (turned) turn_unit<T, N>(p[j], r[j], cs[j], o, t.rotary, t.pairs);
+      const long to = query ? (place[j][0] == kNoText ? -1 : j * t.q_out_stride) : place[j][1];
+      if (to >= 0) {
+        __builtin_memcpy(into + to + o.d1, p[j], sizeof p[j]);
+        if (o.d2 < a.c.dim) __builtin_memcpy(into + to + o.d2, r[j], sizeof r[j]);
       }
     }
-    if (gridDim.x < a.rows) __syncthreads();  // before the next token's angles
   }
 }
 
@@ -78,8 +102,14 @@ hipError_t launch_turned(TurnedAppendArgs a, hipStream_t s) {
   // As many threads as units, or as few as share them evenly; at least one an angle.
   const long items = (a.t.heads + 2L * a.a.c.heads) * a.units, rounds = (items + 511) / 512;
   const int threads = std::max(int(((items + rounds - 1) / rounds + 63) / 64 * 64), 128);
-  const dim3 grid(unsigned(std::min(a.a.rows, 1L << 20))), block(threads);
-  return launch_kernel(kv_append_turned<T, N>, grid, block, 0, s, a);
+  const dim3 block(threads);
+  a.by_half = Divide(std::max(a.t.rotary / 2, 1));
+  // Four rows a workgroup where that leaves every compute unit one.
+  const bool four = N > 1 && a.a.rows >= 4 * 256;
+  const long groups = four ? (a.a.rows + 3) / 4 : a.a.rows, wide = std::min(groups, 1L << 20);
+  const dim3 grid(unsigned(wide), unsigned((groups + wide - 1) / wide));
+  return four ? launch_kernel(kv_append_turned<T, N, N == 1 ? 1 : 4>, grid, block, 0, s, a)
+              : launch_kernel(kv_append_turned<T, N, 1>, grid, block, 0, s, a);
 }
 
 }  // namespace

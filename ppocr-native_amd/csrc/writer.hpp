@@ -22,7 +22,7 @@ struct TurnedAppendArgs {
   AppendArgs a;
   TurnArgs t;
   int units;  // of two pieces of a head
-  Divide by_unit;
+  Divide by_unit, by_half;
 };
 hipError_t launch_kv_append_turned(const TurnedAppendArgs &a, int type, hipStream_t s);
 
