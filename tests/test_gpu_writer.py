@@ -480,3 +480,61 @@ def test_cache4_far_offsets():
         kk, vv = ([np.array([x[part][j][h] for x in parts]) for j in (0, 1)] for part in (0, 1))
         want, size, reach = W.attend4(q[0, h].astype(np.float64), kk, vv, np.ones(70, bool), 0.1)
         R.close(got[0, h], want, W.attend4_bound(want, size, reach, D.F32))
+
+
+# ---------------------------------------------- many rows, and long texts
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads,kv,dim,rotary,pairs", [(4, 2, 64, 64, False), (5, 1, 40, 16, True), (70, 2, 128, 64, False),
+                                                       (2, 1, 15, 14, False)])
+def test_rotated_append_many_rows(t, heads, kv, dim, rotary, pairs):
+    # More rows than the compute units have: odd counts, texts that end between two rows of a workgroup.
+    run_rotated(t, [1100, 3, 9, 200], [1023, 1, 0, 3], 16, heads, kv, dim, rotary, pairs, "heads", in_place=True)
+    run_rotated(t, [600, 701], [600, 423], 48, heads, kv, dim, rotary, pairs, gap=8, far=1000, queries=False)
+
+
+def test_rotated_append_many_rows_of_no_text():
+    # Rows before the first text, between those of a start that goes back, and behind the last are left.
+    rng = np.random.default_rng(4)
+    rows, dim = 1101, 32
+    p = R.Pages(rng, [600, 600], 16, 1, dim, D.F16)
+    cache = p.upload()
+    k = R.stored(rng.normal(0, 1, (rows, 1, dim)), D.F16)
+    dk, dl, df = R.on_gpu(k), R.on_gpu(np.array([500, 510], np.int32)), R.on_gpu(W.frequencies(dim))
+    ds, do = R.on_gpu(np.array([3, 503, 1013], np.int32)), R.on_gpu(np.full(k.shape, 7, np.float16))
+    print("rotated append, many rows of no text", flush=True)
+    D.kv_append_rotated(dk.addr, dk.addr, cache, p.gpu_table.addr, p.width, dl.addr, 2, rows, freqs=df.addr, rotary=dim,
+                        starts=ds.addr, q=dk.addr, q_out=do.addr, heads=1)
+    synchronize()
+    out = R.back(do, np.float16, k.shape)
+    assert (out[:3] == 7).all() and (out[1013:] == 7).all()
+    places = np.concatenate([np.arange(500), np.arange(510)])
+    want, size = W.turned(k[3:1013].astype(np.float64), places, W.frequencies(dim), dim, False)
+    R.close(out[3:1013].astype(np.float64), want, W.turned_bound(want, size, D.F16))
+    for i, (b, at) in enumerate([(0, i) for i in range(500)] + [(1, i) for i in range(510)]):
+        p.put(b, at, out[3 + i], k[3 + i])
+    for got, held in zip(p.gpu, p.host):
+        assert np.array_equal(R.back(got, np.float16, held.shape).view(np.uint16), held.view(np.uint16))
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim,group", DIMS4)
+def test_attend4_eight_heads(t, dim, group):
+    # Five to eight query heads a key head: two columns each.
+    run_attend4([1, 0, 130, 16, 33], 16, 16, 2, dim, group, t)
+    run_attend4([250, 31], 48, 5, 1, dim, group, t, work=0, gap=5)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim,group", DIMS4)
+def test_attend4_sixteen_heads(t, dim, group):
+    run_attend4([1, 0, 130, 16, 33], 16, 11, 1, dim, group, t)
+    run_attend4([250, 31], 48, 20, 1, dim, group, t, work=0, gap=5)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads", [2, 6, 9])
+def test_attend4_long_without_parts(t, heads):
+    # More tokens than a workgroup looks pages up for at once, in one part.
+    run_attend4([4097, 8300], 16, heads, 1, 32, 0, t, work=0)
+    run_attend4([9000], 16, heads, 1, 32, 0, t, 4500, 20, work=0)
