@@ -8,6 +8,8 @@
 // results do not depend on how a library rounds its f32 functions. A token's
 // angles are computed once, into LDS, for all of its heads.
 #pragma once
+#include <type_traits>
+
 #include "writer.hpp"
 
 namespace ppocr {
@@ -41,6 +43,18 @@ __device__ __forceinline__ v2f cosine_sine(double a) {
   const int turn = (int)(long)n & 3;  // quarter turns
   const float fc = (float)(turn & 1 ? s : c), fs = (float)(turn & 1 ? c : s);
   return v2f{turn == 1 || turn == 2 ? -fc : fc, turn >= 2 ? -fs : fs};
+}
+
+// Stores of values that are not looked at again soon, as a stream.
+template <class V, int N>
+__device__ __forceinline__ void stream_out(V *p, const V (&v)[N]) {
+  constexpr int kBytes = N * sizeof(V), kWord = kBytes < 16 ? kBytes : 16;
+  typedef std::conditional_t<kWord == 16, v4u, std::conditional_t<kWord == 8, v2u, std::conditional_t<kWord == 4, uint32_t, uint16_t>>> Word;
+  typedef Word __attribute__((aligned(sizeof(V)))) Loose;  // (a caller's rows are aligned to their values only)
+  Word w[kBytes / kWord];
+  __builtin_memcpy(w, v, kBytes);
+#pragma unroll
+  for (int i = 0; i < kBytes / kWord; i++) __builtin_nontemporal_store(w[i], (Loose *)p + i);
 }
 
 // The last of `n` not decreasing numbers at(0), at(1), ... that is not past

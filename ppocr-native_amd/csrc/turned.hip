@@ -88,8 +88,8 @@ __global__ __launch_bounds__(512) void kv_append_turned(TurnedAppendArgs g) {
       if (turned) turn_unit<T, N>(p[j], r[j], cs[j], o, t.rotary, t.pairs);
       const long to = query ? (place[j][0] == kNoText ? -1 : j * t.q_out_stride) : place[j][1];
       if (to >= 0) {
-        __builtin_memcpy(into + to + o.d1, p[j], sizeof p[j]);
-        if (o.d2 < a.c.dim) __builtin_memcpy(into + to + o.d2, r[j], sizeof r[j]);
+        stream_out(into + to + o.d1, p[j]);
+        if (o.d2 < a.c.dim) stream_out(into + to + o.d2, r[j]);
       }
     }
   }

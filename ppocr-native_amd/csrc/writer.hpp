@@ -49,7 +49,8 @@ struct Append4Args {
   int batch;
   TurnArgs t;
   int units;
-  Divide by_unit, by_items, by_half;  // of a head, of a row; the turned pairs
+  int teams;                // of threads, for the queries
+  Divide by_unit, by_half;  // of a head; the turned pairs
 };
 hipError_t launch_kv4_append(const Append4Args &a, int type, hipStream_t s);
 
