@@ -224,9 +224,9 @@ struct Choice {
 // A chain of waits: the parts' statistics, their logarithm, the candidates (asked
 // for before it), the bound, the list.
 __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Divide by_beams) {
-  __shared__ Choice list[kChoices];
+  __shared__ Choice list[kChoices], chosen[kMostKeep];
   __shared__ double lds_base[kMostBeams], lds_top[kMostBeams], lds_log[kMostBeams];
-  __shared__ Choice lds_least[16], lds_most[16];
+  __shared__ float lds_least[16];
   __shared__ int lds_live[kMostBeams], lds_n[16], lds_groups[16], lds_count;  // live: 0 no candidates, 1 its tokens, 2 ended
   const int b = blockIdx.x, threads = blockDim.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = threads / 64;
   const int each = a.parts * a.keep, all = a.beams * each, count = all + a.beams;  // (at most 2^25)
@@ -243,20 +243,23 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
   for (int i = wave; i < a.beams; i += waves) {
     const long row = (long)b * a.beams + i;
     const float base = a.scores[row];
+    const v2f *stats = (const v2f *)a.stats + row * a.parts;
+    const v2f first = stats[min(lane, a.parts - 1)];  // (asked for with the score)
     int live = !(base > -INFINITY) ? 0 : a.ended && a.ended[row] ? 2 : 1;
     float top = -INFINITY;
     double sum = 0;
     if (live == 1) {
-      for (int k = lane; k < a.parts; k += 64) top = fmaxf(top, a.stats[2 * (row * a.parts + k)]);
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
-      for (int k = lane; k < a.parts; k += 64) {
-        const float t = a.stats[2 * (row * a.parts + k)], s = a.stats[2 * (row * a.parts + k) + 1];
-        sum += t == -INFINITY ? (double)s : (double)s * (double)exp_of(t - top);
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) sum += __longlong_as_double((long long)shuffled((uint64_t)__double_as_longlong(sum), o));
-      // (Not so for a row of -infinity, or with an infinity or a NaN.)
+      if (lane < a.parts) top = first[0];
+      for (int k = lane + 64; k < a.parts; k += 64) top = fmaxf(top, stats[k][0]);
+      for (int o = 1; o < min(a.parts, 64); o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+      top = __shfl(top, 0);
+      auto add = [&](const v2f &of) {
+        sum += of[0] == -INFINITY ? (double)of[1] : (double)of[1] * (double)exp_of(of[0] - top);
+      };
+      if (lane < a.parts) add(first);
+      for (int k = lane + 64; k < a.parts; k += 64) add(stats[k]);
+      for (int o = 1; o < min(a.parts, 64); o *= 2) sum += __longlong_as_double((long long)shuffled((uint64_t)__double_as_longlong(sum), o));
+      // (Of lane 0. Not so for a row of -infinity, or with an infinity or a NaN.)
       if (!(sum > 0) || !(top < INFINITY)) live = 0;
     }
     if (lane == 0) {
@@ -288,41 +291,36 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
     }
     for (int c = (int)threadIdx.x + kAhead * threads; c < count; c += threads) take(choice(c, key_at(c)));
   };
-  Choice best{0, 0};
+  // The bound: of a group of lanes the largest, of groups the least, of scores rounded to 32 bits (which keeps their
+  // order).
+  float best = -INFINITY;
+  bool some = false;
   each_choice([&](const Choice &k) {
-    if (k > best) best = k;
+    if (k.score) best = fmaxf(best, (float)unordered(k.score)), some = true;
   });
-  for (int o = 1; o < lanes; o *= 2) {
-    const Choice other{shuffled(best.score, o), shuffled(best.at, o)};
-    if (other > best) best = other;
-  }
-  const uint64_t any = __ballot(best.score != 0 && lane % lanes == 0);
-  constexpr Choice kPast{~uint64_t(0), ~uint64_t(0)};
-  Choice least = best.score ? best : kPast, most = best;
-  for (int o = lanes; o < 64; o *= 2) {
-    const Choice other{shuffled(least.score, o), shuffled(least.at, o)};
-    if (least > other) least = other;
-    const Choice more{shuffled(most.score, o), shuffled(most.at, o)};
-    if (more > most) most = more;
-  }
-  if (lane == 0) lds_least[wave] = least, lds_most[wave] = most, lds_groups[wave] = __popcll(any);
+  uint64_t has = __ballot(some);
+  for (int o = 1; o < lanes; o *= 2) best = fmaxf(best, __shfl_xor(best, o)), has |= has >> o;
+  // (A group's first lane's bit: whether any of its lanes has one.)
+  uint64_t firsts = 0;
+  for (int o = 0; o < 64; o += lanes) firsts |= uint64_t(1) << o;
+  float least = has >> (lane & ~(lanes - 1)) & 1 ? best : INFINITY;
+  for (int o = lanes; o < 64; o *= 2) least = fminf(least, __shfl_xor(least, o));
+  if (lane == 0) lds_least[wave] = least, lds_groups[wave] = __popcll(has & firsts);
   __syncthreads();
-  int groups = 0;
-  for (int w = 0; w < waves; w++) {
-    if (least > lds_least[w]) least = lds_least[w];
-    if (lds_most[w] > most) most = lds_most[w];
-    groups += lds_groups[w];
-  }
-  if (groups < a.keep) least = Choice{0, 1};  // all there are (none, 0, is not chosen)
-  auto gather = [&] {
+  least = lds_least[min(lane % 16, waves - 1)];
+  int groups = lane % 16 < waves ? lds_groups[lane % 16] : 0;
+#pragma unroll
+  for (int o = 1; o < 16; o *= 2) least = fminf(least, __shfl_xor(least, o)), groups += __shfl_xor(groups, o);
+  const float from = groups < a.keep ? -INFINITY : least;  // (too few groups: all there are)
+  auto gather = [&](auto past) {
     each_choice([&](const Choice &k) {
-      if (!(least > k)) {
+      if (k.score && past(k)) {
         const int at = atomicAdd(&lds_count, 1);
         if (at < kChoices) list[at] = k;
       }
     });
   };
-  gather();
+  gather([&](const Choice &k) { return (float)unordered(k.score) >= from; });
   __syncthreads();
   if (lds_count > kChoices) {  // (the same in all threads)
     auto count_from = [&](const Choice &bound) {
@@ -338,7 +336,8 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
       return n;
     };
     // First by scores alone, then, where too many share one, by positions.
-    uint64_t low = least.score, high = most.score + 1;
+    uint64_t low = 1, high = ordered((double)INFINITY);
+    Choice bound{0, 0};
     bool done = false;
     while (high - low > 1) {
       const uint64_t mid = low + (high - low) / 2;
@@ -348,7 +347,7 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
       } else if (n < a.keep) {
         high = mid;
       } else {
-        least = Choice{mid, 0}, done = true;
+        bound = Choice{mid, 0}, done = true;
         break;
       }
     }
@@ -367,32 +366,30 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
           break;
         }
       }
-      least = Choice{score, below};
+      bound = Choice{score, below};
     }
     if (threadIdx.x == 0) lds_count = 0;
     __syncthreads();
-    gather();
+    gather([&](const Choice &k) { return !(bound > k); });
     __syncthreads();
   }
   const int n = min(lds_count, kChoices);
   const long out = (long)b * a.keep;
-  for (int i = threadIdx.x; i < n; i += threads) {
+  for (int i = wave; i < n; i += waves) {  // a wave ranks one of them against 64 at a time
     const Choice mine = list[i];
     int rank = 0;
-    for (int j = 0; j < n; j++) rank += list[j] > mine;
-    if (rank >= a.keep) continue;
-    const uint64_t at = ~mine.at;
-    const int parent = (int)(at / a.vocab), token = (int)(at - (uint64_t)parent * a.vocab);
-    a.out_scores[out + rank] = (float)unordered(mine.score);
-    a.parents[out + rank] = parent;
-    a.tokens[out + rank] = token;
-    if (a.out_ended) a.out_ended[out + rank] = token == a.end || lds_live[parent] == 2;
+    for (int j = lane; j < n + lane; j += 64) rank += __popcll(__ballot(j < n && list[min(j, n - 1)] > mine));
+    if (lane == 0 && rank < a.keep) chosen[rank] = mine;
   }
-  for (int i = n + threadIdx.x; i < a.keep; i += threads) {
-    a.out_scores[out + i] = -INFINITY;
-    a.parents[out + i] = min(i, a.beams - 1);
-    a.tokens[out + i] = -1;
-    if (a.out_ended) a.out_ended[out + i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.keep; i += threads) {
+    const uint32_t at = i < n ? (uint32_t)~chosen[i].at : 0u;  // (below 2^31)
+    const int parent = (int)(at / (uint32_t)a.vocab), token = (int)(at - (uint32_t)parent * a.vocab);
+    const long to = out + i;
+    a.out_scores[to] = i < n ? (float)unordered(chosen[i].score) : -INFINITY;
+    a.parents[to] = i < n ? parent : min(i, a.beams - 1);
+    a.tokens[to] = i < n ? token : -1;
+    if (a.out_ended) a.out_ended[to] = i < n && (token == a.end || lds_live[parent] == 2);
   }
 }
 
