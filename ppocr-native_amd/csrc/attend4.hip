@@ -1,7 +1,6 @@
 // Attention over a cache in 4 bits: the choice of a kernel, the parts of a split
 // cache and their join.
-#include "seen.hpp"
-#include "writer.hpp"
+#include "parts4.hpp"
 
 namespace ppocr {
 namespace {
@@ -15,9 +14,8 @@ template <int J>
 __global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a, int keys) {
   __shared__ float lds_o[4][256], lds_f[kMostParts4];
   const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  const int length = a.c.lengths[b];
-  const Seen s = seen_of(length > a.c.table_width * a.c.page_size ? 0 : length, a.window, a.sinks, keys);
-  const int each = tiles_a_part(s.tiles, a.each, a.splits);
+  const Seen s = seen4(a, b, keys);
+  const int each = tiles_a_part(s.tiles, each4(a, keys), a.splits);
   const int parts = max(1, (s.tiles + each - 1) / each), dim = a.c.dim, row = dim + 2, far = lane + 64;
   const float *p = a.part + ((long)b * a.heads + head) * a.splits * row;
   const float b0 = lane < parts ? p[(long)lane * row] : -INFINITY, l0 = lane < parts ? p[(long)lane * row + 1] : 0.0f;
@@ -57,13 +55,13 @@ __global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a, int key
 }  // namespace
 
 PagedParts kv4_parts(int batch, int heads, int kv_heads, long longest) {
-  // As long as were 2048 workgroups of it if all texts were the longest: two to
-  // four times what the card holds at once (1024: 92 instead of 76 us for 32 texts
-  // of every length up to 16384; 4096: 78); but of 512 tokens at least, or 128
-  // where that leaves too few for the card. A text of 512 is done without a join.
+  // At least as long as were 4096 workgroups of it if all texts were the longest
+  // (with a thousand texts or fewer the device makes them longer, by the lengths
+  // that it has); but of 512 tokens at least, or 128 where that leaves too few for
+  // the card. A text of 512 is done without a join.
   const int per = heads / kv_heads, keys = 16 * halves4(copies4(per)), least = 512 / keys, few = 128 / keys;
   const long groups = (long)batch * kv_heads * ((per + 15) / 16), tiles = (longest + keys - 1) / keys + 2;
-  long each = (tiles * groups + 2047) / 2048;
+  long each = (tiles * groups + 4095) / 4096;
   if (each < least) {
     const long fill = (tiles * groups + 511) / 512;
     each = tiles <= least + 1 ? least + 1 : fill < few ? few : fill < least ? fill : least;
@@ -73,7 +71,7 @@ PagedParts kv4_parts(int batch, int heads, int kv_heads, long longest) {
   return {int(splits < 1 ? 1 : splits), int(each)};
 }
 
-hipError_t launch_kv4_attention(const Attend4Args &a, hipStream_t s) {
+hipError_t launch_kv4_attention(Attend4Args a, hipStream_t s) {
   const int copies = copies4(a.heads / a.c.heads);
   const bool two = a.type == PPOCR_F32;
   const hipError_t e = copies == 4   ? (two ? launch_attention4<true, 4>(a, s) : launch_attention4<false, 4>(a, s))

@@ -8,27 +8,32 @@
 // so that the products are of codes, which f16 holds exactly, and scales and
 // minima meet sums of 32 bits: nothing of the cache is rounded.
 //
-// Four bits are an f16 as they are: bits 0 .. 3 of a 16-bit half are n 2^-24,
-// bits 4 .. 7 are n 2^-20, both below the smallest normal number. So eight codes
-// of a word cost four masks and one shift. The matrix cores take such numbers,
-// but line products up by exponents that leave out the zeros in front, and cut
-// each product 2^-20 or so below the largest: 16-bit queries' logits are off by
-// some 2^-16 of their terms, an eighth of an f16's half step at most. For f32
-// queries four packed products with 2^15 make them normal numbers, n 2^-9 and
-// n 2^-5. The 2^4 between the two goes into q (K) or into the result (V). K's
-// words have eight dims of a token; V's have two dims of four tokens, so that
-// the same masks give pairs of keys, which is what the product over keys wants.
+// Four bits are an f16 as they are: shifted to bits 6 .. 9 of a 16-bit half they
+// are n 2^-18, below the smallest normal number. So eight codes of a word cost four
+// masks and four shifts. The matrix cores take such numbers, but line a product's
+// terms up by exponents that leave out the zeros in front, and cut them 2^-24 below
+// the largest of those: n q is off by 2^-20 of the largest q, a sum of weights times
+// codes by 2^-20 of the largest weight a tile, where 16-bit results keep 2^-9 or
+// 2^-12 of theirs. (Without the shifts, n 2^-24, it would be 2^-14.) For f32 queries
+// masks of bits 0 .. 3 and 4 .. 7, one shift and four packed products with 2^15 make
+// them normal numbers, n 2^-9 and n 2^-5; the 2^4 between the two goes into q (K) or
+// into the result (V). K's words have eight dims of a token; V's have two dims of four
+// tokens, so that codes of a word side by side are pairs of keys, which is what the
+// product over keys wants.
 //
 // The sixteen columns of a product are a key head's query heads, or where those
 // are eight or four at most, two or four of each: then a column has every second
 // or fourth 16 keys, and its own largest and sum, and a lane half or a quarter of
 // the softmax's work (32 texts to 16384 tokens, four query heads a key head, 8 key
-// heads of 128 in bf16 and groups of 64: 97 us with one column a row).
+// heads of 128 in bf16 and groups of 64, 305 MB: 97 us with one column a row, 73 with
+// four). What else counted there: codes read as a stream (69), parts by the lengths
+// that there are, so that no workgroup is left over for a last, short round (63: 4.8
+// TB/s). The loads alone take 57, the arithmetic alone 51.
 #pragma once
+#include <algorithm>
 #include <type_traits>
 
-#include "seen.hpp"
-#include "writer.hpp"
+#include "parts4.hpp"
 
 namespace ppocr {
 
@@ -37,12 +42,16 @@ constexpr int kWaves4 = 4;
 __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-// The codes that a mask leaves, as they are or as normal numbers.
-template <bool NORMAL>
-__device__ __forceinline__ uint32_t codes16(uint32_t w, uint32_t mask) {
-  const uint32_t n = w & mask;
-  if constexpr (!NORMAL) return n;
-  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, n) * v2h{(_Float16)0x1p15f, (_Float16)0x1p15f});
+// Codes I of a word's halves (of four): n 2^-18, or as normal numbers n 2^-9, and
+// n 2^-5 where I is odd.
+template <bool NORMAL, int I>
+__device__ __forceinline__ uint32_t codes16(uint32_t w) {
+  if constexpr (NORMAL) {
+    const uint32_t n = (I < 2 ? w : w >> 8) & (I % 2 ? 0x00f000f0u : 0x000f000fu);
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, n) * v2h{(_Float16)0x1p15f, (_Float16)0x1p15f});
+  } else {
+    return (I == 0 ? w << 6 : I == 1 ? w << 2 : I == 2 ? w >> 2 : w >> 6) & 0x03c003c0u;
+  }
 }
 __device__ __forceinline__ uint32_t pair16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
@@ -59,6 +68,15 @@ __device__ __forceinline__ Words<N> words_at(const char *p) {
   __builtin_memcpy(&w, p, sizeof w);
   return w;
 }
+// The same as a stream: codes are read once.
+template <int N>
+__device__ __forceinline__ void stream_in(uint32_t (&n)[N], const char *p) {
+  typedef typename Words<N>::Piece Piece;
+  Words<N> w;
+#pragma unroll
+  for (int j = 0; j < int(sizeof w / sizeof(Piece)); j++) w.w[j] = __builtin_nontemporal_load((const Piece *)p + j);
+  __builtin_memcpy(n, &w, sizeof w);
+}
 
 // The state of 16 columns, a wave's worth: a lane has column lane % 16, row lane %
 // (16 / CP) of the query heads, and of each 16 keys the four of quarter lane / 16.
@@ -68,16 +86,18 @@ template <int NC, int GC, bool TWO, int CP>
 struct Rows4 {
   static constexpr int G = (NC + GC - 1) / GC, DP = 32 * NC, E = 2 * NC;
   static constexpr int H = halves4(CP), L = H / CP;  // 16s of keys a tile, and a lane
-  static constexpr int UNIT = TWO ? 9 : 24;  // codes are multiplied as n 2^-UNIT
+  static constexpr int UNIT = TWO ? 9 : 18;  // codes are multiplied as n 2^-UNIT
   static constexpr int FEW = H * G / 2;      // dwords of a tile's scales and minima a lane brings
-  v4u q[TWO ? 2 : 1][NC];  // times 2^e of the row, odd dims 2^-4 of that
+  v4u q[TWO ? 2 : 1][NC];  // times 2^e of the row; TWO: odd dims 2^-4 of that
   float qs[G];             // sums of q over a group, times 2^(e - UNIT)
   v4f o[E];                // lane's column, dim 32 c + 2 (4 quarter + r) + b in o[2 c + b][r]
   float om[G];             // this lane's share of sum P m
-  // Weights are 2^(S scale - base); base is the largest S scale less `up`, and
-  // 2^up times any scale of V is at most 2^15, so that products of the two
-  // fill f16's range. `most`: the largest scale of V so far, as a power of two
-  // above it.
+  // Weights are 2^(S scale - base); base is less by `up` than the largest S scale
+  // was when it was set, and 2^up times any scale of V is at most 2^12, so that
+  // products of the two fill f16's range. Results are scaled anew only where a
+  // product passes that largest by 2^kSlack (or a scale of V `most`, a power of two
+  // above the largest so far): with each new largest it would be in most tiles.
+  static constexpr float kSlack = 3.0f;
   float m, l, base, scale, most, up;
 
   // Eight neighbouring dims of a row from d, as they are stored; past dim some
@@ -145,7 +165,7 @@ struct Rows4 {
       for (int c = 0; c < NC; c++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float x = __builtin_ldexpf(value(raw[c][i]), i & 1 ? e - 4 : e), y = __builtin_ldexpf(value(raw[c][i + 4]), i & 1 ? e - 4 : e);
+          const float x = __builtin_ldexpf(value(raw[c][i]), TWO && i & 1 ? e - 4 : e), y = __builtin_ldexpf(value(raw[c][i + 4]), TWO && i & 1 ? e - 4 : e);
           if constexpr (TWO) {
             const v2h high = __builtin_convertvector(v2f{x, y}, v2h);
             q[0][c][i] = __builtin_bit_cast(uint32_t, high);
@@ -172,18 +192,18 @@ struct Rows4 {
 #pragma unroll
           for (int part = 0; part <= TWO; part++) {
             const uint32_t two = q[part][c][i];
-            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, two), i & 1 ? few_ : one, sum, false);
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(v2h, two), TWO && i & 1 ? few_ : one, sum, false);
           }
       sum += __shfl_xor(sum, 16);
       sum += __shfl_xor(sum, 32);
-      qs[g] = TWO ? sum : sum * 0x1p-15f;
+      qs[g] = TWO ? sum : sum * 0x1p-9f;
       om[g] = 0.0f;
     }
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = v4f{0, 0, 0, 0};
     m = base = -INFINITY;
     l = most = 0.0f;
-    up = 15.0f;
+    up = 15.0f - kSlack;
   }
 
   // A tile's codes: 16s of keys, of which this lane has row lane % 16 of K and the
@@ -208,7 +228,7 @@ struct Rows4 {
     if (large > most) {
       const int e = min((int)(__float_as_uint(large) >> 23) - 126, 17);  // large <= 2^e
       most = __builtin_ldexpf(1.0f, e);
-      up = (float)(15 - e);
+      up = 15.0f - kSlack - (float)e;
     }
     const float next = now == -INFINITY ? -INFINITY : fmaf(now, scale, -up);
     const float shrink = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - next);
@@ -226,7 +246,6 @@ struct Rows4 {
   // ask for the next tile's as soon as this one's are used.
   template <class Seen, class NextK, class NextV>
   __device__ __forceinline__ void use(const char *lds, Seen seen, bool masked, int lane, NextK next_k, NextV next_v) {
-    constexpr uint32_t kLow = 0x000f000fu, kHigh = 0x00f000f0u;
     const int quarter = lane / 16, copy = lane % 16 / (16 / CP);
     // The products of K with q: of a lane's own 16s of keys.
     v4f s[L][G];
@@ -237,8 +256,8 @@ struct Rows4 {
         v4f sum{0, 0, 0, 0};
 #pragma unroll
         for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
-          const uint32_t w = k[h][c], u = w >> 8;
-          const v4u a{codes16<TWO>(w, kLow), codes16<TWO>(w, kHigh), codes16<TWO>(u, kLow), codes16<TWO>(u, kHigh)};
+          const uint32_t w = k[h][c];
+          const v4u a{codes16<TWO, 0>(w), codes16<TWO, 1>(w), codes16<TWO, 2>(w), codes16<TWO, 3>(w)};
           sum = mfma16(a, q[0][c], sum);
           if constexpr (TWO) sum = mfma16(a, q[1][c], sum);
         }
@@ -291,8 +310,7 @@ struct Rows4 {
     const float large = (float)__builtin_elementwise_max(wide[0], wide[1]);
     top = fmaxf(top, __shfl_xor(top, 16));
     top = fmaxf(top, __shfl_xor(top, 32));
-    const float now = fmaxf(m, top);
-    if (__any(now != m || large > most)) raise(now, large);
+    if (__any(fmaf(top, scale, -up) > base + kSlack || large > most)) raise(fmaxf(m, top), large);
     const float from = base == -INFINITY ? 0.0f : base;
     float p[L][4];
 #pragma unroll
@@ -331,9 +349,9 @@ struct Rows4 {
         }
 #pragma unroll
         for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) {
-          const uint32_t w0 = v[h][c], w1 = v[h + 1][c], u0 = w0 >> 8, u1 = w1 >> 8;
-          const v4u even{codes16<TWO>(w0, kLow), codes16<TWO>(u0, kLow), codes16<TWO>(w1, kLow), codes16<TWO>(u1, kLow)};
-          const v4u odd{codes16<TWO>(w0, kHigh), codes16<TWO>(u0, kHigh), codes16<TWO>(w1, kHigh), codes16<TWO>(u1, kHigh)};
+          const uint32_t w0 = v[h][c], w1 = v[h + 1][c];
+          const v4u even{codes16<TWO, 0>(w0), codes16<TWO, 2>(w0), codes16<TWO, 0>(w1), codes16<TWO, 2>(w1)};
+          const v4u odd{codes16<TWO, 1>(w0), codes16<TWO, 3>(w0), codes16<TWO, 1>(w1), codes16<TWO, 3>(w1)};
           o[2 * c] = mfma16(even, b, o[2 * c]);
           o[2 * c + 1] = mfma16(odd, b, o[2 * c + 1]);
           o[2 * c] = mfma16(even, a, o[2 * c]);
@@ -365,9 +383,9 @@ constexpr int waves_a_simd4() {
   return n <= 130 ? 4 : n <= 170 ? 3 : n <= 300 ? 2 : 1;
 }
 
-// Text blockIdx.z, a key head's 16 (or fewer) query heads blockIdx.x, part
-// blockIdx.y of its tiles, a tile a wave at a time. EIGHTS: heads are of a
-// multiple of 8 dims.
+// A key head's 16 (or fewer) query heads blockIdx.x, text blockIdx.z and part
+// blockIdx.y of its tiles, or the parts' number blockIdx.y where there are
+// `pieces`; a tile a wave at a time. EIGHTS: heads are of a multiple of 8 dims.
 template <int NC, int GC, bool TWO, int CP, bool EIGHTS>
 __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) void kv4_attention_parts(Attend4Args a) {
   typedef Rows4<NC, GC, TWO, CP> A;
@@ -378,15 +396,22 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
   __shared__ int lds_bad;
   const int lane = threadIdx.x % 64, col = lane % 16, quarter = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-  const int b = blockIdx.z, per = a.heads / a.c.heads, blocks = (per + 15) / 16;
+  const int wanted = each4(a, KEYS);
+  int b = blockIdx.z, part = blockIdx.y;
+  if (a.pieces) {
+    const Piece4 piece = piece4(a, KEYS, wanted, part);
+    if (piece.b < 0) return;
+    b = piece.b, part = piece.part;
+  }
+  const int per = a.heads / a.c.heads, blocks = (per + 15) / 16;
   const int kv = blockIdx.x / blocks, h0 = kv * per + blockIdx.x % blocks * 16;
   const int rows = min(16, kv * per + per - h0);
   const int length = a.c.lengths[b];
   const bool too_long = length > a.c.table_width * a.c.page_size;
   const Seen s = seen_of(too_long ? 0 : length, a.window, a.sinks, KEYS);
-  const int each = tiles_a_part(s.tiles, a.each, a.splits);
-  const int begin = blockIdx.y * each, end = min(begin + each, s.tiles);
-  if (begin >= end && blockIdx.y) return;  // part 0 of an empty text writes its zeros
+  const int each = tiles_a_part(s.tiles, wanted, a.splits);
+  const int begin = part * each, end = min(begin + each, s.tiles);
+  if (begin >= end && part) return;  // part 0 of an empty text writes its zeros
   if (threadIdx.x == 0) lds_bad = too_long;
   __syncthreads();
 
@@ -429,7 +454,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
     auto load_codes = [&](uint32_t (&n)[H][NC], int i, uint32_t at_) {
 #pragma unroll
       for (int h = 0; h < H; h++)
-        __builtin_memcpy(n[h], page_of(H * i + h) + slot_of(H * i + h) * 16 * NC + at_, 4 * NC);
+        stream_in(n[h], page_of(H * i + h) + slot_of(H * i + h) * 16 * NC + at_);
     };
     // A lane's share of a tile's scales and minima.
     auto load_few = [&](int i) {
@@ -470,7 +495,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
 #pragma unroll
       for (int r = 0; r < 4; r++)
         lds_o[wave][col][32 * c + 2 * (4 * quarter + r) + odd] =
-            fmaf(at.o[2 * c + odd][r], TWO ? (odd ? 0x1p5f : 0x1p9f) : (odd ? 0x1p20f : 0x1p24f), at.om[c / GC]);
+            fmaf(at.o[2 * c + odd][r], TWO ? (odd ? 0x1p5f : 0x1p9f) : 0x1p18f, at.om[c / GC]);
   __syncthreads();
   // A column's factor, and a row's sum: a wave's columns in 16 neighbouring lanes.
   {
@@ -502,7 +527,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
     for (int w = 0; w < kWaves4 * CP; w++)
       o = fmaf(lds_b[w / CP][w % CP * R + row], lds_o[w / CP][w % CP * R + row][d], o);
     if (split) {
-      float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + blockIdx.y) * (a.c.dim + 2);
+      float *p = a.part + (((long)b * a.heads + h0 + row) * a.splits + part) * (a.c.dim + 2);
       p[d + 2] = o;
       if (d == 0) p[0] = lds_l[1][row], p[1] = sum;
     } else {
@@ -511,17 +536,28 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
   }
 }
 
+// As many parts as the card holds workgroups at once, or a multiple of it of two
+// and a half parts a text, less the half part a text that their lengths leave; with
+// many texts, whose lengths each workgroup would have to add up (1 us for one load of
+// them), or few workgroups in all, as the host chose.
 template <int NC, int GC, bool TWO, int CP>
-hipError_t launch_parts4(const Attend4Args &a, hipStream_t s) {
-  const int per = a.heads / a.c.heads;
-  const dim3 grid(a.c.heads * ((per + 15) / 16), a.splits, a.batch), block(64 * kWaves4);
+hipError_t launch_parts4(Attend4Args &a, hipStream_t s) {
+  typedef Rows4<NC, GC, TWO, CP> A;
+  constexpr int kLds = kWaves4 * (16 * (A::DP + 4) * 4 + 256 * A::FEW + 128) + 64;
+  constexpr int kHeld = 256 * std::min(waves_a_simd4<NC, GC, TWO, CP>(), (160 << 10) / kLds);
+  const int per = a.heads / a.c.heads, groups = a.c.heads * ((per + 15) / 16);
+  if (a.splits > 1 && a.batch <= 1024 && long(a.splits) * a.batch * groups > kHeld) {
+    const long wanted = (5L * a.batch * groups + 1) / 2, times = std::max((wanted + kHeld - 1) / kHeld, 1L);
+    a.pieces = int(std::max(times * kHeld / groups - a.batch / 2, 1L));
+  }
+  const dim3 grid = a.pieces ? dim3(groups, a.pieces + a.batch + 1) : dim3(groups, a.splits, a.batch), block(64 * kWaves4);
   if (a.c.dim % 8 == 0) return launch_kernel(kv4_attention_parts<NC, GC, TWO, CP, true>, grid, block, 0, s, a);
   return launch_kernel(kv4_attention_parts<NC, GC, TWO, CP, false>, grid, block, 0, s, a);
 }
 
 // Groups of a whole head, of 32 and of 64 (where a head has more than one).
 template <int NC, bool TWO, int CP>
-hipError_t launch_groups4(const Attend4Args &a, hipStream_t s) {
+hipError_t launch_groups4(Attend4Args &a, hipStream_t s) {
   if constexpr (NC > 1) {
     if (a.c.group == 32) return launch_parts4<NC, 1, TWO, CP>(a, s);
   }
@@ -532,7 +568,7 @@ hipError_t launch_groups4(const Attend4Args &a, hipStream_t s) {
 }
 
 template <bool TWO, int CP>
-hipError_t launch_attention4(const Attend4Args &a, hipStream_t s) {
+hipError_t launch_attention4(Attend4Args &a, hipStream_t s) {
   switch (a.c.nc) {
     case 1: return launch_groups4<1, TWO, CP>(a, s);
     case 2: return launch_groups4<2, TWO, CP>(a, s);

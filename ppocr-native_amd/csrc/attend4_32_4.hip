@@ -2,5 +2,5 @@
 #include "attend4.hpp"
 
 namespace ppocr {
-template hipError_t launch_attention4<true, 4>(const Attend4Args &, hipStream_t);
+template hipError_t launch_attention4<true, 4>(Attend4Args &, hipStream_t);
 }  // namespace ppocr

@@ -75,14 +75,15 @@ struct Attend4Args {
   float scale;  // not negative
   bool turn;    // the given one was negative
   float *part;  // splits > 1: batch x heads x splits rows of dim + 2 floats
+  int pieces;   // parts of all texts that are wanted (but for batch of them at most), or 0: `each` says
 };
 PagedParts kv4_parts(int batch, int heads, int kv_heads, long longest);
 // Columns of a product that a query head has (attend4.hpp), and 16s of keys a tile.
 constexpr int copies4(int per) { return per <= 4 ? 4 : per <= 8 ? 2 : 1; }
 constexpr int halves4(int copies) { return copies == 4 ? 4 : 2; }
 template <bool TWO, int CP>
-hipError_t launch_attention4(const Attend4Args &a, hipStream_t s);
-hipError_t launch_kv4_attention(const Attend4Args &a, hipStream_t s);
+hipError_t launch_attention4(Attend4Args &a, hipStream_t s);
+hipError_t launch_kv4_attention(Attend4Args a, hipStream_t s);
 
 // Beam search: the choice over beams and vocabulary.
 constexpr int kMostBeams = 128, kMostKeep = 128;

@@ -538,3 +538,21 @@ def test_attend4_long_without_parts(t, heads):
     # More tokens than a workgroup looks pages up for at once, in one part.
     run_attend4([4097, 8300], 16, heads, 1, 32, 0, t, work=0)
     run_attend4([9000], 16, heads, 1, 32, 0, t, 4500, 20, work=0)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads,kv", [(2, 1), (3, 3), (14, 2)])
+def test_attend4_many_texts(t, heads, kv):
+    # Texts of very different lengths, whose parts share out the card's workgroups: more texts than a wave has lanes.
+    rng = np.random.default_rng(heads)
+    lengths = [int(x) for x in rng.integers(0, 40, 150)]
+    lengths[3], lengths[70], lengths[149], lengths[64] = 2500, 1300, 900, 0
+    run_attend4(lengths, 16, heads, kv, 32, 0, t, work=1 << 26)
+    run_attend4(lengths, 16, heads, kv, 32, 32, t, 600, 20, work=1 << 26)
+    run_attend4(lengths, 16, heads, kv, 32, 0, t, work=150 * heads * 34 * 4 * 3)  # three parts a text at most
+
+
+def test_attend4_more_texts_than_are_added_up():
+    lengths = [0, 1, 2, 17] * 300
+    lengths[5], lengths[1030], lengths[1199] = 1500, 2100, 700
+    run_attend4(lengths, 16, 2, 1, 32, 0, D.F16, work=1 << 26)
