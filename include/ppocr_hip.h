@@ -428,7 +428,8 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
  * scales go into their products in two F16 parts (22 bits), f32 queries too, 16-bit
  * queries whole. A text with a token of scale NaN that it sees gives NaN (in K:
  * its whole head, in V: the group's dims), a query with an infinity or NaN gives
- * NaN. Everything else, and the workspace, is as there. */
+ * NaN. The parts of up to 1024 texts are as long as all their lengths ask for.
+ * Everything else, and the workspace, is as there. */
 size_t ppocr_hip_kv4_attention_workspace(const ppocr_kv4_cache *cache, size_t batch, size_t heads, size_t longest);
 int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cache *cache, const int32_t *table,
                             size_t table_width, const int32_t *lengths, void *y, size_t y_stride, size_t batch,
@@ -440,7 +441,7 @@ int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cach
  * x of `type` (rows of beams, `stride` values apart; 0: vocab),
  *   score(i, v) = scores[b][i] + log_softmax(x[b][i])[v],
  * computed and ordered in 64 bits (sums of exponentials in 32), ties to the
- * lower i, then the lower v; [batch][keep] scores, the best first, their beams'
+ * lower i, then the larger logit, then the lower v; [batch][keep] scores, the best first, their beams'
  * numbers `parents` and their `tokens`. A beam whose `ended` byte is not 0
  * (`ended` NULL: none) goes on with the token `end` alone, its score as it is.
  * `out_ended` (or NULL) says of each choice whether its beam had ended or its

@@ -211,8 +211,8 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
 
 constexpr int kChoices = 2048;
 
-// A candidate: its score, ordered, and its position among beams x vocabulary,
-// the lower one the larger. 0, 0: none.
+// A candidate: its score, ordered, and what decides where scores are equal: the
+// lower beam (8 bits), the larger logit (32), the lower token (24). 0, 0: none.
 struct Choice {
   uint64_t score, at;
   __device__ __forceinline__ bool operator>(const Choice &o) const {
@@ -222,7 +222,9 @@ struct Choice {
 
 // A workgroup a text, a candidate or more a thread; `lanes` of a group, as above.
 // A chain of waits: the parts' statistics, their logarithm, the candidates (asked
-// for before it), the bound, the list.
+// for before it), the bound, the list. Bounds of 32-bit scores, ranks by waves, and
+// results written side by side took it from 12.5 to 7.7 us for 32 texts of 8 beams
+// with 1024 candidates each (4 beams and 144: 5.9).
 __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Divide by_beams) {
   __shared__ Choice list[kChoices], chosen[kMostKeep];
   __shared__ double lds_base[kMostBeams], lds_top[kMostBeams], lds_log[kMostBeams];
@@ -269,10 +271,13 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
   }
   if (threadIdx.x == 0) lds_count = 0;
   __syncthreads();
+  const auto place = [](int i, uint32_t logit, uint32_t token) {
+    return (uint64_t)(255 - i) << 56 | (uint64_t)logit << 24 | (0xffffffu - token);
+  };
   auto choice = [&](int c, uint64_t key) -> Choice {
     if (c >= all) {
       const int i = c - all;
-      return lds_live[i] == 2 ? Choice{ordered(lds_base[i] + 0.0), ~((uint64_t)i * a.vocab + a.end)} : Choice{0, 0};
+      return lds_live[i] == 2 ? Choice{ordered(lds_base[i] + 0.0), place(i, 0, a.end)} : Choice{0, 0};
     }
     const int i = c - by_beams(c) * a.beams;
     if (lds_live[i] != 1) return Choice{0, 0};
@@ -280,7 +285,7 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
     const double x = (double)unordered((uint32_t)(key >> 32));
     const double score = lds_base[i] + ((x - lds_top[i]) - lds_log[i]);
     if (!(score > -INFINITY)) return Choice{0, 0};
-    return Choice{ordered(score + 0.0), ~((uint64_t)i * a.vocab + (uint32_t)~(uint32_t)key)};
+    return Choice{ordered(score + 0.0), place(i, (uint32_t)(key >> 32), ~(uint32_t)key)};
   };
   // Each thread's candidates: the first from what was asked for ahead.
   auto each_choice = [&](auto &&take) {
@@ -383,8 +388,8 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
   }
   __syncthreads();
   for (int i = threadIdx.x; i < a.keep; i += threads) {
-    const uint32_t at = i < n ? (uint32_t)~chosen[i].at : 0u;  // (below 2^31)
-    const int parent = (int)(at / (uint32_t)a.vocab), token = (int)(at - (uint32_t)parent * a.vocab);
+    const uint64_t at = i < n ? chosen[i].at : 0;
+    const int parent = 255 - (int)(at >> 56), token = (int)(0xffffffu - ((uint32_t)at & 0xffffffu));
     const long to = out + i;
     a.out_scores[to] = i < n ? (float)unordered(chosen[i].score) : -INFINITY;
     a.parents[to] = i < n ? parent : min(i, a.beams - 1);

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(64 * kMostWaves4, EIGHTS ? 4 : 2) void kv4_append_r
   __shared__ uint32_t words[kMostWaves4][S::WORDS];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int threads = blockDim.x, waves = threads / 64;
-  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, blockIdx.x);
+  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
   if (k16.b < 0) return;
   const TurnArgs &t = a.t;
   const int dim = a.c.dim, half = t.rotary / 2;
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(64 * kMostWaves4) void kv4_read_rows(Read4Args a) {
   typedef Split4<LP, F4> S;
   __shared__ uint32_t words[kMostWaves4][S::WORDS];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
-  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, blockIdx.x);
+  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
   if (k16.b < 0) return;
   const int l = lane % LP, d = 8 * l, dim = a.c.dim, have = min(max(dim - d, 0), 8);
   const int nc = a.c.nc, block = min(l / 4, nc - 1), quarter = l % 4, group = min(d / a.c.group, a.c.groups - 1);
@@ -407,8 +407,10 @@ __global__ __launch_bounds__(64 * kMostWaves4) void kv4_read_rows(Read4Args a) {
   }
 }
 
-inline unsigned blocks4(long rows, int batch) {
-  return unsigned((rows + (2 * kPlaces - 2L) * batch) / kPlaces + 1);
+// (A grid's side has fewer than 2^32 threads.)
+inline dim3 grid4(long rows, int batch, unsigned roles) {
+  const long blocks = (rows + (2 * kPlaces - 2L) * batch) / kPlaces + 1, wide = std::min(blocks, 1L << 20);
+  return dim3(unsigned(wide), roles, unsigned((blocks + wide - 1) / wide));
 }
 
 // Four waves, or eight where the keys and values of 16 tokens have work for them.
@@ -426,7 +428,7 @@ hipError_t launch_append4(Append4Args a, hipStream_t s) {
   a.units = units_of(whole && eights ? N : 1, a.c.dim, a.t.rotary, a.t.pairs);
   a.by_unit = Divide(a.units);
   a.by_half = Divide(std::max(a.t.rotary / 2, 1));
-  const dim3 grid(blocks4(a.rows, a.batch), a.t.q ? 2 : 1), block = threads4<LP, 1>(a.c.heads, a.rows, a.batch);
+  const dim3 grid = grid4(a.rows, a.batch, a.t.q ? 2 : 1), block = threads4<LP, 1>(a.c.heads, a.rows, a.batch);
   // Teams of whole waves: fewest steps, of which a new unit is half a one.
   const long items = (long)a.t.heads * a.units, tokens = a.rows > a.batch ? kPlaces : 1;
   long least = -1;
@@ -455,7 +457,7 @@ hipError_t launch_read4(const Read4Args &a, hipStream_t s) {
   // Four times the heads a wave where there is more than a token a text: 25000
   // tokens of 8 heads of 128 as f16 take 26 us instead of 32; 64 texts' newest 5.4
   // instead of 4.3.
-  const dim3 grid(blocks4(a.rows, a.batch));
+  const dim3 grid = grid4(a.rows, a.batch, 1);
   if (a.rows <= a.batch) return launch_kernel(kv4_read_rows<T, LP, 1>, grid, threads4<LP, 1>(a.c.heads, a.rows, a.batch), 0, s, a);
   return launch_kernel(kv4_read_rows<T, LP, 4>, grid, threads4<LP, 4>(a.c.heads, a.rows, a.batch), 0, s, a);
 }

@@ -25,7 +25,8 @@ def choose(x, base, keep, ended=None, end=-1):
             if base[i] > -np.inf:
                 s[i, end] = base[i]
     flat = s.reshape(-1)
-    order = np.argsort(-flat, kind="stable")
+    at = np.arange(beams * vocab)
+    order = np.lexsort((at, -x.reshape(-1), at // vocab, -flat))  # ties: the lower beam, the larger logit, the lower token
     order = order[flat[order] > -np.inf]
     near, order = order[:keep + 1], order[:keep]
     out = [np.full(keep, -np.inf), np.minimum(np.arange(keep), beams - 1), np.full(keep, -1), np.zeros(keep, np.uint8)]

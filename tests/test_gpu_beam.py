@@ -294,3 +294,15 @@ def test_reorder_states_alone():
     D.beam_reorder([], dp.addr, 0, 0, 0, 0, 0, 0, 2, 3, states=[D.BeamState(d.addr, o.addr, 1 << 21)])
     synchronize()
     assert np.array_equal(R.back(o, np.uint8, a.shape), a[[2, 0, 0, 4, 4, 5]])
+
+
+@pytest.mark.parametrize("base", [-1e9, -3e38, 1e9])
+def test_select_of_scores_that_32_bits_do_not_tell_apart(base):
+    # Scores so far from 0 that all candidates' are one number in 32 bits, many more than a workgroup lists; logits are
+    # whole numbers of 1/8, so that in 64 bits each keeps its place (1e9), or all are equal and the logits decide (3e38).
+    rng = np.random.default_rng(5)
+    x = rng.permutation(131072).reshape(1, 1, -1) / 8.0
+    s = Select(x, np.full((1, 1), base), 128, D.F32)
+    s.run()
+    synchronize()
+    s.check()
