@@ -57,7 +57,8 @@ __host__ __device__ inline int lanes_of(int used, int keep) {
 // gathered in LDS and ranked there. Of shuffled numbers that leaves a few times
 // `keep`; where more than LDS holds (sorted ones, or equal ones), the bound is
 // halved in on. What costs is the logits' own arithmetic, ten operations each,
-// four of them the exponential's: 256 rows of 131072 in bf16, 30 % of them ended.
+// four of them the exponential's: 256 rows of 131072 in bf16, some of them ended,
+// take 16 us, 67 MB at 4.2 TB/s; four rows of 18385 in f32 take 4.1.
 // R: rounds of 8 values a thread. FEW: rows of fewer than 8 values.
 template <int T, int R, bool FEW>
 __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
@@ -438,8 +439,9 @@ __device__ __forceinline__ void copy_pieces(char *to, const char *from, long byt
 }
 
 // Row (a text's beam) blockIdx.y; workgroup 0 of it has its table, the next ones
-// the states, the others a split of a plane's tokens each. Memory bound, or by
-// the launch.
+// the states, the others a split of a plane's tokens each. Memory bound (64 rows,
+// 12 layers, 143 MB: 27 us, 5.4 TB/s, where a copy has 5.2), or by the launch (4
+// rows of one layer: 3.1 us).
 __global__ __launch_bounds__(256) void beam_reorder_rows(ReorderArgs a) {
   const int row = blockIdx.y, text = a.by_beams(row);
   const int parent = a.parents[row];

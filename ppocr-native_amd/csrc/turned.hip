@@ -11,8 +11,10 @@ constexpr long kNoText = -(1L << 40);  // below every token's number
 
 // TOKENS rows a workgroup: their loads need no more than the rows' numbers, so
 // they are on their way while waves find the texts, places and angles; a thread
-// has the same unit of each row. Memory bound; at a token a text bound by that
-// chain of waits.
+// has the same unit of each row. Memory bound: six prompts, 5400 rows of 32 heads
+// of 128 and 8 key heads in f16, 133 MB, take 25 us, 5.3 TB/s (a copy of as much
+// has 5.2; 28 us without the stores as a stream). At a token a text the chain of
+// waits is the whole: 64 take 4.8 us.
 template <int T, int N, int TOKENS>
 __global__ __launch_bounds__(512) void kv_append_turned(TurnedAppendArgs g) {
   typedef num_t<T> V;
@@ -104,8 +106,8 @@ hipError_t launch_turned(TurnedAppendArgs a, hipStream_t s) {
   const int threads = std::max(int(((items + rounds - 1) / rounds + 63) / 64 * 64), 128);
   const dim3 block(threads);
   a.by_half = Divide(std::max(a.t.rotary / 2, 1));
-  // Two rows a workgroup where that leaves every compute unit two (38 us with one
-  // row at 8192 rows of 32 + 2 x 8 heads of 128 in 16 bits, 28 with two, 30 with four).
+  // Two rows a workgroup where that leaves every compute unit two (the six
+  // prompts above: 38 us with one row, 28 with two, 30 with four, all without streams).
   const bool two = N > 1 && a.a.rows >= 4 * 256;
   const long groups = two ? (a.a.rows + 1) / 2 : a.a.rows, wide = std::min(groups, 1L << 20);
   const dim3 grid(unsigned(wide), unsigned((groups + wide - 1) / wide));
