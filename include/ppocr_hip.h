@@ -428,7 +428,7 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
  * scales go into their products in two F16 parts (22 bits), f32 queries too, 16-bit
  * queries whole. A text with a token of scale NaN that it sees gives NaN (in K:
  * its whole head, in V: the group's dims), a query with an infinity or NaN gives
- * NaN. The parts of up to 1024 texts are as long as all their lengths ask for.
+ * NaN. Into how many parts a text is split may depend on all texts' lengths.
  * Everything else, and the workspace, is as there. */
 size_t ppocr_hip_kv4_attention_workspace(const ppocr_kv4_cache *cache, size_t batch, size_t heads, size_t longest);
 int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cache *cache, const int32_t *table,

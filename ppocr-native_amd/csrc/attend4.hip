@@ -55,13 +55,14 @@ __global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a, int key
 }  // namespace
 
 PagedParts kv4_parts(int batch, int heads, int kv_heads, long longest) {
-  // At least as long as were 4096 workgroups of it if all texts were the longest
-  // (with a thousand texts or fewer the device makes them longer, by the lengths
-  // that it has); but of 512 tokens at least, or 128 where that leaves too few for
-  // the card. A text of 512 is done without a join.
+  // At least as long as were 2048 workgroups of it if all texts were the longest, or
+  // 4096 where the device makes them longer, by the lengths that it has; but of 512
+  // tokens at least, or 128 where that leaves too few for the card. A text of 512 is
+  // done without a join.
   const int per = heads / kv_heads, keys = 16 * halves4(copies4(per)), least = 512 / keys, few = 128 / keys;
   const long groups = (long)batch * kv_heads * ((per + 15) / 16), tiles = (longest + keys - 1) / keys + 2;
-  long each = (tiles * groups + 4095) / 4096;
+  const long most = groups <= kShared4 ? 4096 : 2048;
+  long each = (tiles * groups + most - 1) / most;
   if (each < least) {
     const long fill = (tiles * groups + 511) / 512;
     each = tiles <= least + 1 ? least + 1 : fill < few ? few : fill < least ? fill : least;

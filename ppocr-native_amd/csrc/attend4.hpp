@@ -538,15 +538,14 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
 
 // As many parts as the card holds workgroups at once, or a multiple of it of two
 // and a half parts a text, less the half part a text that their lengths leave; with
-// many texts, whose lengths each workgroup would have to add up (1 us for one load of
-// them), or few workgroups in all, as the host chose.
+// many texts and heads, or few workgroups in all, as the host chose.
 template <int NC, int GC, bool TWO, int CP>
 hipError_t launch_parts4(Attend4Args &a, hipStream_t s) {
   typedef Rows4<NC, GC, TWO, CP> A;
   constexpr int kLds = kWaves4 * (16 * (A::DP + 4) * 4 + 256 * A::FEW + 128) + 64;
   constexpr int kHeld = 256 * std::min(waves_a_simd4<NC, GC, TWO, CP>(), (160 << 10) / kLds);
   const int per = a.heads / a.c.heads, groups = a.c.heads * ((per + 15) / 16);
-  if (a.splits > 1 && a.batch <= 1024 && long(a.splits) * a.batch * groups > kHeld) {
+  if (a.splits > 1 && long(a.batch) * groups <= kShared4 && long(a.splits) * a.batch * groups > kHeld) {
     const long wanted = (5L * a.batch * groups + 1) / 2, times = std::max((wanted + kHeld - 1) / kHeld, 1L);
     a.pieces = int(std::max(times * kHeld / groups - a.batch / 2, 1L));
   }

@@ -6,6 +6,12 @@
 
 namespace ppocr {
 
+// Texts times their groups of heads up to which a call's parts go by what the
+// lengths are. Each workgroup adds the lengths up, and with more of them there is
+// enough to do without parts (100 texts to 4000, 8 key heads: 79 us so, 67 as the
+// host chose; 300 to 2000: 156 and 85; but 128 to 4000 of 2 key heads: 30 and 46).
+constexpr long kShared4 = 768;
+
 // A text's tiles.
 __device__ __forceinline__ Seen seen4(const Attend4Args &a, int b, int keys) {
   const int length = a.c.lengths[b];
