@@ -380,7 +380,7 @@ template <int NC, int GC, bool TWO, int CP>
 constexpr int waves_a_simd4() {
   typedef Rows4<NC, GC, TWO, CP> A;
   constexpr int n = NC * (8 + (TWO ? 8 : 4) + 2 * A::H) + A::FEW + A::G * (4 * A::L + 8 * A::L) + 55;
-  return n <= 130 ? 4 : n <= 170 ? 3 : n <= 300 ? 2 : 1;
+  return n <= 130 ? 4 : n <= 170 ? 3 : n <= 250 ? 2 : 1;
 }
 
 // A key head's 16 (or fewer) query heads blockIdx.x, text blockIdx.z and part
