@@ -1,6 +1,6 @@
 // Attention of one new token a text over a cache in 4 bits
 // (ppocr_hip_kv4_attention): the kernel, compiled for 16-bit and for 32-bit
-// queries (attend4_16.hip, attend4_32.hip).
+// queries (attend4_16_*.hip, attend4_32_*.hip).
 //
 // A key is n s + m with codes n of 0 .. 15 and a scale and a minimum a group:
 //   S[key][row] = sum over groups g of  s_g (sum of n q over g) + m_g (sum of q over g)
@@ -28,7 +28,7 @@
 // heads of 128 in bf16 and groups of 64, 305 MB: 97 us with one column a row, 73 with
 // four). What else counted there: codes read as a stream (69), parts by the lengths
 // that there are, so that no workgroup is left over for a last, short round (63: 4.8
-// TB/s). The loads alone take 57, the arithmetic alone 51.
+// TB/s). Of the 73 the loads alone took 66, the arithmetic alone 51.
 #pragma once
 #include <algorithm>
 #include <type_traits>

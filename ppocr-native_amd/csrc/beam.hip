@@ -69,8 +69,9 @@ __device__ __forceinline__ int rank_of(const float *numbers, int n, float mine, 
 // gathered in LDS and ranked there. Of shuffled numbers that leaves a few times
 // `keep`; where more than LDS holds (sorted ones, or equal ones), the bound is
 // halved in on. What costs is the logits' own arithmetic, ten operations each,
-// four of them the exponential's: 256 rows of 131072 in bf16, some of them ended,
-// take 16 us, 67 MB at 4.2 TB/s; four rows of 18385 in f32 take 4.1.
+// four of them the exponential's: 256 rows of 131072 in bf16, 30 % of them ended,
+// take 17 us, 47 MB at 2.7 TB/s and 71 % of the vector units' time; four rows of 18385
+// in f32 take 4.5.
 // R: rounds of 8 values a thread. FEW: rows of fewer than 8 values.
 template <int T, int R, bool FEW>
 __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
@@ -236,8 +237,8 @@ struct Choice {
 // A workgroup a text, a candidate or more a thread; `lanes` of a group.
 // A chain of waits: the parts' statistics, their logarithm, the candidates (asked
 // for before it), the bound, the list. Bounds of 32-bit scores, ranks by waves, and
-// results written side by side took it from 12.5 to 7.7 us for 32 texts of 8 beams
-// with 1024 candidates each (4 beams and 144: 5.9).
+// results written side by side took it from 12.5 to 7.5 us for 32 texts of 8 beams
+// with 1024 candidates each (4 beams and 144: 6.1).
 __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Divide by_beams) {
   __shared__ Choice list[kChoices], chosen[kMostKeep];
   __shared__ double lds_base[kMostBeams], lds_top[kMostBeams], lds_log[kMostBeams];
