@@ -43,6 +43,7 @@ __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f
 // ---------------------------------------------------------------- a row's parts
 
 constexpr int kThreads = 256, kList = 1024;
+constexpr float kLowest = -3.402823466e38f;  // a bound that only -infinity, which is never chosen, is below
 
 // Lanes of a group, of `used` threads that have values: as many as leave `groups`
 // of them, up to a wave.
@@ -133,16 +134,25 @@ __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
   if (lane % lanes == 0) lds_group[threadIdx.x / lanes] = most;
   if (threadIdx.x < 4) lds_group[groups + threadIdx.x] = -INFINITY;
   if (lane == 0) lds_top[wave] = top;
-  if (threadIdx.x == 0) lds_count = 0, lds_bound = -3.402823466e38f;  // (nothing of -infinity is chosen)
+  if (threadIdx.x == 0) lds_count = 0;
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 4; w++) top = fmaxf(top, lds_top[w]);
-  if ((int)threadIdx.x < groups) {
-    const float mine = lds_group[threadIdx.x];
-    if (rank_of(lds_group, groups, mine, threadIdx.x) == a.keep - 1 && mine > -INFINITY) lds_bound = mine;
+  float bound;
+  if (groups <= 64) {  // each wave for itself
+    const float mine = lds_group[min(lane, groups)];
+    const uint64_t is = __ballot(lane < groups && rank_of(lds_group, groups, mine, lane) == a.keep - 1 && mine > -INFINITY);
+    bound = is ? __shfl(mine, __builtin_ctzll(is)) : kLowest;
+  } else {
+    if (threadIdx.x == 0) lds_bound = kLowest;
+    __syncthreads();
+    if ((int)threadIdx.x < groups) {
+      const float mine = lds_group[threadIdx.x];
+      if (rank_of(lds_group, groups, mine, threadIdx.x) == a.keep - 1 && mine > -INFINITY) lds_bound = mine;
+    }
+    __syncthreads();
+    bound = lds_bound;
   }
-  __syncthreads();
-  const float bound = lds_bound;
   // Which of a thread's values are past it, a bit each; their values are read once more, where there are any.
   const auto push = [&](uint64_t key) {
     const int at = atomicAdd(&lds_count, 1);
