@@ -7,7 +7,7 @@ import decoder_plain as R
 import writer_plain as W
 from ppocr_native_amd import decoder as D
 from ppocr_native_amd.devmem import DeviceArray, synchronize
-from test_gpu_decoder import pages_of
+from test_gpu_decoder import Graph, _stream, pages_of
 
 pytestmark = pytest.mark.gpu
 
@@ -556,3 +556,46 @@ def test_attend4_more_texts_than_are_added_up():
     lengths = [0, 1, 2, 17] * 300
     lengths[5], lengths[1030], lengths[1199] = 1500, 2100, 700
     run_attend4(lengths, 16, 2, 1, 32, 0, D.F16, work=1 << 26)
+
+
+@pytest.mark.parametrize("longest", [1000, 2000])
+def test_attend4_longer_than_said(longest):
+    # Texts longer than `longest`, whose parts go by the lengths that there are.
+    lengths = [3, 40, 2500, 0, 700] * 30
+    run_attend4(lengths, 16, 4, 4, 32, 0, D.F16, longest=longest, work=1 << 27)
+
+
+def test_attend4_captured_with_lengths_that_change():
+    # The parts of a captured call go by the lengths of each replay: as eager calls, bit for bit.
+    rng = np.random.default_rng(8)
+    batch, heads, dim = 150, 4, 64
+    most = rng.integers(1, 1500, batch)
+    p = W.Cache4(rng, most.tolist(), 32, heads, dim, 32)
+    p.fill(rng, most.tolist())
+    cache = p.upload()
+    q = R.stored(rng.normal(0, 2, (batch, heads * dim)), D.BF16)
+    dq, dl = R.on_gpu(q), DeviceArray(4 * batch)
+    size = D.kv4_attention_workspace(cache, batch, heads, 1500)
+    out = [R.on_gpu(np.zeros(q.shape, q.dtype)) for _ in range(2)]
+    work = [R.on_gpu(np.full(size, 0xFF, np.uint8)) for _ in range(2)]
+
+    def call(i, stream=0):
+        D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, out[i].addr, batch, heads, scale=0.1,
+                        type=D.BF16, longest=1500, workspace=work[i].addr, workspace_bytes=size, stream=stream)
+
+    s = _stream()
+    dl.upload(most.astype(np.int32))
+    call(0, s.value)
+    synchronize()
+    graph = Graph(s, lambda: call(0, s.value))
+    for i in range(5):
+        lengths = np.where(rng.random(batch) < 0.3, 0, rng.integers(0, most + 1)) if i else np.minimum(most, 5)
+        dl.upload(lengths.astype(np.int32))
+        print(f"captured 4-bit attention, replay {i}", flush=True)
+        graph.launch()
+        synchronize()
+        call(1)
+        synchronize()
+        one, other = (R.back(o, q.dtype, q.shape) for o in out)
+        assert np.array_equal(one.view(np.uint16), other.view(np.uint16))
+        assert not one[lengths == 0].any() and one[lengths > 0].astype(np.float32).any(-1).all()
