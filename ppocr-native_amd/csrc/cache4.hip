@@ -9,7 +9,8 @@
 // of them at a time, one of V's blocks, where a code word is four tokens' bytes: a
 // lane has eight neighbouring dims of one of them, which are a word of K's codes
 // and a byte of each of four words of V's. Those go through a wave's own piece of
-// LDS, so that memory sees whole words. The queries have workgroups of their own.
+// LDS, so that memory sees whole words. The queries have workgroups of their own;
+// they are turned at places below 0, too, where there is nothing to append.
 //
 // Memory bound where there are many tokens: four chunks of prompts (11500 tokens
 // of 32 heads of 128, 8 key heads, f16, groups of 32) are appended in 54 us, 250 MB
@@ -40,7 +41,8 @@ __device__ __forceinline__ void store_past(V *p, int have, const V (&v)[8]) {
 }
 
 // The 16 places that workgroup g has, with as many workgroups for each text as
-// its rows could touch: text b's begin at (its first row + 30 b) / 16.
+// its rows could touch: text b's begin at (its first row + 30 b) / 16. BELOW: with
+// the places below 0 of a text that has fewer tokens than rows.
 constexpr int kPlaces = 16;
 struct Block16 {
   int b;        // text, or -1
@@ -53,6 +55,7 @@ struct Block16 {
 
 __device__ __forceinline__ long clamped(long v, long most) { return min(max(v, 0L), most); }
 
+template <bool BELOW>
 __device__ __forceinline__ Block16 block_of(const Kv4Args &c, const int *starts, long rows, int batch, long g) {
   Block16 o;
   o.b = -1;
@@ -64,14 +67,16 @@ __device__ __forceinline__ Block16 block_of(const Kv4Args &c, const int *starts,
   long first = b, last = b + 1L;
   if (starts) first = starts[b], last = starts[b + 1];
   const long count = last - first, base = (long)c.lengths[b] - count;  // row first + i has place base + i
-  const long begin = max(max(0L, -first), -base), end = min(count, rows - first);
+  const long begin = max(max(0L, -first), BELOW ? 0L : -base), end = min(count, rows - first);
   if (begin >= end) return o;
-  o.place = (base + begin) / kPlaces * kPlaces + kPlaces * (g - start(b));
+  o.place = ((base + begin) & -(long)kPlaces) + kPlaces * (g - start(b));
   if (o.place >= base + end) return o;
   o.b = b;
   o.row0 = first + o.place - base;
   o.from = (int)max(0L, base + begin - o.place);
   o.to = (int)min((long)kPlaces, base + end - o.place);
+  o.slot = 0;
+  if (o.place < 0) return o;  // (all 16 are)
   const int slot = c.by_page((int)o.place);
   o.slot = (int)(o.place - (long)slot * c.page_size);
   if (slot < c.table_width) {
@@ -185,7 +190,7 @@ __global__ __launch_bounds__(64 * kMostWaves4, EIGHTS ? 4 : 2) void kv4_append_r
   __shared__ uint32_t words[kMostWaves4][S::WORDS];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int threads = blockDim.x, waves = threads / 64;
-  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
+  const Block16 k16 = block_of<true>(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
   if (k16.b < 0) return;
   const TurnArgs &t = a.t;
   const int dim = a.c.dim, half = t.rotary / 2;
@@ -341,7 +346,7 @@ __global__ __launch_bounds__(64 * kMostWaves4) void kv4_read_rows(Read4Args a) {
   typedef Split4<LP, F4> S;
   __shared__ uint32_t words[kMostWaves4][S::WORDS];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
-  const Block16 k16 = block_of(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
+  const Block16 k16 = block_of<false>(a.c, a.starts, a.rows, a.batch, (long)blockIdx.z * gridDim.x + blockIdx.x);
   if (k16.b < 0) return;
   const int l = lane % LP, d = 8 * l, dim = a.c.dim, have = min(max(dim - d, 0), 8);
   const int nc = a.c.nc, block = min(l / 4, nc - 1), quarter = l % 4, group = min(d / a.c.group, a.c.groups - 1);

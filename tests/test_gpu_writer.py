@@ -599,3 +599,106 @@ def test_attend4_captured_with_lengths_that_change():
         one, other = (R.back(o, q.dtype, q.shape) for o in out)
         assert np.array_equal(one.view(np.uint16), other.view(np.uint16))
         assert not one[lengths == 0].any() and one[lengths > 0].astype(np.float32).any(-1).all()
+
+
+# -------------------------- the 4-bit append's queries, in every kind of row
+
+def run_append4(t, lengths, new, page, heads, kv, dim, group, rotary, pairs, gap=0, in_place=False, far=None, held=None,
+                change=None, first=0, behind=0):
+    """Texts of `lengths` tokens get `new` rows, behind `first` rows of no text and before `behind` of them. What is in
+    range is held: k near its line, v as the formula has it; every other byte stays; all texts' queries are turned."""
+    rng = np.random.default_rng(dim * 3 + rotary + len(new))
+    p = W.Cache4(rng, held or lengths, page, kv, dim, group)
+    if change:
+        change(p)
+    cache = p.upload()
+    rows = first + sum(new) + behind
+    wide = lambda n: np.concatenate([R.stored(rng.normal(0, 1, (rows, n * dim)), t), np.full((rows, gap), 7, R.dtype(t))], 1)  # noqa: E731
+    q, k, v = wide(heads), wide(kv), wide(kv)
+    starts = (first + np.concatenate([[0], np.cumsum(new)])).astype(np.int32)
+    text = np.repeat(np.arange(len(new)), new)
+    places = np.concatenate([np.arange(n) + length - n for n, length in zip(new, lengths)]).astype(np.int64)
+    positions = np.zeros(rows, np.int64)
+    positions[first:first + len(places)] = places + (far or 0)
+    freqs = W.frequencies(rotary)
+    dq, dk, dv, df = R.on_gpu(q), R.on_gpu(k), R.on_gpu(v), R.on_gpu(freqs)
+    do = dq if in_place else R.on_gpu(np.full(q.shape, 7, R.dtype(t)))
+    dl, ds, dp = R.on_gpu(np.array(lengths, np.int32)), R.on_gpu(starts), R.on_gpu(positions.astype(np.int32))
+    single = new == [1] * len(new) and rows == len(new)
+    print(f"4-bit append, type {t}, lengths {lengths[:6]}, new {new[:6]}, heads {heads}/{kv} of {dim} in {group}, {rotary} "
+          f"turned, pairs {pairs}, gap {gap}, in place {in_place}, far {far}", flush=True)
+    D.kv4_append(dk.addr, dv.addr, cache, p.gpu_table.addr, p.width, dl.addr, len(new), rows, type=t,
+                 starts=0 if single else ds.addr, freqs=df.addr, rotary=rotary, pairs=pairs,
+                 positions=0 if far is None else dp.addr, q=dq.addr, q_out=do.addr, heads=heads,
+                 q_stride=heads * dim + gap, q_out_stride=heads * dim + gap, k_stride=kv * dim + gap,
+                 v_stride=kv * dim + gap)
+    synchronize()
+    own = slice(first, first + len(places))
+    out = R.back(do, R.dtype(t), q.shape)
+    cut = lambda a, n: R.values(a[own, :n * dim].reshape(-1, n, dim), t)  # noqa: E731
+    left = q if in_place else np.full_like(q, 7)
+    for a, b in ((out[:, heads * dim:], left[:, heads * dim:]), (out[:first], left[:first]),
+                 (out[own.stop:], left[own.stop:])):
+        assert np.array_equal(a, b)
+    want, size = W.turned(cut(q, heads), positions[own], freqs, rotary, pairs)
+    R.close(cut(out, heads), want, W.turned_bound(want, size, t) * (size > 0))
+    want, size = W.turned(cut(k, kv), positions[own], freqs, rotary, pairs)
+    rest, got = p.data.copy(), p.back()
+    p.data[...] = got
+    of = np.arange(dim) // p.size
+    for i, (b, at) in enumerate(zip(text, places)):
+        if at < 0 or at // page >= p.width or not 0 <= p.table[b, at // page] < p.pages:
+            continue
+        (ks, km), (vs, vm) = p.get(b, at)
+        page_, slot = p.place(b, at)
+        s, m = (p.few()[j][page_, :, slot].astype(np.float64)[:, of] for j in (0, 1))
+        R.close(ks + km, want[i], s / 2 + 15 * s * 2.0 ** -11 + np.abs(m) * 2.0 ** -10 + size[i] * 4 * 2.0 ** -24 + 1e-7)
+        n4, s4, m4 = W.quantised(cut(v, kv)[i], p.p, p.size)
+        assert np.array_equal(vs, n4[:, :dim] * s4.astype(np.float64)[:, of])
+        assert np.array_equal(vm, m4.astype(np.float64)[:, of])
+        # This token's bytes may differ from what was there.
+        for x, y in zip(rest[page_, :kv * p.chunk].reshape(kv, -1), got[page_, :kv * p.chunk].reshape(kv, -1)):
+            for bytes_ in p.dims(slot):
+                x[bytes_] = y[bytes_]
+            for j in (1, 2, 4, 5):
+                at_ = p.at[j] + slot * 2 * p.groups
+                x[at_:at_ + 2 * p.groups] = y[at_:at_ + 2 * p.groups]
+    assert np.array_equal(got, rest)
+
+
+TURNS4 = [(128, 64, 128, False), (64, 0, 32, False), (96, 32, 48, False), (40, 0, 40, True), (15, 0, 14, False),
+          (15, 0, 6, True), (72, 32, 24, False), (256, 32, 256, False)]
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim,group,rotary,pairs", TURNS4)
+def test_append4_of_places_below_0(t, dim, group, rotary, pairs):
+    # A text of fewer tokens than rows: a finished one of length 0 with its one row, or a prompt whose length was cut.
+    turn = (dim, group, rotary, pairs)
+    run_append4(t, [5, 0, 7, 0], [1, 1, 1, 1], 16, 4, 2, *turn)
+    run_append4(t, [5, 0, -40, 16], [1, 1, 1, 1], 16, 4, 2, *turn, gap=3, in_place=True, far=1000, held=[5, 1, 1, 16])
+    run_append4(t, [3, 0, 20, 2], [40, 17, 3, 2], 16, 4, 2, *turn, first=2, behind=3)
+    run_append4(t, [1, 33], [17, 34], 48, 6, 1, *turn, in_place=True, far=50)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+def test_append4_leaves_what_is_out_of_range(t):
+    # As the plain cache's: places past the table and in pages that do not exist are written nowhere; the queries of
+    # these rows are turned all the same.
+    def change(p):
+        p.table[2, 1], p.table[3, 1] = -1, p.pages
+    for in_place in (False, True):
+        run_append4(t, [1, 33, 18, 18], [2, 2, 4, 5], 16, 2, 1, 8, 0, 8, False, held=[20] * 4, change=change, first=1,
+                    behind=1, in_place=in_place)
+        run_append4(t, [40, 33, 18, 18], [1] * 4, 16, 4, 2, 64, 32, 64, False, held=[20] * 4, change=change,
+                    in_place=in_place)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("dim,group,rotary,pairs", TURNS4)
+def test_append4_of_a_token_a_text(t, dim, group, rotary, pairs):
+    # The newest token of each text, turned with its queries, in place or not, rows with gaps.
+    lengths = [1, 16, 17, 40, 5, 100, 33]
+    for in_place, gap, far in ((False, 0, None), (True, 5, None), (True, 0, 2 ** 20 + 1), (False, 8, 300)):
+        run_append4(t, lengths, [1] * 7, 16, 6, 3, dim, group, rotary, pairs, gap=gap, in_place=in_place, far=far)
+    run_append4(t, [70, 49, 4], [9, 17, 4], 48, 40, 8, dim, group, rotary, pairs, gap=8, in_place=True)
