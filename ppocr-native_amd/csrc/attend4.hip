@@ -23,12 +23,7 @@ __global__ __launch_bounds__(256) void kv4_attention_join(Attend4Args a, int key
   float base = fmaxf(b0, b1);
 #pragma unroll
   for (int o = 32; o; o >>= 1) base = fmaxf(base, __shfl_xor(base, o));
-  // A part's base is -infinity only where nothing of it is seen (or a seen page
-  // does not exist: then its sum is NaN, and so is the whole).
-  auto factor = [&](float bi, float li) {
-    return bi == -INFINITY ? (li == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(bi - base);
-  };
-  const float f0 = factor(b0, l0), f1 = factor(b1, l1);
+  const float f0 = __builtin_amdgcn_exp2f(b0 - base), f1 = __builtin_amdgcn_exp2f(b1 - base);
   float sum = f0 * l0 + f1 * l1;
 #pragma unroll
   for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);

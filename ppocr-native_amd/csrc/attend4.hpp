@@ -92,13 +92,16 @@ struct Rows4 {
   float qs[G];             // sums of q over a group, times 2^(e - UNIT)
   v4f o[E];                // lane's column, dim 32 c + 2 (4 quarter + r) + b in o[2 c + b][r]
   float om[G];             // this lane's share of sum P m
-  // Weights are 2^(S scale - base); base is less by `up` than the largest S scale
-  // was when it was set, and 2^up times any scale of V is at most 2^12, so that
-  // products of the two fill f16's range. Results are scaled anew only where a
-  // product passes that largest by 2^kSlack (or a scale of V `most`, a power of two
-  // above the largest so far): with each new largest it would be in most tiles.
-  static constexpr float kSlack = 3.0f;
-  float m, l, base, scale, most, up;
+  // Weights are 2^(S scale - base), base the largest S scale when it was set (before
+  // that -2^126, below all that are finite). Their products with a group's scales of V
+  // are taken times f, a power of two that brought the largest product, of all that a
+  // column has seen of the group, to 2^11 or more and below 2^12: so f16's range is a
+  // group's own, and neither another group's scale nor that of a token without weight
+  // takes bits from it. Products of 2^-11 of the largest or more keep 22 bits, smaller
+  // ones are off by 2^-35 of it. Results are scaled anew only where a weight passes
+  // 2^kSlack or a product 2^15: with each new largest it would be in most tiles.
+  static constexpr float kSlack = 3.0f, kMostF = 0x1p100f;
+  float l, base, scale, f[G];
 
   // Eight neighbouring dims of a row from d, as they are stored; past dim some
   // others of the row. EIGHTS: heads are of a multiple of 8 dims.
@@ -198,12 +201,12 @@ struct Rows4 {
       sum += __shfl_xor(sum, 32);
       qs[g] = TWO ? sum : sum * 0x1p-9f;
       om[g] = 0.0f;
+      f[g] = kMostF;
     }
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = v4f{0, 0, 0, 0};
-    m = base = -INFINITY;
-    l = most = 0.0f;
-    up = 15.0f - kSlack;
+    base = -0x1p126f;
+    l = 0.0f;
   }
 
   // A tile's codes: 16s of keys, of which this lane has row lane % 16 of K and the
@@ -221,24 +224,33 @@ struct Rows4 {
     return f;
   }
 
-  // Raises the largest product and V's largest scale to a tile's.
-  __device__ __forceinline__ void raise(float now, float large) {
-    large = fmaxf(large, __shfl_xor(large, 16));
-    large = fmaxf(large, __shfl_xor(large, 32));
-    if (large > most) {
-      const int e = min((int)(__float_as_uint(large) >> 23) - 126, 17);  // large <= 2^e
-      most = __builtin_ldexpf(1.0f, e);
-      up = 15.0f - kSlack - (float)e;
-    }
-    const float next = now == -INFINITY ? -INFINITY : fmaf(now, scale, -up);
-    const float shrink = base == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - next);
+  // Of a column's four lanes. (Rows of 16 lanes change places between two registers:
+  // a chain of waits on LDS less than shuffles, where a tile needs three of these.)
+  static __device__ __forceinline__ float largest(float v) {
+    auto two = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+    two = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
+  }
+  // Raises the base to a tile's largest S; by how much, as a 2-logarithm.
+  __device__ __forceinline__ float raise(float top) {
+    const float next = fmaxf(base, largest(top) * scale), rise = next - base, shrink = __builtin_amdgcn_exp2f(-rise);
     l *= shrink;
 #pragma unroll
-    for (int i = 0; i < E; i++) o[i] *= shrink;
-#pragma unroll
     for (int g = 0; g < G; g++) om[g] *= shrink;
-    m = now;
     base = next;
+    return rise;
+  }
+  // After that, or where a product passes 2^15: a group's results, and its f, which
+  // goes up as they went down, but no further than the tile's products allow.
+  __device__ __forceinline__ void fit(int g, float product, float rise) {
+    const int up = min((int)fminf(rise, 256.0f), 100 + 127 - (int)(__float_as_uint(f[g]) >> 23));
+    const float now = __builtin_ldexpf(f[g], up), most = largest(product) * now;
+    const int down = most > 0x1p15f ? (int)(__float_as_uint(most) >> 23) - 126 - 12 : 0;  // most < 2^(12 + down)
+    f[g] = __builtin_ldexpf(now, -down);
+    const float by = __builtin_ldexpf(__builtin_amdgcn_exp2f((float)up - rise), -down);
+#pragma unroll
+    for (int c = g * GC; c < NC && c < (g + 1) * GC; c++) o[2 * c] *= by, o[2 * c + 1] *= by;
   }
 
   // Takes in the tile in k and v, its scales and minima at `lds`. seen(key of the
@@ -298,41 +310,55 @@ struct Rows4 {
         }
       }
     }
-    float top = -INFINITY;
-    v2h wide{0, 0};
+    float top = -INFINITY, rise = 0.0f;
 #pragma unroll
-    for (int j = 0; j < L; j++) {
+    for (int j = 0; j < L; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) top = fmaxf(top, z[j][r]);
-#pragma unroll
-      for (int i = 0; i < 4 * G; i += 2) wide = __builtin_elementwise_max(wide, v2h{vs[j].of[i], vs[j].of[i + 1]});
-    }
-    const float large = (float)__builtin_elementwise_max(wide[0], wide[1]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    if (__any(fmaf(top, scale, -up) > base + kSlack || large > most)) raise(fmaxf(m, top), large);
-    const float from = base == -INFINITY ? 0.0f : base;
+    const bool higher = __any(fmaf(top, scale, -base) > kSlack);
+    if (higher) rise = raise(top);
     float p[L][4];
 #pragma unroll
     for (int j = 0; j < L; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        p[j][r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], scale, -from));
+        p[j][r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], scale, -base));
         l += p[j][r];
 #pragma unroll
         for (int g = 0; g < G; g++) om[g] = fmaf(p[j][r], (float)vm[j].of[r * G + g], om[g]);
       }
+    // Weights times scales, 16 or 24 at a time.
+    constexpr int SOME = G % 4 == 0 && L == 1 ? 4 : G % 3 == 0 ? 3 : G % 2 == 0 ? 2 : 1;
+    float w[SOME][L][4];
 #pragma unroll
     for (int g = 0; g < G; g++) {
-      // Weights times scales in two f16 parts: 22 bits. Keys r and r + 2 of a quarter side by side, as the masks
-      // leave V's; a column has its own 16s of keys and zeros for the others.
+      if (g % SOME == 0) {
+        float product[SOME] = {};
+        bool past = false;
+#pragma unroll
+        for (int i = 0; i < SOME; i++) {
+#pragma unroll
+          for (int j = 0; j < L; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+              w[i][j][r] = fmaf(p[j][r], (float)vs[j].of[r * G + g + i], 0.0f);
+              product[i] = fmaxf(product[i], w[i][j][r]);
+            }
+          past = past || product[i] * f[g + i] > 0x1p15f;
+        }
+        if (higher || __any(past)) {
+#pragma unroll
+          for (int i = 0; i < SOME; i++) fit(g + i, product[i], rise);
+        }
+      }
+      // In two f16 parts: 22 bits. Keys r and r + 2 of a quarter side by side, as the masks leave V's; a column has
+      // its own 16s of keys and zeros for the others.
       uint32_t high[L][2], low[L][2];
 #pragma unroll
       for (int j = 0; j < L; j++)
 #pragma unroll
         for (int r = 0; r < 2; r++) {
-          const float x = fmaf(p[j][r], (float)vs[j].of[r * G + g], 0.0f);
-          const float y = fmaf(p[j][r + 2], (float)vs[j].of[(r + 2) * G + g], 0.0f);
+          const float x = w[g % SOME][j][r] * f[g], y = w[g % SOME][j][r + 2] * f[g];
           const uint32_t both = pair16(x, y);
           const v2h back = __builtin_bit_cast(v2h, both);
           high[j][r] = both;
@@ -375,12 +401,14 @@ struct Rows4 {
 };
 
 // Waves that a SIMD's 512 registers a lane hold without spilling: results, q,
-// codes, the tile's products, scales and minima, and some 55 others.
+// codes, the tile's products, scales and minima, and some 55 others; four only
+// with 20 to spare (heads of 64 in one group, counted as 109: 46 us with four, 44
+// with three).
 template <int NC, int GC, bool TWO, int CP>
 constexpr int waves_a_simd4() {
   typedef Rows4<NC, GC, TWO, CP> A;
   constexpr int n = NC * (8 + (TWO ? 8 : 4) + 2 * A::H) + A::FEW + A::G * (4 * A::L + 8 * A::L) + 55;
-  return n <= 130 ? 4 : n <= 170 ? 3 : n <= 250 ? 2 : 1;
+  return n <= 105 ? 4 : n <= 170 ? 3 : n <= 250 ? 2 : 1;
 }
 
 // A key head's 16 (or fewer) query heads blockIdx.x, text blockIdx.z and part
@@ -495,7 +523,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
 #pragma unroll
       for (int r = 0; r < 4; r++)
         lds_o[wave][col][32 * c + 2 * (4 * quarter + r) + odd] =
-            fmaf(at.o[2 * c + odd][r], TWO ? (odd ? 0x1p5f : 0x1p9f) : 0x1p18f, at.om[c / GC]);
+            fmaf(at.o[2 * c + odd][r], (TWO ? (odd ? 0x1p5f : 0x1p9f) : 0x1p18f) / at.f[c / GC], at.om[c / GC]);
   __syncthreads();
   // A column's factor, and a row's sum: a wave's columns in 16 neighbouring lanes.
   {
@@ -507,8 +535,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
       return v;
     };
     base_ = all(base_, [](float x, float y) { return fmaxf(x, y); });
-    // (A base is -infinity where the column had no key; NaN where q is not finite.)
-    const float f = bw == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(bw - base_);
+    const float f = __builtin_amdgcn_exp2f(bw - base_);
     const float sum = all(f * lds_l[lane / 16][col], [](float x, float y) { return x + y; });
     __syncthreads();
     if (wave == 0) {

@@ -702,3 +702,72 @@ def test_append4_of_a_token_a_text(t, dim, group, rotary, pairs):
     for in_place, gap, far in ((False, 0, None), (True, 5, None), (True, 0, 2 ** 20 + 1), (False, 8, 300)):
         run_append4(t, lengths, [1] * 7, 16, 6, 3, dim, group, rotary, pairs, gap=gap, in_place=in_place, far=far)
     run_append4(t, [70, 49, 4], [9, 17, 4], 48, 40, 8, dim, group, rotary, pairs, gap=8, in_place=True)
+
+
+# ------------------------------------- attention: scales of V of very different sizes
+
+def check_attend4(p, lengths, q, t, scale, work=1 << 22):
+    """Attention over the cache as it is, of q [texts][heads][dim] (as stored), against 64 bits."""
+    cache = p.upload()
+    batch, heads, dim = q.shape
+    dq, dl, dy = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32)), R.on_gpu(np.zeros_like(q))
+    dw = R.on_gpu(np.full(max(work, 4), 0xFF, np.uint8))
+    print(f"4-bit attention {lengths}, heads {heads}/{p.heads} of {dim} in {p.group} type {t} scale {scale} work {work}",
+          flush=True)
+    D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, batch, heads, scale=scale, type=t,
+                    workspace=dw.addr if work else 0, workspace_bytes=work)
+    synchronize()
+    got = R.values(R.back(dy, q.dtype, q.shape), t)
+    for b, n in enumerate(lengths):
+        parts = [p.get(b, i) for i in range(n)]
+        for h in range(heads):
+            k, v = ([np.array([x[part][j][h * p.heads // heads] for x in parts]).reshape(n, dim) for j in (0, 1)]
+                    for part in (0, 1))
+            want, size, reach = W.attend4(R.values(q[b, h], t), k, v, np.ones(n, bool), scale)
+            R.close(got[b, h], want, W.attend4_bound(want, size, reach, t))
+
+
+def spread_v(p, lengths, ratio, tokens=(), group=None):
+    """V's scales `ratio` times as large for some tokens of each text, or in one group of each head; its minima 0, so
+    that outputs are sums of weights times scales times codes alone."""
+    for b, n in enumerate(lengths):
+        for i in range(n):
+            page, slot = p.place(b, i)
+            s, m = p.few()[2][page, :, slot], p.few()[3][page, :, slot]
+            large = (i in tokens) | (np.arange(p.groups) == group)
+            s[...] = s.astype(np.float64) * np.where(large, 8000.0, 8000.0 / ratio)
+            m[...] = 0
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads", [2, 6, 11])
+@pytest.mark.parametrize("ratio", [2.0 ** 16, 2.0 ** 22, 2.0 ** 26])
+def test_attend4_of_a_group_with_large_scales(t, heads, ratio):
+    # A group's bits are its own: another group of the same head has scales up to 2^26 times as large.
+    lengths = [400, 90, 33]
+    for dim, group, work in ((64, 0, 1 << 22), (64, 1, 0), (128, 2, 1 << 22)):
+        rng = np.random.default_rng(dim + group)
+        p = W.Cache4(rng, lengths, 16, 1, dim, 32, nan=True)
+        p.fill(rng, lengths)
+        spread_v(p, lengths, ratio, group=group)
+        check_attend4(p, lengths, R.stored(rng.normal(0, 1, (3, heads, dim)), t), t, dim ** -0.5, work)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads", [2, 6, 11])
+@pytest.mark.parametrize("where", [[0, 1, 200], [63, 64, 399], list(range(0, 400, 7))])
+def test_attend4_of_large_scales_without_weight(t, heads, where):
+    # Tokens whose scales are 2^26 times the others', but whose keys give them weights of e^-30 beside these (and
+    # that may come first): the others keep their bits.
+    lengths = [400, 401]
+    for group, work in ((32, 1 << 22), (0, 0)):
+        rng = np.random.default_rng(group + 3)
+        p = W.Cache4(rng, lengths, 16, 1, 64, group, nan=True)
+        p.fill(rng, lengths)
+        spread_v(p, lengths, 2.0 ** 26, tokens=where)
+        for b, n in enumerate(lengths):
+            for i in range(n):  # keys the same in all dims: the score is that times the query's sum
+                page, slot = p.place(b, i)
+                p.few()[0][page, :, slot] = 0
+                p.few()[1][page, :, slot] = -1.0 if i in where else (i % 5) / 32
+        check_attend4(p, lengths, R.stored(1 + rng.integers(0, 2, (2, heads, 64)), t), t, 20 / 64, work)
