@@ -101,7 +101,10 @@ struct Rows4 {
   // ones are off by 2^-35 of it. Results are scaled anew only where a weight passes
   // 2^kSlack or a product 2^15: with each new largest it would be in most tiles.
   static constexpr float kSlack = 3.0f, kMostF = 0x1p100f;
-  float l, base, scale, f[G];
+  // The base is near + far, one of which is 0. Below 2^24 S scale - near is rounded
+  // once; beyond, half a step of the base can be any power of two, and S scale is
+  // rounded as the base was, so that the largest has 0 and equal ones are equal.
+  float l, near, far, scale, f[G];
 
   // Eight neighbouring dims of a row from d, as they are stored; past dim some
   // others of the row. EIGHTS: heads are of a multiple of 8 dims.
@@ -205,8 +208,8 @@ struct Rows4 {
     }
 #pragma unroll
     for (int i = 0; i < E; i++) o[i] = v4f{0, 0, 0, 0};
-    base = -0x1p126f;
-    l = 0.0f;
+    near = l = 0.0f;
+    far = -0x1p126f;
   }
 
   // A tile's codes: 16s of keys, of which this lane has row lane % 16 of K and the
@@ -232,13 +235,16 @@ struct Rows4 {
     two = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return fmaxf(__uint_as_float(two[0]), __uint_as_float(two[1]));
   }
+  __device__ __forceinline__ float above_base(float z) const { return fmaf(z, scale, -near) - far; }
   // Raises the base to a tile's largest S; by how much, as a 2-logarithm.
   __device__ __forceinline__ float raise(float top) {
-    const float next = fmaxf(base, largest(top) * scale), rise = next - base, shrink = __builtin_amdgcn_exp2f(-rise);
+    const float base = near + far, next = fmaxf(base, largest(top) * scale), rise = next - base;
+    const float shrink = __builtin_amdgcn_exp2f(-rise);
     l *= shrink;
 #pragma unroll
     for (int g = 0; g < G; g++) om[g] *= shrink;
-    base = next;
+    near = fabsf(next) < 0x1p24f ? next : 0.0f;
+    far = next - near;
     return rise;
   }
   // After that, or where a product passes 2^15: a group's results, and its f, which
@@ -315,14 +321,14 @@ struct Rows4 {
     for (int j = 0; j < L; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) top = fmaxf(top, z[j][r]);
-    const bool higher = __any(fmaf(top, scale, -base) > kSlack);
+    const bool higher = __any(above_base(top) > kSlack);
     if (higher) rise = raise(top);
     float p[L][4];
 #pragma unroll
     for (int j = 0; j < L; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        p[j][r] = __builtin_amdgcn_exp2f(fmaf(z[j][r], scale, -base));
+        p[j][r] = __builtin_amdgcn_exp2f(above_base(z[j][r]));
         l += p[j][r];
 #pragma unroll
         for (int g = 0; g < G; g++) om[g] = fmaf(p[j][r], (float)vm[j].of[r * G + g], om[g]);
@@ -515,7 +521,7 @@ __global__ __launch_bounds__(64 * kWaves4, (waves_a_simd4<NC, GC, TWO, CP>())) v
   // The waves' columns, joined.
   if (bad) lds_bad = 1;
   const float l = at.total();
-  if (quarter == 0) lds_b[wave][col] = at.base, lds_l[wave][col] = l;
+  if (quarter == 0) lds_b[wave][col] = at.near + at.far, lds_l[wave][col] = l;
 #pragma unroll
   for (int c = 0; c < NC; c++)
 #pragma unroll

@@ -771,3 +771,40 @@ def test_attend4_of_large_scales_without_weight(t, heads, where):
                 p.few()[0][page, :, slot] = 0
                 p.few()[1][page, :, slot] = -1.0 if i in where else (i % 5) / 32
         check_attend4(p, lengths, R.stored(1 + rng.integers(0, 2, (2, heads, 64)), t), t, 20 / 64, work)
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads", [2, 6, 11])
+@pytest.mark.parametrize("scale", [1e4, 1e6, -3.3e7, 1e9, 7e12, 1e20, 1e30])
+def test_attend4_of_very_large_scores(t, heads, scale):
+    # Products of q with keys that f32 holds exactly, times a scale that makes scores of 10^6 and more of them: all
+    # weight goes to the keys whose product is the largest, in equal parts, wherever they lie.
+    lengths, dim = [300, 301, 40], 64
+    for work, group in ((1 << 22, 32), (0, 0)):
+        rng = np.random.default_rng(heads)
+        p = W.Cache4(rng, lengths, 16, 1, dim, group, nan=True)
+        p.fill(rng, lengths)
+        keys = [rng.integers(-3, 3, n) for n in lengths]
+        for b, n in enumerate(lengths):
+            keys[b][rng.integers(0, n, 3)] = 3
+            keys[b][rng.integers(0, n, 3)] = -4
+            for i in range(n):
+                page, slot = p.place(b, i)
+                p.few()[0][page, :, slot] = 0
+                p.few()[1][page, :, slot] = keys[b][i]
+        q = R.stored(rng.integers(1, 7, (3, heads, dim)), t)
+        cache = p.upload()
+        dq, dl, dy = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32)), R.on_gpu(np.zeros_like(q))
+        dw = R.on_gpu(np.full(max(work, 4), 0xFF, np.uint8))
+        print(f"4-bit attention, scale {scale}, heads {heads} type {t} group {group} work {work}", flush=True)
+        D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, 3, heads, scale=scale, type=t,
+                        workspace=dw.addr if work else 0, workspace_bytes=work)
+        synchronize()
+        got = R.values(R.back(dy, q.dtype, q.shape), t)
+        for b, n in enumerate(lengths):
+            best = np.nonzero(keys[b] == (keys[b].max() if scale > 0 else keys[b].min()))[0]
+            v = [p.get(b, i)[1] for i in best]
+            want = np.mean([n_ + m for n_, m in v], 0)[0]
+            size = np.mean([np.abs(n_) + np.abs(m) for n_, m in v], 0)[0]
+            for h in range(heads):  # the scores of the best are equal: no error of theirs counts
+                R.close(got[b, h], want, W.attend4_bound(want, size, 0.0, t))
