@@ -425,8 +425,8 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
 
 /* ppocr_hip_paged_attention over a cache in 4 bits, q and y of `type`. Codes,
  * scales and minima enter the sums as they are; the softmax's weights times V's
- * scales go into their products in two F16 parts (22 bits where one is 2^-11 of the
- * largest of its group or more, 2^-35 of that else), f32 queries too, 16-bit
+ * scales go into their products in two F16 parts, f32 queries too (23 bits where one
+ * is 2^-11 of the largest, of its group or query, or more; else 2^-34 of that), 16-bit
  * queries whole; with these, terms of a product are cut 2^-20 below the largest
  * query value or weight times scale of it. A text with a token of scale NaN that it sees gives NaN (in K:
  * its whole head, in V: the group's dims), a query with an infinity or NaN gives

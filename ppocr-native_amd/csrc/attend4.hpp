@@ -80,7 +80,7 @@ __device__ __forceinline__ void stream_in(uint32_t (&n)[N], const char *p) {
 
 // The state of 16 columns, a wave's worth: a lane has column lane % 16, row lane %
 // (16 / CP) of the query heads, and of each 16 keys the four of quarter lane / 16.
-// NC: 32s of a padded head; GC: those of a group; TWO: q in two f16 parts (22
+// NC: 32s of a padded head; GC: those of a group; TWO: q in two f16 parts (23
 // bits) instead of one (11 bits, all that 16-bit queries have); CP: columns a row.
 template <int NC, int GC, bool TWO, int CP>
 struct Rows4 {
@@ -97,8 +97,8 @@ struct Rows4 {
   // are taken times f, a power of two that brought the largest product, of all that a
   // column has seen of the group, to 2^11 or more and below 2^12: so f16's range is a
   // group's own, and neither another group's scale nor that of a token without weight
-  // takes bits from it. Products of 2^-11 of the largest or more keep 22 bits, smaller
-  // ones are off by 2^-35 of it. Results are scaled anew only where a weight passes
+  // takes bits from it. Products of 2^-13 of the largest or more keep 23 bits, smaller
+  // ones are off by 2^-36 of it. Results are scaled anew only where a weight passes
   // 2^kSlack or a product 2^15: with each new largest it would be in most tiles.
   static constexpr float kSlack = 3.0f, kMostF = 0x1p100f;
   // The base is near + far, one of which is 0. Below 2^24 S scale - near is rounded
@@ -357,18 +357,18 @@ struct Rows4 {
           for (int i = 0; i < SOME; i++) fit(g + i, product[i], rise);
         }
       }
-      // In two f16 parts: 22 bits. Keys r and r + 2 of a quarter side by side, as the masks leave V's; a column has
-      // its own 16s of keys and zeros for the others.
+      // In two f16 parts, each rounded to the nearest: 23 bits, and off to neither side. Keys r and r + 2 of a quarter
+      // side by side, as the masks leave V's; a column has its own 16s of keys and zeros for the others.
       uint32_t high[L][2], low[L][2];
 #pragma unroll
       for (int j = 0; j < L; j++)
 #pragma unroll
         for (int r = 0; r < 2; r++) {
           const float x = w[g % SOME][j][r] * f[g], y = w[g % SOME][j][r + 2] * f[g];
-          const uint32_t both = pair16(x, y);
-          const v2h back = __builtin_bit_cast(v2h, both);
-          high[j][r] = both;
-          low[j][r] = pair16(fmaf((float)back[0], -1.0f, x), fmaf((float)back[1], -1.0f, y));
+          const v2h first = __builtin_convertvector(v2f{x, y}, v2h);
+          const v2f rest{fmaf((float)first[0], -1.0f, x), fmaf((float)first[1], -1.0f, y)};
+          high[j][r] = __builtin_bit_cast(uint32_t, first);
+          low[j][r] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, v2h));
         }
 #pragma unroll
       for (int h = 0; h < H; h += 2) {

@@ -808,3 +808,28 @@ def test_attend4_of_very_large_scores(t, heads, scale):
             size = np.mean([np.abs(n_) + np.abs(m) for n_, m in v], 0)[0]
             for h in range(heads):  # the scores of the best are equal: no error of theirs counts
                 R.close(got[b, h], want, W.attend4_bound(want, size, 0.0, t))
+
+
+@pytest.mark.parametrize("heads", [4, 8, 16])
+@pytest.mark.parametrize("dim,group", [(64, 0), (128, 32)])
+def test_attend4_of_f32_is_not_off_to_one_side(heads, dim, group):
+    # Values that are all the same number: what is left is the weights' rounding into two F16 parts. Cut, these would
+    # be less by 2^-22 (1/2 + 1/8 + 1/32 ...) of 1 .. 2 on average, 0.92 steps of 2^-23 of the result; rounded, by
+    # nothing. An output's other roundings (its sums' over 10 tiles of a column) come to two steps, independent from
+    # text to text and head to head: the mean of 256 or more is within 4 * 2 / 16 = 0.5 steps.
+    rng = np.random.default_rng(heads)
+    lengths = [300] * 64
+    p = W.Cache4(rng, lengths, 16, 1, dim, group)
+    p.data[...] = rng.integers(0, 256, p.data.shape)
+    ks, km, vs, vm = p.few()
+    ks[...], km[...], vs[...], vm[...] = rng.uniform(0.01, 0.2, ks.shape), rng.normal(0, 1, km.shape), 0.0713, 0
+    p.plane(3)[...] = 0xFF
+    cache = p.upload()
+    q = rng.normal(0, 1, (64, heads, dim)).astype(np.float32)
+    dq, dl, dy = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32)), R.on_gpu(np.zeros_like(q))
+    print(f"4-bit attention of equal values, heads {heads} of {dim} in {group}", flush=True)
+    D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, 64, heads, scale=0.3)
+    synchronize()
+    want = 15 * float(np.float16(0.0713))
+    off = (R.back(dy, np.float32, q.shape).astype(np.float64) / want - 1) / R.STEP
+    assert abs(off.mean()) < 0.5, off.mean()
