@@ -416,9 +416,10 @@ int ppocr_hip_kv4_append(const void *q, size_t q_stride, void *q_out, size_t q_o
 /* What a cache in 4 bits holds, as rows of `type`: text b's rows starts[b] ..
  * starts[b + 1] - 1 of k and v (`rows` of heads x dim; starts NULL: one a text)
  * get the last tokens below lengths[b], for ppocr_hip_window_attention over a
- * prompt's past. Rows whose place is negative, or outside every text, are left
- * as they were; those past the table's row or in a page that does not exist
- * get NaN. */
+ * prompt's past. In F16, what a code stands for past 65504 (60 more at most) is
+ * held there. Rows whose place is negative, or outside every text, are left as
+ * they were; those past the table's row or in a page that does not exist get
+ * NaN. */
 int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const ppocr_kv4_cache *cache,
                        const int32_t *table, size_t table_width, const int32_t *lengths, const int32_t *starts,
                        size_t batch, size_t rows, int type, void *stream, char *err, size_t err_len);

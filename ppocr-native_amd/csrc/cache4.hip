@@ -337,12 +337,19 @@ __global__ __launch_bounds__(64 * kMostWaves4, EIGHTS ? 4 : 2) void kv4_append_r
   }
 }
 
+// What a code stands for, as it is read: 15 of a group that reaches f16's largest
+// value can stand for 60 more (15 half steps of a scale), which f16 rounds to
+// infinity; it is held at the largest. (NaN stays NaN.)
+template <int T>
+__device__ __forceinline__ num_t<T> put_held(float v) {
+  return Num<T>::put(T == PPOCR_F16 && v > 65504.0f ? 65504.0f : v);
+}
+
 // A wave's words of V, its lanes' words of K and their scales are asked for
 // together. F4: times the heads that a wave has in the append.
 template <int T, int LP, int F4>
 __global__ __launch_bounds__(64 * kMostWaves4) void kv4_read_rows(Read4Args a) {
   typedef num_t<T> V;
-  typedef Num<T> F;
   typedef Split4<LP, F4> S;
   __shared__ uint32_t words[kMostWaves4][S::WORDS];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64;
@@ -399,14 +406,12 @@ __global__ __launch_bounds__(64 * kMostWaves4) void kv4_read_rows(Read4Args a) {
       V k[8], v[8];
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        k[j] = F::put(fmaf((float)(held.k[pass] >> 4 * j & 15), ks, km));
-        v[j] = F::put(fmaf((float)(w >> 4 * j & 15), vs, vm));
+        k[j] = put_held<T>(fmaf((float)(held.k[pass] >> 4 * j & 15), ks, km));
+        v[j] = put_held<T>(fmaf((float)(w >> 4 * j & 15), vs, vm));
       }
       const long row = k16.row0 + token;
-      {
       store_past<V>((V *)a.k + row * a.k_stride + (long)h * dim + d, have, k);
       store_past<V>((V *)a.v + row * a.v_stride + (long)h * dim + d, have, v);
-      }
     }
     wave_sync();
   }

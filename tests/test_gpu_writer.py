@@ -833,3 +833,37 @@ def test_attend4_of_f32_is_not_off_to_one_side(heads, dim, group):
     want = 15 * float(np.float16(0.0713))
     off = (R.back(dy, np.float32, q.shape).astype(np.float64) / want - 1) / R.STEP
     assert abs(off.mean()) < 0.5, off.mean()
+
+
+# ------------------------------------------------ values next to F16's largest
+
+LARGEST = [(0.0, 65504.0), (-65504.0, 65504.0), (-65504.0, 0.0), (65000.0, 65504.0), (65504.0, 65504.0), (-3.0, 65488.0)]
+
+
+@pytest.mark.parametrize("dim,group", [(64, 0), (128, 32), (40, 32)])
+def test_read4_of_the_largest_values(dim, group):
+    # Finite rows come back finite in F16 where code 15 stands for 65520 or 65536; in BF16 and F32 as they are held.
+    rng = np.random.default_rng(dim)
+    rows = len(LARGEST)
+    p = W.Cache4(rng, [rows], 16, 2, dim, group)
+    cache = p.upload()
+    k, v = (np.stack([rng.uniform(low, high, (2, dim)) for low, high in LARGEST]).astype(np.float16) for _ in range(2))
+    for x in (k, v):  # each group has both ends
+        for i, (low, high) in enumerate(LARGEST):
+            x[i, :, ::8], x[i, :, 3::8] = low, high
+    dk, dv, dl, ds = R.on_gpu(k), R.on_gpu(v), R.on_gpu(np.array([rows], np.int32)), R.on_gpu(np.array([0, rows], np.int32))
+    print(f"4-bit read of the largest values, heads of {dim} in {group}", flush=True)
+    D.kv4_append(dk.addr, dv.addr, cache, p.gpu_table.addr, p.width, dl.addr, 1, rows, starts=ds.addr, type=D.F16)
+    for t in R.REAL:
+        out = [R.on_gpu(np.full((rows, 2, dim), 7, R.dtype(t))) for _ in range(2)]
+        D.kv4_read(out[0].addr, out[1].addr, cache, p.gpu_table.addr, p.width, dl.addr, 1, rows, starts=ds.addr, type=t)
+        synchronize()
+        for x, d in ((k, out[0]), (v, out[1])):
+            n, s, m = W.quantised(x, p.p, p.size)
+            of = np.arange(dim) // p.size
+            want = n[..., :dim] * s.astype(np.float64)[..., of] + m.astype(np.float64)[..., of]
+            assert want.max() > 65504
+            got = R.values(R.back(d, R.dtype(t), (rows, 2, dim)), t)
+            assert np.isfinite(got).all()
+            want = np.minimum(want, 65504) if t == D.F16 else want
+            R.close(got, want, R.half_step(want, t))
