@@ -429,9 +429,11 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
  * scales go into their products in two F16 parts, f32 queries too (23 bits where one
  * is 2^-11 of the largest, of its group or query, or more; else 2^-34 of that), 16-bit
  * queries whole; with these, terms of a product are cut 2^-20 below the largest
- * query value or weight times scale of it. A text with a token of scale NaN that it sees gives NaN (in K:
- * its whole head, in V: the group's dims), a query with an infinity or NaN gives
- * NaN. Into how many parts a text is split may depend on all texts' lengths.
+ * query value or weight times scale of it. A text with a token of scale NaN that
+ * it sees gives NaN (in K: its whole head, in V: the group's dims), a query with an
+ * infinity or NaN gives NaN. Results in F16 are held at 65504, as what
+ * ppocr_hip_kv4_read gives. Into how many parts a text is split may depend on all
+ * texts' lengths.
  * Everything else, and the workspace, is as there. */
 size_t ppocr_hip_kv4_attention_workspace(const ppocr_kv4_cache *cache, size_t batch, size_t heads, size_t longest);
 int ppocr_hip_kv4_attention(const void *q, size_t q_stride, const ppocr_kv4_cache *cache, const int32_t *table,

@@ -55,4 +55,15 @@ __device__ __forceinline__ Piece4 piece4(const Attend4Args &a, int keys, int eac
   return {-1, 0};
 }
 
+// A mean of values into an output of `type`. In f16 it is held at the largest, as
+// what is read of the cache is: codes can stand for 60 more. (NaN stays NaN.)
+__device__ __forceinline__ void put_at(void *p, long i, int type, float v) {
+  if (type == PPOCR_F32)
+    ((float *)p)[i] = v;
+  else if (type == PPOCR_BF16)
+    ((__bf16 *)p)[i] = (__bf16)v;
+  else
+    ((_Float16 *)p)[i] = (_Float16)(v > 65504.0f ? 65504.0f : v);
+}
+
 }  // namespace ppocr

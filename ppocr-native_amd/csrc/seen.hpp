@@ -32,14 +32,4 @@ __device__ __forceinline__ int tiles_a_part(int tiles, int each, int splits) {
   return max((tiles + splits - 1) / splits, each);
 }
 
-// A value into an output of `type`.
-__device__ __forceinline__ void put_at(void *p, long i, int type, float v) {
-  if (type == PPOCR_F32)
-    ((float *)p)[i] = v;
-  else if (type == PPOCR_BF16)
-    ((__bf16 *)p)[i] = (__bf16)v;
-  else
-    ((_Float16 *)p)[i] = (_Float16)v;
-}
-
 }  // namespace ppocr

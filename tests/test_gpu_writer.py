@@ -867,3 +867,40 @@ def test_read4_of_the_largest_values(dim, group):
             assert np.isfinite(got).all()
             want = np.minimum(want, 65504) if t == D.F16 else want
             R.close(got, want, R.half_step(want, t))
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("work", [0, 1 << 20])
+@pytest.mark.parametrize("dim,group", [(64, 0), (128, 32)])
+def test_attend4_of_the_largest_values(t, work, dim, group):
+    # Means of values that are held as 65520 or 65536: finite in F16, too.
+    rng = np.random.default_rng(dim)
+    n = len(LARGEST)
+    for lengths in ([n, 1, 2], [2000, 1, 1500]):
+        p = W.Cache4(rng, lengths, 16, 1, dim, group, nan=True)
+        p.fill(rng, lengths)
+        for b, length in enumerate(lengths):
+            for i in range(length):
+                x = np.full((1, dim), LARGEST[i % 2][1], np.float32)
+                x[:, ::8] = LARGEST[i % 2][0]
+                _, s, m = W.quantised(x, p.p, p.size)
+                page, slot = p.place(b, i)
+                p.few()[2][page, :, slot], p.few()[3][page, :, slot] = s, m
+        p.plane(3)[...] = 0xFF
+        cache = p.upload()
+        q = R.stored(rng.normal(0, 1, (3, 2, dim)), t)
+        dq, dl, dy = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32)), R.on_gpu(np.zeros_like(q))
+        dw = R.on_gpu(np.full(max(work, 4), 0xFF, np.uint8))
+        print(f"4-bit attention of the largest values, type {t} heads of {dim} in {group} work {work}", flush=True)
+        D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, 3, 2, scale=0.1, type=t,
+                        workspace=dw.addr if work else 0, workspace_bytes=work)
+        synchronize()
+        got = R.values(R.back(dy, q.dtype, q.shape), t)
+        for b, length in enumerate(lengths):
+            parts = [p.get(b, i) for i in range(length)]
+            k, v = ([np.array([x[part][j][0] for x in parts]) for j in (0, 1)] for part in (0, 1))
+            for h in range(2):
+                want, size, reach = W.attend4(R.values(q[b, h], t), k, v, np.ones(length, bool), 0.1)
+                assert want.max() > 65504 and np.isfinite(got[b, h]).all()
+                want = np.minimum(want, 65504) if t == D.F16 else want
+                R.close(got[b, h], want, W.attend4_bound(want, size, reach, t))
