@@ -362,7 +362,7 @@ __global__ __launch_bounds__(1024) void beam_choice(SelectArgs a, int lanes, Div
       return n;
     };
     // First by scores alone, then, where too many share one, by positions.
-    uint64_t low = 1, high = ordered((double)INFINITY);
+    uint64_t low = 1, high = ordered((double)INFINITY) + 1;
     Choice bound{0, 0};
     bool done = false;
     while (high - low > 1) {

@@ -306,3 +306,25 @@ def test_select_of_scores_that_32_bits_do_not_tell_apart(base):
     s.run()
     synchronize()
     s.check()
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("beams,vocab,keep", [(1, 131072, 128), (32, 20000, 128), (3, 131072, 64), (2, 300, 5)])
+def test_select_of_infinite_scores(t, beams, vocab, keep):
+    # A score of +infinity: every continuation of its beam has it, more than a workgroup lists, and the lower beam, the
+    # larger logit and the lower token decide. A beam that has ended goes on with its end token at that.
+    rng = np.random.default_rng(beams)
+    x = rng.normal(0, 2, (2, beams, vocab))
+    base = np.full((2, beams), np.inf)
+    base[1, :beams // 2] = -1
+    s = Select(x, base, keep, t)
+    s.run()
+    synchronize()
+    got = s.check()
+    assert (got[0] == np.inf).all() or beams == 2
+    ended = np.zeros((2, beams), np.uint8)
+    ended[:, 0] = 1
+    s = Select(x, base, keep, t, ended=ended, end=5)
+    s.run()
+    synchronize()
+    s.check()
