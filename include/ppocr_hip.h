@@ -485,9 +485,9 @@ typedef struct ppocr_beam_state {
  * allocator: each beam begins with pages of its own for all it may write, a
  * spare one, and appends only to the page being written. table_out and
  * spare_out overlap nothing. A copy has the page's tokens in use (in 4 bits up
- * to the next multiple of four); if the parent's page does not exist, its
- * number is taken over and nothing copied. More caches than 28 (9 in 4 bits)
- * take more than one launch. */
+ * to the next multiple of four); if the parent's page does not exist (in one of
+ * the caches), its number is taken over and nothing copied. More caches than 28
+ * (9 in 4 bits) take more than one launch. */
 int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const ppocr_kv4_cache *caches4,
                            size_t n_caches4, const ppocr_beam_state *states, size_t n_states, const int32_t *parents,
                            const int32_t *table, int32_t *table_out, size_t table_width, const int32_t *lengths,

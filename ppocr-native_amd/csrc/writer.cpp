@@ -269,9 +269,9 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
   ReorderArgs a{};
   a.rows = int(batch * beams), a.beams = int(beams), a.by_beams = Divide(a.beams), a.parents = parents;
   const bool paged = n_caches || n_caches4;
-  size_t page_size = 0;
-  // Each cache's planes, twice: counted and checked, then launched.
+  // Each cache's planes, its pages and a page's tokens, twice: counted and checked, then launched.
   Plane planes[6];
+  int pages = 0, tokens = 0, page_size = 0;
   auto planes_of = [&](size_t i, int &n) -> int {
     n = 0;
     if (n_caches4) {
@@ -282,9 +282,7 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
         const int bytes = k % 3 ? 2 * c.groups : 16 * c.nc;
         planes[n++] = Plane{c.data + at[k], c.page_stride, bytes, c.chunk, c.heads, bytes};
       }
-      a.pages = i && a.pages < c.pages ? a.pages : c.pages;
-      if (i && page_size != size_t(c.page_size)) return fail("%s: caches of pages of %zu and %d tokens", what, page_size, c.page_size);
-      page_size = size_t(c.page_size);
+      pages = c.pages, tokens = c.page_size;
     } else {
       CacheArgs c{};
       if (const int rc = cache_of(fail, what, caches + i, table, table_width, lengths, c)) return rc;
@@ -295,9 +293,7 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
                                    int(c.token_stride * size)}
                            : Plane{static_cast<char *>(p), c.page_stride * size, c.token_stride * size,
                                    c.head_stride * size, c.heads, int(c.dim * size)};
-      a.pages = i && a.pages < c.pages ? a.pages : c.pages;
-      if (i && page_size != size_t(c.page_size)) return fail("%s: caches of pages of %zu and %d tokens", what, page_size, c.page_size);
-      page_size = size_t(c.page_size);
+      pages = c.pages, tokens = c.page_size;
     }
     return 0;
   };
@@ -305,6 +301,9 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
   for (size_t i = 0; i < count; i++) {
     int n;
     if (const int rc = planes_of(i, n)) return rc;
+    if (i && tokens != page_size) return fail("%s: caches of pages of %d and %d tokens", what, page_size, tokens);
+    // Pages that all caches have: a page's copy and its place in the tables go by the same in every launch.
+    a.pages = i && a.pages < pages ? a.pages : pages, page_size = tokens;
   }
   if (paged) {
     if (!table_out || !spare || !spare_out || table_out == table || spare_out == spare)
@@ -313,7 +312,7 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
       return fail("%s: a pointer is not aligned to its type", what);
     a.table = table, a.table_out = table_out, a.table_width = long(table_width);
     a.lengths = lengths, a.spare = spare, a.spare_out = spare_out;
-    a.by_page = Divide(int(page_size)), a.whole4 = n_caches4 != 0;
+    a.by_page = Divide(page_size), a.whole4 = n_caches4 != 0;
   }
   for (size_t i = 0; i < n_states; i++) {
     const ppocr_beam_state &s = states[i];

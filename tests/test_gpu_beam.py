@@ -328,3 +328,47 @@ def test_select_of_infinite_scores(t, beams, vocab, keep):
     s.run()
     synchronize()
     s.check()
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("layers", [2, 60])
+def test_reorder_of_caches_with_fewer_pages(four, layers):
+    # A page is there if all caches have it, however many launches they take: the last layer's has fewer. What one cache
+    # copies all do, and the tables say.
+    rng = np.random.default_rng(layers)
+    batch, beams, page, heads, dim = 3, 4, 16, 2, 32
+    lengths = [40, 21, 70]
+    table, spare, pages = beams_of(rng, batch, beams, page, lengths)
+    rows, fewer = batch * beams, pages - 9
+    parents = rng.integers(0, beams, rows).astype(np.int32)
+    frm, want_table, want_spare, copies = B.reorder(parents, table, np.repeat(lengths, beams), spare, beams, page, fewer)
+    assert copies and len(copies) < len(B.reorder(parents, table, np.repeat(lengths, beams), spare, beams, page, pages)[3])
+    caches, held = [], []
+    size = D.kv4_page_bytes(page, heads, dim, 0) if four else page * heads * dim * 4
+    for i in range(layers):
+        n = fewer if i == layers - 1 else pages
+        arrays = [rng.integers(0, 256, (n, size)).astype(np.uint8) for _ in range(1 if four else 2)]
+        on = [R.on_gpu(a) for a in arrays]
+        held += list(zip(arrays, on))
+        caches.append(D.Kv4Cache(on[0].addr, n, page, heads, dim, 0) if four else
+                      D.KvCache(on[0].addr, on[1].addr, n, page, heads, dim, D.F32))
+    dp, dt, dsp = R.on_gpu(parents), R.on_gpu(table), R.on_gpu(spare)
+    dl = R.on_gpu(np.repeat(np.array(lengths, np.int32), beams))
+    ot, osp = R.on_gpu(np.full_like(table, 9)), R.on_gpu(np.full_like(spare, 9))
+    print(f"reorder, fewer pages in the last of {layers} layers, 4 bits {four}", flush=True)
+    D.beam_reorder(caches, dp.addr, dt.addr, ot.addr, table.shape[1], dl.addr, dsp.addr, osp.addr, batch, beams)
+    synchronize()
+    assert np.array_equal(R.back(ot, np.int32, table.shape), want_table)
+    assert np.array_equal(R.back(osp, np.int32, spare.shape), want_spare)
+    for a, d in held:
+        want = a.copy()
+        for src, dst, n in copies:
+            if four:  # of each head's planes the tokens in use, up to the next multiple of four
+                n, at, chunk = -(-n // 4) * 4, 0, size // heads
+                one, two = want[dst].reshape(heads, chunk), a[src].reshape(heads, chunk)
+                for part in [page * 16, page * 2, page * 2] * 2:
+                    one[:, at:at + part * n // page] = two[:, at:at + part * n // page]
+                    at += part
+            else:
+                want[dst, :n * heads * dim * 4] = a[src, :n * heads * dim * 4]
+        assert np.array_equal(R.back(d, np.uint8, a.shape), want)
