@@ -506,7 +506,7 @@ __global__ __launch_bounds__(256) void beam_reorder_rows(ReorderArgs a) {
       copy_pieces(dst + h * p.head_stride, src + h * p.head_stride, (long)tokens * p.bytes, split * 256 + threadIdx.x,
                   a.splits * 256);
   } else {
-    // A row of a head a wave at a time.
+    // A row of a head a wave at a time (at most 2^31 - 4096).
     const int lane = threadIdx.x % 64;
     for (int i = split * 4 + threadIdx.x / 64; i < tokens * p.heads; i += a.splits * 4) {
       const int token = i / p.heads, h = i - token * p.heads;

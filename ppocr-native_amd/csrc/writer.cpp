@@ -288,6 +288,9 @@ int ppocr_hip_beam_reorder(const ppocr_kv_cache *caches, size_t n_caches, const 
       if (const int rc = cache_of(fail, what, caches + i, table, table_width, lengths, c)) return rc;
       const long size = long(size_of(caches[i].type));
       const bool rows = c.head_stride == c.dim && c.token_stride == long(c.heads) * c.dim;
+      // (Where a head's tokens do not lie together, its rows are counted in 32 bits.)
+      if (!rows && c.token_stride != c.dim && caches[i].page_size * caches[i].heads > (size_t(1) << 31) - 4096)
+        return fail("%s: pages of %zu tokens of %zu heads, which do not lie together", what, caches[i].page_size, caches[i].heads);
       for (void *p : {c.k, c.v})
         planes[n++] = rows ? Plane{static_cast<char *>(p), c.page_stride * size, c.token_stride * size, 0, 1,
                                    int(c.token_stride * size)}

@@ -179,3 +179,15 @@ def test_select_workspace():
     n = D.beam_select_workspace(32, 8, 131072, 8)
     assert n % (256 * 9 * 8) == 0 and 16 <= n // (256 * 9 * 8) <= 64
     assert D.beam_select_workspace(1, 129, 100, 4) == 0 and D.beam_select_workspace(1, 1, 100, 0) == 0
+
+
+@pytest.mark.parametrize("tokens,heads,strides,refused", [
+    (1 << 16, 1 << 15, (1 << 35, 1 << 20, 16), True), (1 << 16, 1 << 15, (1 << 35, 16, 1 << 20), True),
+    (1 << 30, 2, (1 << 36, 32, 16), True), ((1 << 16) - 1, 1 << 15, (1 << 35, 1 << 20, 16), False),
+    (1 << 16, 1 << 15, (1 << 35, 8, 1 << 19), False), (1 << 16, 1 << 15, (0, 0, 0), False)])
+def test_reorder_of_very_many_heads_of_tokens(tokens, heads, strides, refused):
+    # Rows of heads that lie apart are counted in 32 bits: from 2^31 on they are refused, and others are not. (The call
+    # that is not refused ends at the legacy handle, which is.)
+    c = cache(page_size=tokens, heads=heads, dim=8, page_stride=strides[0], token_stride=strides[1], head_stride=strides[2])
+    with pytest.raises(GpuError, match="do not lie together" if refused else "handle"):
+        reorder(caches=[c], table_width=1, stream=1)
