@@ -904,3 +904,33 @@ def test_attend4_of_the_largest_values(t, work, dim, group):
                 assert want.max() > 65504 and np.isfinite(got[b, h]).all()
                 want = np.minimum(want, 65504) if t == D.F16 else want
                 R.close(got[b, h], want, W.attend4_bound(want, size, reach, t))
+
+
+@pytest.mark.parametrize("t", R.REAL)
+@pytest.mark.parametrize("heads,dim,group", [(32, 128, 64), (16, 64, 0)])
+def test_attend4_again(t, heads, dim, group):
+    # The same call gives the same bits, whatever the workspace and the output held before and whatever ran between.
+    rng = np.random.default_rng(dim)
+    lengths = [4000] + [int(x) for x in rng.integers(1, 4000, 31)]
+    p = W.Cache4(rng, lengths, 64, 8, dim, group)
+    p.data[...] = rng.integers(0, 256, p.data.shape, np.uint8)
+    ks, km, vs, vm = p.few()
+    ks[...], vs[...] = rng.uniform(0.05, 0.3, (2,) + ks.shape)
+    km[...], vm[...] = rng.normal(-2, 0.5, (2,) + km.shape)
+    cache = p.upload()
+    q = R.stored(rng.normal(0, 2, (32, heads, dim)), t)
+    dq, dl = R.on_gpu(q), R.on_gpu(np.array(lengths, np.int32))
+    size = D.kv4_attention_workspace(cache, 32, heads, 4000)
+    assert size
+    print(f"4-bit attention again, type {t} heads {heads} of {dim}", flush=True)
+    got = []
+    for i in range(6):
+        dy, dw = R.on_gpu(np.full(q.shape, i, q.dtype)), R.on_gpu(np.full(size, (0, 255, 127, 60, 1, 0)[i], np.uint8))
+        D.kv4_attention(dq.addr, cache, p.gpu_table.addr, p.width, dl.addr, dy.addr, 32, heads, scale=dim ** -0.5, type=t,
+                        longest=4000, workspace=dw.addr, workspace_bytes=size)
+        if i % 2:
+            D.kv4_read(dy.addr, dy.addr, cache, p.gpu_table.addr, p.width, dl.addr, 0, 0, type=t)
+        synchronize()
+        got.append(R.back(dy, q.dtype, q.shape).copy())
+    assert all(np.array_equal(g.view(np.uint8), got[0].view(np.uint8)) for g in got)
+    assert np.isfinite(R.values(got[0], t)).all()
