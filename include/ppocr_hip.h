@@ -321,7 +321,8 @@ int ppocr_hip_kv_append(const void *k, size_t k_stride, const void *v, size_t v_
  * passes table_width * page_size, or with a seen token in a page that does
  * not exist, gives NaN. What lies in unseen tokens does not matter; an
  * infinity in the v of a seen one gives that infinity (in F16, NaN where its
- * weight is below 2^-39 of the largest).
+ * weight is below 2^-39 of the largest). Scores, products times `scale`, are
+ * f32: past 2^29 in size (F16: 2^24) results can be wrong, or NaN.
  *
  * `longest` bounds the lengths (0: table_width * page_size); it only guides
  * how far the cache is split, and longer texts are right too. The parts are
@@ -349,7 +350,8 @@ int ppocr_hip_paged_attention(const void *q, size_t q_stride, const ppocr_kv_cac
  * dim a row, k and v: kv_heads x dim, dim up to 256, type F32, BF16 or F16.
  * What lies in keys that a query does not see does not matter to it; an
  * infinity in the v of one that it sees gives that infinity (in F16, NaN where
- * its weight is below 2^-38 of the largest). In BF16
+ * its weight is below 2^-38 of the largest). Scores past 2^29 in size (F16: 2^24)
+ * can give wrong results, or NaN. In BF16
  * and F16 the softmax's weights may be rounded to the type before the product
  * with v, as v itself is, and are then summed as rounded. */
 int ppocr_hip_window_attention(const void *q, size_t q_stride, const void *k, size_t k_stride, const void *v,
@@ -431,7 +433,8 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
  * queries whole; with these, terms of a product are cut 2^-20 below the largest
  * query value or weight times scale of it. A text with a token of scale NaN that
  * it sees gives NaN (in K: its whole head, in V: the group's dims), a query with an
- * infinity or NaN gives NaN. Results in F16 are held at 65504, as what
+ * infinity or NaN gives NaN. Scores of any size are taken: past 2^23 they are
+ * rounded to f32. Results in F16 are held at 65504, as what
  * ppocr_hip_kv4_read gives. Into how many parts a text is split may depend on all
  * texts' lengths.
  * Everything else, and the workspace, is as there. */

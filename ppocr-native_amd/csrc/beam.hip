@@ -69,10 +69,11 @@ __device__ __forceinline__ int rank_of(const float *numbers, int n, float mine, 
 // `keep` are not below, which is the `keep`-th of twice as many groups' largest,
 // gathered in LDS and ranked there. Of shuffled numbers that leaves a few times
 // `keep`; where more than LDS holds (sorted ones, or equal ones), the bound is
-// halved in on. What costs is the logits' own arithmetic, ten operations each,
-// four of them the exponential's: 256 rows of 131072 in bf16, 30 % of them ended,
-// take 17 us, 47 MB at 2.7 TB/s and 71 % of the vector units' time; four rows of 18385
-// in f32 take 4.5.
+// halved in on. What costs is arithmetic: eight instructions a value, four of them the
+// exponential's, come to 250 of a wave's 580, and the bound, the list's pushes and
+// its ranks to the others: 256 rows of 131072 in bf16, 30 % of them ended, take
+// 18 us, 47 MB at 2.6 TB/s and 80 % of the vector units' time; four rows of 18385 in
+// f32 take 4.8.
 // R: rounds of 8 values a thread. FEW: rows of fewer than 8 values.
 template <int T, int R, bool FEW>
 __global__ __launch_bounds__(kThreads) void beam_parts(SelectArgs a) {
@@ -435,7 +436,7 @@ __device__ __forceinline__ v4u piece_at(const char *p, long i) {
   __builtin_memcpy(&v, p + 16 * i, 16);
   return v;
 }
-// (As a stream: the copies of 64 rows' pages, 143 MB, take 27 us so, and 29 without.)
+// (As a stream: the copies of 64 rows' pages, 143 MB, take 26 us so, and 29 without.)
 __device__ __forceinline__ void put_piece(char *p, long i, v4u v) {
   typedef v4u __attribute__((aligned(1))) Loose;
   __builtin_nontemporal_store(v, (Loose *)(p + 16 * i));
@@ -459,9 +460,12 @@ __device__ __forceinline__ void copy_pieces(char *to, const char *from, long byt
 }
 
 // Row (a text's beam) blockIdx.y; workgroup 0 of it has its table, the next ones
-// the states, the others a split of a plane's tokens each. Memory bound (64 rows,
-// 12 layers, 143 MB: 27 us, 5.4 TB/s, where a copy has 5.2), or by the launch (4
-// rows of one layer: 3.1 us).
+// the states, the others a split of a plane's tokens each. Memory bound where a
+// page's tokens lie together (64 rows, 12 layers, 143 MB: 26 us, 5.5 TB/s, where a
+// copy has 5.2; head by head: 29), or by the launch (4 rows of one layer: 3.8 us).
+// Caches in 4 bits have two or four pieces of 16 bytes a head of some planes, for
+// 256 threads, and their heads go one after another: the same rows, 38 to 45 MB, take
+// 18 to 20 us, two launches.
 __global__ __launch_bounds__(256) void beam_reorder_rows(ReorderArgs a) {
   const int row = blockIdx.y, text = a.by_beams(row);
   const int parent = a.parents[row];

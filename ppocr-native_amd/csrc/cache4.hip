@@ -12,11 +12,13 @@
 // LDS, so that memory sees whole words. The queries have workgroups of their own;
 // they are turned at places below 0, too, where there is nothing to append.
 //
-// Memory bound where there are many tokens: four chunks of prompts (11500 tokens
-// of 32 heads of 128, 8 key heads, f16, groups of 32) are appended in 54 us, 250 MB
-// at 4.6 TB/s where a copy of as much has 5.2; all 25000 tokens of their texts are
-// read in 26 us, 125 MB at 4.8. With a token a text the chain of waits is the
-// whole: 64 take 6.2 and 4.3 us.
+// Memory bound where there are many tokens: four chunks of prompts (11344 tokens
+// of 32 heads of 128, 8 key heads, f16, groups of 32) are appended in 56 us, 247 MB
+// at 4.4 TB/s where a copy of as much has 5.2; all 22611 tokens of their texts are
+// read in 26 us, 122 MB at 4.6. With a token a text the chain of waits is the
+// whole: 64 take 6.5 and 4.5 us. Where a turned half is no multiple of eight values
+// a piece is one value: heads of 96 with 24 turned, the same chunks, take 116 us
+// for both, with 96 turned 69.
 #include <algorithm>
 
 #include "turn.hpp"
@@ -27,7 +29,7 @@ namespace {
 constexpr int kMostWaves4 = 8;
 
 // Eight values, or `have` of them, of what a kernel that follows reads: as a
-// stream, which leaves the caches to what else is written (a read of 25000
+// stream, which leaves the caches to what else is written (a read of 22611
 // tokens of 8 heads of 128 as f16: 36 us with plain stores, 27 so).
 template <class V>
 __device__ __forceinline__ void store_past(V *p, int have, const V (&v)[8]) {
@@ -464,7 +466,7 @@ hipError_t launch_append4_of(const Append4Args &a, hipStream_t s) {
 
 template <int T, int LP>
 hipError_t launch_read4(const Read4Args &a, hipStream_t s) {
-  // Four times the heads a wave where there is more than a token a text: 25000
+  // Four times the heads a wave where there is more than a token a text: 22611
   // tokens of 8 heads of 128 as f16 take 26 us instead of 32; 64 texts' newest 5.4
   // instead of 4.3.
   const dim3 grid = grid4(a.rows, a.batch, 1);
