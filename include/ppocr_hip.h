@@ -430,8 +430,8 @@ int ppocr_hip_kv4_read(void *k, size_t k_stride, void *v, size_t v_stride, const
  * scales and minima enter the sums as they are; the softmax's weights times V's
  * scales go into their products in two F16 parts, f32 queries too (23 bits where one
  * is 2^-11 of the largest, of its group or query, or more; else 2^-34 of that), 16-bit
- * queries whole; with these, terms of a product are cut 2^-20 below the largest
- * query value or weight times scale of it. A text with a token of scale NaN that
+ * queries whole down to 2^-27 of their largest value; with these, terms of a product
+ * are cut 2^-20 below the largest query value or weight times scale of it. A text with a token of scale NaN that
  * it sees gives NaN (in K: its whole head, in V: the group's dims), a query with an
  * infinity or NaN gives NaN. Scores of any size are taken: past 2^23 they are
  * rounded to f32. Results in F16 are held at 65504, as what
