@@ -409,14 +409,15 @@ struct Rows4 {
 };
 
 // Waves that a SIMD's 512 registers a lane hold without spilling: results, q,
-// codes, the tile's products, scales and minima, and some 55 others; four only
-// with 20 to spare (heads of 64 in one group, counted as 109: 46 us with four, 44
-// with three).
+// codes, the tile's products, scales and minima, and some 55 others. (Four columns
+// of 16-bit queries over one group spill with four waves: the texts above, with heads
+// of 64 and of 96, take 47 and 57 us so, and 45 and 53 with three. With more groups,
+// f32 queries or fewer columns four waves are the faster by 1 to 5 %.)
 template <int NC, int GC, bool TWO, int CP>
 constexpr int waves_a_simd4() {
   typedef Rows4<NC, GC, TWO, CP> A;
   constexpr int n = NC * (8 + (TWO ? 8 : 4) + 2 * A::H) + A::FEW + A::G * (4 * A::L + 8 * A::L) + 55;
-  return n <= 105 ? 4 : n <= 170 ? 3 : n <= 250 ? 2 : 1;
+  return n <= (A::G == 1 && CP == 4 && !TWO ? 105 : 130) ? 4 : n <= 170 ? 3 : n <= 250 ? 2 : 1;
 }
 
 // A key head's 16 (or fewer) query heads blockIdx.x, text blockIdx.z and part
